@@ -300,6 +300,69 @@ NKB_API void nkb_dots_packed_columns(uint32_t dtype, void const *a, void const *
 NKB_API int nkb_angulars_packed_noalloc(uint32_t dtype, void const *a, void const *b_packed, void *c, nk_size_t height,
                                         nk_size_t width, nk_size_t depth, nk_size_t a_stride, nk_size_t c_stride);
 
+/* ---- microscaled 4-bit floats (MXFP4) and the experts that use them ------------------------------
+ * No counterpart in the reference. A value is an e2m1 code (0 .5 1 1.5 2 3 4 6 and their negatives) times a scale that 32
+ * consecutive values of a row share, 2^(s - 127) for a scale byte s; s = 255 stands for NaN. Row-major form: two codes to a
+ * byte, the even value in the low half, ceil(depth / 2) bytes of codes and ceil(depth / 32) scale bytes per row, each with a
+ * stride of its own. Types are given by their codes: F32, F16 or BF16 for inputs, F32 or BF16 for results of products.
+ *
+ * Pointers may be host or device memory, mixed freely, as everywhere; device operands have to live on the calling thread's
+ * current GPU (a call with one that does not is refused). On failure the outputs are filled with 0xFF bytes, i.e. NaN scales
+ * and cells and ids of -1. `workspace` is device memory of at least the stated size on a 256-byte boundary that no
+ * other call uses at the same time; with NULL the calling thread's staging memory is used, which allocates on first use and is
+ * shared by everything the thread enqueues - captured graphs want a workspace of their own. The first product on each GPU
+ * allocates the device error word; make it before a capture starts.
+ *
+ * nkb_mx_quantise: per block with largest magnitude t the scale is 2^X, X = clamp(floor(log2 t) - 2, -127, 127); each value over
+ *   it is rounded to the nearest code, ties to the even code, beyond 6 to 6. A block that holds an infinity or a NaN gets scale 255
+ *   and zero codes. The unused half of the last byte of an odd depth is a zero code.
+ * nkb_mx_dequantise: the values the codes stand for (f16: rounded to nearest, beyond its range infinite).
+ * nkb_dots_pack_mxfp4: `groups` matrices of width x depth, one after the other in rows, into one blob of
+ *   nkb_dots_packed_size_mxfp4 bytes; groups = 1 is a plain packed matrix, more are the matrices of nkb_experts_packed_mxfp4.
+ * nkb_dots_packed_mxfp4: C = A . B^T in f32 sums, stored as f32 or rounded to bf16. A is row-major codes and scales; the
+ *   _quantised_ form takes a float A and quantises it first, with the same result as the two calls one after the other. Both
+ *   codes of the last byte of an odd depth take part, as for the other 4-bit types. Workspace: nkb_dots_workspace_mxfp4.
+ */
+#define NKB_DTYPE_MXFP4 (1u << 28) /* in blob headers only */
+NKB_API void nkb_mx_quantise(void const *x, uint32_t x_type, nk_size_t rows, nk_size_t depth, nk_size_t x_stride, void *codes,
+                             nk_size_t codes_stride, void *scales, nk_size_t scales_stride);
+NKB_API void nkb_mx_dequantise(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride, nk_size_t rows,
+                               nk_size_t depth, void *x, uint32_t x_type, nk_size_t x_stride);
+NKB_API nk_size_t nkb_dots_packed_size_mxfp4(nk_size_t groups, nk_size_t width, nk_size_t depth);
+NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride, nk_size_t groups,
+                                 nk_size_t width, nk_size_t depth, void *packed);
+NKB_API nk_size_t nkb_dots_workspace_mxfp4(nk_size_t height, nk_size_t depth);
+NKB_API void nkb_dots_packed_mxfp4(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride,
+                                   void const *b_packed, void *c, uint32_t c_type, nk_size_t height, nk_size_t width, nk_size_t depth,
+                                   nk_size_t c_stride, void *workspace);
+NKB_API void nkb_dots_packed_quantised_mxfp4(void const *a, uint32_t a_type, nk_size_t a_stride, void const *b_packed, void *c,
+                                             uint32_t c_type, nk_size_t height, nk_size_t width, nk_size_t depth, nk_size_t c_stride,
+                                             void *workspace);
+/* nkb_route: for every token, `top` (<= 32) of `experts` (<= 1024) and their weights.
+ *   score  s = softmax(logits) (`score` 0) or 1 / (1 + exp(-logit)) (1);  key = s + bias (f32 per expert, or NULL)
+ *   `groups` (<= 32, of equal size): a group is worth the sum of its two best keys, only the `top_groups` best stay open
+ *   ids[token, j]: the open expert with the j-th largest key, ties (of groups too) to the lower index
+ *   weights[token, j] = scale * s, or scale * s / (sum over the chosen) with `renormalise`
+ * Keys are compared in 64 bits. A logit of -infinity or NaN gives score 0 and is never chosen, a bias of -infinity or NaN only
+ * bars its expert, +infinity counts as the largest finite value. Slots left without an expert hold id -1 and weight 0.
+ * weights and ids are dense [tokens, top]. `logits` rows are `logits_stride` bytes apart.
+ * nkb_route_gradient: d(sum of weights * weights_grad) / d logits for given ids, dense f32 [tokens, experts]; ids outside
+ * [0, experts) and experts whose logit is masked get and give nothing, an id named twice counts twice. */
+NKB_API void nkb_route(void const *logits, uint32_t type, nk_size_t tokens, nk_size_t experts, nk_size_t logits_stride, float const *bias,
+                       uint32_t score, nk_size_t groups, nk_size_t top_groups, nk_size_t top, int renormalise, float scale, float *weights,
+                       int32_t *ids);
+NKB_API void nkb_route_gradient(float const *weights_grad, int32_t const *ids, void const *logits, uint32_t type, nk_size_t tokens,
+                                nk_size_t experts, nk_size_t logits_stride, uint32_t score, nk_size_t top, int renormalise, float scale,
+                                float *logits_grad);
+/* nkb_experts_packed_mxfp4: y[token, j] = quantised(x[token]) . B_{ids[token, j]}^T on a blob packed with groups = experts. With
+ * `per_slot` x holds a row per (token, j), else one per token. `weights` NULL: out has a row of `width` cells per (token, j), zero
+ * where the id lies outside [0, experts); else out[token] = sum over j, in order, of weights[token, j] * y[token, j] in f32, such
+ * slots left out. Workspace: nkb_experts_workspace_mxfp4. */
+NKB_API nk_size_t nkb_experts_workspace_mxfp4(nk_size_t tokens, nk_size_t top, nk_size_t experts, nk_size_t width, nk_size_t depth, int weighted);
+NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t x_stride, int per_slot, int32_t const *ids, nk_size_t tokens,
+                                      nk_size_t top, void const *b_packed, nk_size_t experts, nk_size_t width, nk_size_t depth,
+                                      float const *weights, void *out, uint32_t out_type, nk_size_t out_stride, void *workspace);
+
 /* ---- additions (no counterpart in the reference) -------------------------------------------- */
 /** Last error of the calling thread, "" when the last call succeeded. The string stays valid until the next call. */
 NKB_API char const *nkb_last_error(void);

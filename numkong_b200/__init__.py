@@ -17,6 +17,7 @@ or as ml_dtypes / torch low-precision dtypes.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Any, Optional, Tuple
 
 import numpy as np
@@ -30,6 +31,7 @@ __all__ = [
     "hammings_packed", "jaccards_packed", "hammings_symmetric", "jaccards_symmetric",
     "maxsim_pack", "maxsim_packed", "maxsim", "maxsims_packed", "angulars_packed_topk", "euclideans_packed_topk",
     "topk_smallest", "merge_topk", "synchronize", "set_wait_limit_ns", "set_stream", "launch_count", "last_error", "dots_compact", "cast", "moments", "set_accumulation_span",
+    "MxMatrix", "mx_quantise", "mx_dequantise", "route", "route_gradient", "experts_packed",
 ]
 
 _NUMPY_NAMES = {
@@ -176,8 +178,9 @@ class PackedMatrix:
 
     kind = "dots"
 
-    def __init__(self, buffer: Any, dtype: str, width: int, depth: int):
+    def __init__(self, buffer: Any, dtype: str, width: int, depth: int, groups: int = 1):
         self.buffer, self.dtype, self.width, self.depth = buffer, dtype, width, depth
+        self.groups = groups  # matrices of width x depth in the blob: the experts of experts_packed (mxfp4 only)
 
     @property
     def nbytes(self) -> int:
@@ -209,8 +212,13 @@ class MaxSimPackedMatrix(PackedMatrix):
         return int(getattr(lib, f"nk_maxsim_packed_size_{dtype}")(count, depth))
 
 
-def dots_pack(b: Any, dtype: Optional[str] = None) -> PackedMatrix:
-    """Packs B (width x depth, row-major) once for repeated multiplication. Mirrors nk.dots_pack."""
+def dots_pack(b: Any, dtype: Optional[str] = None, *, groups: int = 1) -> PackedMatrix:
+    """Packs B (width x depth, row-major) once for repeated multiplication. Mirrors nk.dots_pack. An MxMatrix packs as
+    "mxfp4"; `groups` then splits its rows into that many matrices for experts_packed."""
+    if isinstance(b, MxMatrix):
+        return _pack_mx(b, groups)
+    if groups != 1:
+        raise ValueError("groups are available for MxMatrix only")
     v = _View(b, dtype)
     if v.dtype not in PACKED_DTYPES:
         raise LookupError(f"no packed kernels for dtype {v.dtype!r}")
@@ -237,6 +245,8 @@ def _out_matrix(v: _View, width: int, out: Any, dtype_name: str):
 def _packed_call(op: str, a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], columns: Optional[Tuple[int, int]] = None):
     if not isinstance(packed, PackedMatrix) or packed.kind != "dots":
         raise TypeError("second argument must be a PackedMatrix produced by dots_pack")
+    if packed.dtype == "mxfp4":
+        raise TypeError(f"no {op} kernels for mxfp4")
     v = _view_like(a, dtype, packed.dtype)
     if v.depth != packed.depth:
         raise ValueError(f"depth mismatch: a has {v.depth} dimensions, packed matrix has depth {packed.depth}")
@@ -263,10 +273,18 @@ def _packed_call(op: str, a: Any, packed: PackedMatrix, out: Any, dtype: Optiona
     return obj
 
 
-def dots_packed(a: Any, packed: PackedMatrix, *, out: Any = None, dtype: Optional[str] = None, columns: Optional[Tuple[int, int]] = None):
+def dots_packed(a: Any, packed: PackedMatrix, *, out: Any = None, dtype: Optional[str] = None, columns: Optional[Tuple[int, int]] = None,
+                out_dtype: str = "f32"):
     """C = A . B^T with widening accumulation (i8->i32, u8->u32, f32->f64, else f32). Mirrors nk.dots_packed.
     `columns=(first, count)` (an addition; first a multiple of 256) computes only that range of columns of C and leaves
-    the rest of `out` untouched (nkb_dots_packed_columns)."""
+    the rest of `out` untouched (nkb_dots_packed_columns). A matrix packed as "mxfp4" takes an MxMatrix, or a float matrix
+    that is quantised first, and `out_dtype` "f32" or "bf16"."""
+    if isinstance(packed, PackedMatrix) and packed.dtype == "mxfp4":
+        if columns is not None:
+            raise ValueError("a column range is not available for mxfp4")
+        return _packed_mx(a, packed, out, dtype, out_dtype)
+    if out_dtype != "f32":
+        raise ValueError("out_dtype is available for mxfp4 only")
     return _packed_call("dots", a, packed, out, dtype, columns)
 
 
@@ -598,6 +616,251 @@ def merge_topk(values: Any, ids: Any, top: Optional[int] = None):
     return out_v[:, :top], out_i[:, :top]
 
 
+# ---- microscaled 4-bit floats, routing and the experts' products -----------------------------------------------------
+_thread = threading.local()  # .stream: what this thread gave set_stream
+
+
+class _enqueue:
+    """Around the calls below: the GPU of the tensor they work on is made current, and a thread that has not chosen a
+    stream with set_stream enqueues on torch's current one, where the tensors come from and the results go."""
+
+    def __init__(self, x: Any):
+        self.device = x.device if _is_torch(x) and x.is_cuda else None
+
+    def __enter__(self):
+        self.guard, self.switched = None, False
+        if self.device is not None:
+            import torch
+            if self.device.index != torch.cuda.current_device():
+                self.guard = torch.cuda.device(self.device)
+                self.guard.__enter__()
+            if not getattr(_thread, "stream", 0):
+                stream = torch.cuda.current_stream().cuda_stream
+                if stream:
+                    lib.nkb_set_stream(stream)
+                    self.switched = True
+
+    def __exit__(self, *_):
+        if self.switched:
+            lib.nkb_set_stream(None)
+        if self.guard is not None:
+            self.guard.__exit__(None, None, None)
+
+
+def _like(x: Any, shape: Tuple[int, ...], name: str):
+    """A new array of element type `name` where `x` lives; bf16 is uint16 storage in NumPy."""
+    if _is_torch(x):
+        import torch
+        return torch.empty(shape, dtype=getattr(torch, _CAST_TORCH[name]), device=x.device)
+    return np.empty(shape, dtype=_CAST_NUMPY[name])
+
+
+def _workspace(x: Any, nbytes: int):
+    """(buffer, pointer) of a call's workspace: a tensor of the caller's allocator for CUDA operands, none (the library's own
+    staging memory) otherwise - for host operands, and on a stream chosen with set_stream that is not torch's current one: the
+    allocator would hand the memory on when the call returns, in an order that stream does not follow."""
+    if _is_torch(x) and x.is_cuda:
+        import torch
+        if getattr(_thread, "stream", 0) not in (0, torch.cuda.current_stream(x.device).cuda_stream):
+            return None, None
+        buffer = torch.empty(nbytes + 256, dtype=torch.uint8, device=x.device)
+        return buffer, (buffer.data_ptr() + 255) // 256 * 256
+    return None, None
+
+
+def _checked(x: Any, shape: Tuple[int, ...], names: Tuple[str, ...], what: str, like: Any = None):
+    """`x` as a dense array of the given shape and one of the given types, where `like` lives."""
+    if not _is_torch(x):
+        x = np.asarray(x)
+    name = str(x.dtype).replace("torch.", "")
+    if name not in names or tuple(x.shape) != shape:
+        raise ValueError(f"{what} must be {' or '.join(names)} of shape {shape}, got {name} of shape {tuple(x.shape)}")
+    if not (x.is_contiguous() if _is_torch(x) else x.flags.c_contiguous):
+        raise ValueError(f"{what} must be contiguous")
+    if like is not None and (_is_torch(x) != _is_torch(like) or (_is_torch(x) and x.device != like.device)):
+        raise ValueError(f"{what} must live where the other operands live")
+    return x
+
+
+def _float_view(x: Any, dtype: Optional[str], what: str) -> _View:
+    v = _View(x, dtype)
+    if v.dtype not in ("f32", "f16", "bf16"):
+        raise TypeError(f"{what} takes f32, f16 or bf16, not {v.dtype!r}")
+    return v
+
+
+class MxMatrix:
+    """A matrix of microscaled 4-bit floats in row-major form: `codes` (rows x ceil(depth / 2) bytes, two e2m1 codes each, the
+    even value in the low half) and `scales` (rows x ceil(depth / 32) bytes, 2^(s - 127) for 32 values of a row, 255 = NaN)."""
+
+    def __init__(self, codes: Any, scales: Any, depth: int):
+        self.depth = int(depth)
+        c, s = _View(codes, "u8"), _View(scales, "u8")
+        if c.cols != (self.depth + 1) // 2 or s.cols != (self.depth + 31) // 32 or c.rows != s.rows:
+            raise ValueError(f"depth {self.depth} needs rows of {(self.depth + 1) // 2} code bytes and {(self.depth + 31) // 32} scale bytes")
+        if _is_torch(c.obj) != _is_torch(s.obj) or (_is_torch(c.obj) and c.obj.device != s.obj.device):
+            raise ValueError("codes and scales must live in the same place")
+        self.codes, self.scales, self.rows, self._c, self._s = c.obj, s.obj, c.rows, c, s
+
+    @property
+    def is_cuda(self) -> bool:
+        return self._c.is_cuda
+
+    def __repr__(self) -> str:
+        return f"MxMatrix(rows={self.rows}, depth={self.depth})"
+
+
+def mx_quantise(x: Any, *, dtype: Optional[str] = None) -> MxMatrix:
+    """Rounds an f32 / f16 / bf16 matrix to microscaled 4-bit floats (nkb_mx_quantise): per 32 values of a row the scale
+    2^(floor(log2(largest)) - 2), each value to the nearest code, ties to the even code, beyond 6 scales to 6. A block that
+    holds an infinity or a NaN becomes NaN."""
+    v = _float_view(x, dtype, "mx_quantise")
+    codes, scales = _like(v.obj, (v.rows, (v.cols + 1) // 2), "u8"), _like(v.obj, (v.rows, (v.cols + 31) // 32), "u8")
+    with _enqueue(v.obj):
+        lib.nkb_mx_quantise(v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, _ptr(codes), codes.shape[1], _ptr(scales), scales.shape[1])
+    check("mx_quantise")
+    return MxMatrix(codes, scales, v.cols)
+
+
+def mx_dequantise(q: MxMatrix, to_dtype: str = "f32"):
+    """The values an MxMatrix stands for, as f32, bf16 (both exact) or f16 (nkb_mx_dequantise)."""
+    if not isinstance(q, MxMatrix):
+        raise TypeError("mx_dequantise takes an MxMatrix")
+    if to_dtype not in ("f32", "f16", "bf16"):
+        raise TypeError(f"cannot write {to_dtype!r}")
+    out = _like(q.codes, (q.rows, q.depth), to_dtype)
+    with _enqueue(q.codes):
+        lib.nkb_mx_dequantise(q._c.ptr, q._c.stride, q._s.ptr, q._s.stride, q.rows, q.depth, _ptr(out), DTYPE_CODES[to_dtype],
+                              q.depth * DTYPE_BYTES[to_dtype])
+    check("mx_dequantise")
+    return out
+
+
+def _pack_mx(b: MxMatrix, groups: int) -> PackedMatrix:
+    groups = int(groups)
+    if groups < 1 or b.rows % groups:
+        raise ValueError(f"{b.rows} rows do not make {groups} groups of equal size")
+    width = b.rows // groups
+    nbytes = int(lib.nkb_dots_packed_size_mxfp4(groups, width, b.depth))
+    buf = _like(b.codes, (nbytes,), "u8")
+    with _enqueue(b.codes):
+        lib.nkb_dots_pack_mxfp4(b._c.ptr, b._c.stride, b._s.ptr, b._s.stride, groups, width, b.depth, _ptr(buf))
+    check("dots_pack")
+    return PackedMatrix(buf, "mxfp4", width, b.depth, groups)
+
+
+def _mx_result(x: Any, rows: int, width: int, out: Any, out_dtype: str):
+    """(array, stride in bytes) of a product's result."""
+    if out_dtype not in ("f32", "bf16"):
+        raise TypeError(f"results are f32 or bf16, not {out_dtype!r}")
+    if out is None:
+        return _like(x, (rows, width), out_dtype), width * DTYPE_BYTES[out_dtype]
+    v = _View(out, out_dtype)
+    if (v.rows, v.cols) != (rows, width) or str(v.obj.dtype).replace("torch.", "") not in ("float32", "bfloat16", "uint16"):
+        raise ValueError("out has the wrong shape or cell type")
+    if v.is_cuda and (not _is_torch(x) or x.device != v.obj.device):
+        raise ValueError("out must live where the other operands live")
+    return v.obj, v.stride
+
+
+def _packed_mx(a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], out_dtype: str):
+    if packed.groups != 1:
+        raise ValueError("a matrix packed in groups is multiplied with experts_packed")
+    v = a if isinstance(a, MxMatrix) else _float_view(a, dtype, "a product with mxfp4")
+    depth = v.depth
+    if depth != packed.depth:
+        raise ValueError(f"depth mismatch: a has {depth} dimensions, packed matrix has depth {packed.depth}")
+    x = v.codes if isinstance(v, MxMatrix) else v.obj
+    result, stride = _mx_result(x, v.rows, packed.width, out, out_dtype)
+    workspace, ws = _workspace(x, lib.nkb_dots_workspace_mxfp4(v.rows, depth))
+    with _enqueue(x):
+        if isinstance(v, MxMatrix):
+            lib.nkb_dots_packed_mxfp4(v._c.ptr, v._c.stride, v._s.ptr, v._s.stride, _ptr(packed.buffer), _ptr(result), DTYPE_CODES[out_dtype],
+                                      v.rows, packed.width, depth, stride, ws)
+        else:
+            lib.nkb_dots_packed_quantised_mxfp4(v.ptr, DTYPE_CODES[v.dtype], v.stride, _ptr(packed.buffer), _ptr(result),
+                                                DTYPE_CODES[out_dtype], v.rows, packed.width, depth, stride, ws)
+    check("dots_packed")
+    return result
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route(logits: Any, top: int, *, bias: Any = None, score: str = "softmax", groups: int = 1, top_groups: Optional[int] = None,
+          renormalise: bool = True, scale: float = 1.0, dtype: Optional[str] = None):
+    """The `top` experts of every token and their weights, from its logits (nkb_route): (weights f32, ids int32), both
+    [tokens, top]. Scores are the softmax or the sigmoid of the logits; `bias` (f32 per expert) is added for the selection
+    only; with `groups` a group is worth the sum of its two best keys and only the `top_groups` best are open (default: all).
+    Best first, ties to the lower index. Weights are the scores, over their sum with `renormalise`, times `scale`. Logits of
+    -inf or NaN are never chosen; slots that find no expert hold id -1 and weight 0."""
+    v = _float_view(logits, dtype, "route")
+    if score not in _SCORES:
+        raise ValueError(f"score is 'softmax' or 'sigmoid', not {score!r}")
+    if bias is not None:
+        bias = _checked(bias, (v.cols,), ("float32",), "bias", v.obj)
+    weights, ids = _like(v.obj, (v.rows, int(top)), "f32"), _like(v.obj, (v.rows, int(top)), "i32")
+    with _enqueue(v.obj):
+        lib.nkb_route(v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, None if bias is None else _ptr(bias), _SCORES[score], groups,
+                      groups if top_groups is None else top_groups, top, int(renormalise), scale, _ptr(weights), _ptr(ids))
+    check("route")
+    return weights, ids
+
+
+def route_gradient(weights_grad: Any, ids: Any, logits: Any, *, score: str = "softmax", renormalise: bool = True, scale: float = 1.0,
+                   dtype: Optional[str] = None):
+    """Gradient of route's weights with respect to the logits, f32 [tokens, experts], for the incoming `weights_grad` (f32) and
+    the `ids` route chose (nkb_route_gradient). The choice itself, and with it the bias, has no gradient."""
+    v = _float_view(logits, dtype, "route_gradient")
+    if score not in _SCORES:
+        raise ValueError(f"score is 'softmax' or 'sigmoid', not {score!r}")
+    top = int(ids.shape[-1])
+    ids = _checked(ids, (v.rows, top), ("int32",), "ids", v.obj)
+    weights_grad = _checked(weights_grad, (v.rows, top), ("float32",), "weights_grad", v.obj)
+    grad = _like(v.obj, (v.rows, v.cols), "f32")
+    with _enqueue(v.obj):
+        lib.nkb_route_gradient(_ptr(weights_grad), _ptr(ids), v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, _SCORES[score], top,
+                               int(renormalise), scale, _ptr(grad))
+    check("route_gradient")
+    return grad
+
+
+def experts_packed(x: Any, ids: Any, packed: PackedMatrix, *, weights: Any = None, out: Any = None, dtype: Optional[str] = None,
+                   out_dtype: str = "f32"):
+    """Every token's products with its experts (nkb_experts_packed_mxfp4). `packed` holds one matrix per expert
+    (dots_pack(..., groups=experts)), `ids` (int32, [tokens, top]) names them, ids outside the experts none. `x` is
+    [tokens, depth], or [tokens, top, depth] with a row of its own for every choice; it is quantised to mxfp4 first.
+    Returns [tokens, top, width], rows without an expert zero, or with `weights` (f32, [tokens, top]) the weighted sum over a
+    token's choices, [tokens, width]."""
+    if not isinstance(packed, PackedMatrix) or packed.dtype != "mxfp4":
+        raise TypeError("experts_packed needs a matrix packed from an MxMatrix with groups")
+    if not _is_torch(ids):
+        ids = np.asarray(ids)
+    if len(ids.shape) != 2:
+        raise ValueError("ids must be [tokens, top]")
+    tokens, top = (int(n) for n in ids.shape)
+    per_slot = len(x.shape) == 3
+    if per_slot and tuple(x.shape[:2]) != (tokens, top) or not per_slot and x.shape[0] != tokens:
+        raise ValueError(f"x must be [{tokens}, depth] or [{tokens}, {top}, depth]")
+    v = _float_view(x.reshape(tokens * top, x.shape[2]) if per_slot else x, dtype, "experts_packed")
+    if v.depth != packed.depth:
+        raise ValueError(f"depth mismatch: x has {v.depth} dimensions, packed matrices have depth {packed.depth}")
+    ids = _checked(ids, (tokens, top), ("int32",), "ids", v.obj)
+    if weights is not None:
+        weights = _checked(weights, (tokens, top), ("float32",), "weights", v.obj)
+    rows = tokens if weights is not None else tokens * top
+    if out is not None and weights is None:
+        out = _checked(out, (tokens, top, packed.width), ("float32", "bfloat16", "uint16"), "out", v.obj).reshape(rows, packed.width)
+    result, stride = _mx_result(v.obj, rows, packed.width, out, out_dtype)
+    workspace, ws = _workspace(v.obj, lib.nkb_experts_workspace_mxfp4(tokens, top, packed.groups, packed.width, v.depth, int(weights is not None)))
+    with _enqueue(v.obj):
+        lib.nkb_experts_packed_mxfp4(v.ptr, DTYPE_CODES[v.dtype], v.stride, int(per_slot), _ptr(ids), tokens, top, _ptr(packed.buffer),
+                                     packed.groups, packed.width, v.depth, None if weights is None else _ptr(weights), _ptr(result),
+                                     DTYPE_CODES[out_dtype], stride, ws)
+    check("experts_packed")
+    return result if weights is not None else result.reshape(tokens, top, packed.width)
+
+
 def synchronize() -> int:
     """Waits for this thread's stream; returns the device error word (0 = healthy) and clears what it reports."""
     return int(lib.nkb_synchronize())
@@ -609,6 +872,7 @@ def set_wait_limit_ns(site: int, nanoseconds: int) -> None:
 
 
 def set_stream(cuda_stream: int) -> None:
+    _thread.stream = int(cuda_stream or 0)
     lib.nkb_set_stream(ctypes.c_void_p(cuda_stream))
 
 

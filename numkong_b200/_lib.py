@@ -93,6 +93,22 @@ def _load() -> ctypes.CDLL:
     lib.nkb_multicast_store.restype, lib.nkb_multicast_store.argtypes = ctypes.c_int, [vp, vp, sz, ctypes.c_int]
     lib.nkb_peer_barrier.restype = ctypes.c_int
     lib.nkb_peer_barrier.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int, ctypes.c_uint32]
+    u32, i32, f32 = ctypes.c_uint32, ctypes.c_int, ctypes.c_float
+    for name, result, arguments in (
+        ("nkb_mx_quantise", None, [vp, u32, sz, sz, sz, vp, sz, vp, sz]),
+        ("nkb_mx_dequantise", None, [vp, sz, vp, sz, sz, sz, vp, u32, sz]),
+        ("nkb_dots_packed_size_mxfp4", sz, [sz, sz, sz]),
+        ("nkb_dots_pack_mxfp4", None, [vp, sz, vp, sz, sz, sz, sz, vp]),
+        ("nkb_dots_workspace_mxfp4", sz, [sz, sz]),
+        ("nkb_dots_packed_mxfp4", None, [vp, sz, vp, sz, vp, vp, u32, sz, sz, sz, sz, vp]),
+        ("nkb_dots_packed_quantised_mxfp4", None, [vp, u32, sz, vp, vp, u32, sz, sz, sz, sz, vp]),
+        ("nkb_route", None, [vp, u32, sz, sz, sz, vp, u32, sz, sz, sz, i32, f32, vp, vp]),
+        ("nkb_route_gradient", None, [vp, vp, vp, u32, sz, sz, sz, u32, sz, i32, f32, vp]),
+        ("nkb_experts_workspace_mxfp4", sz, [sz, sz, sz, sz, sz, i32]),
+        ("nkb_experts_packed_mxfp4", None, [vp, u32, sz, i32, vp, sz, sz, vp, sz, sz, sz, vp, vp, u32, sz, vp]),
+    ):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = result, arguments
     return lib
 
 

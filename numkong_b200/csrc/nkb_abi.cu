@@ -100,6 +100,11 @@ void release_pins() {
     t_ctx.pins.clear();
 }
 
+ThreadCtx::~ThreadCtx() { release_pins(); }
+
+} // namespace
+
+// ---------------------------------------------------------------- helpers shared with other host files
 uint64_t fresh_nonce() {
     uint64_t t = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count();
     uint64_t c = g_nonce_counter.fetch_add(1) + 1;
@@ -107,12 +112,6 @@ uint64_t fresh_nonce() {
     x ^= x >> 31; x *= 0xBF58476D1CE4E5B9ull; x ^= x >> 29;
     return x ? x : 1;
 }
-
-ThreadCtx::~ThreadCtx() { release_pins(); }
-
-} // namespace
-
-// ---------------------------------------------------------------- helpers shared with other host files
 void set_error(const char *fmt, const char *detail) {
     char buf[512];
     std::snprintf(buf, sizeof buf, fmt, detail ? detail : "");
@@ -242,13 +241,22 @@ const uint8_t *resident_blob(const void *blob, MemKind kind, uint32_t magic, uin
         if (reinterpret_cast<uintptr_t>(blob) & 15u) { set_error("packed blob in device memory must be 16-byte aligned%s", ""); return nullptr; }
         return static_cast<const uint8_t *>(blob);
     }
+    const PackedGeometry g = packed_geometry(dtype, rows, depth);
+    return resident_blob_of_size(blob, kind, magic, dtype, rows, depth, g.total_bytes, header_out);
+}
+
+const uint8_t *resident_blob_of_size(const void *blob, MemKind kind, uint32_t magic, uint32_t dtype, uint64_t rows,
+                                     uint64_t depth, uint64_t total_bytes, PackedHeader *header_out) {
+    if (kind == kMemDevice) {
+        if (reinterpret_cast<uintptr_t>(blob) & 15u) { set_error("packed blob in device memory must be 16-byte aligned%s", ""); return nullptr; }
+        return static_cast<const uint8_t *>(blob);
+    }
     PackedHeader h;
     std::memcpy(&h, blob, sizeof h);
     if (h.magic != magic) { set_error("packed blob was not produced by the matching pack function of this library%s", ""); return nullptr; }
     if (h.dtype != dtype) { set_error("packed blob holds a different element type%s", ""); return nullptr; }
     if (h.rows != rows || h.depth != depth) { set_error("packed blob was packed for a different width/depth%s", ""); return nullptr; }
-    PackedGeometry g = packed_geometry(dtype, rows, depth);
-    if (h.total_bytes != g.total_bytes) { set_error("packed blob header is inconsistent%s", ""); return nullptr; }
+    if (h.total_bytes != total_bytes) { set_error("packed blob header is inconsistent%s", ""); return nullptr; }
     if (header_out) *header_out = h;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -281,6 +289,10 @@ void remember_blob(uint64_t nonce, uint64_t bytes, void *dev_ptr) {
 }
 
 __global__ void write_header_kernel(PackedHeader *dst, PackedHeader h) { *dst = h; }
+cudaError_t launch_write_header(void *blob, const PackedHeader &h, cudaStream_t stream) {
+    write_header_kernel<<<1, 1, 0, stream>>>(static_cast<PackedHeader *>(blob), h);
+    return cudaGetLastError();
+}
 
 // Brings a strided matrix into device memory that TMA can address (16-byte aligned base and pitch).
 // Returns the device pointer and pitch; uses `slot` when a copy is needed.
@@ -377,8 +389,7 @@ void pack_impl(uint32_t magic, uint32_t dt, const void *b, uint64_t rows, uint64
         ok = cuda_ok(cudaMemsetAsync(dev_blob + g.payload_offset, 0, g.total_bytes - g.payload_offset, stream), "clear blob");
     }
     if (ok) {
-        write_header_kernel<<<1, 1, 0, stream>>>(reinterpret_cast<PackedHeader *>(dev_blob), h);
-        ok = cuda_ok(cudaGetLastError(), "header kernel");
+        ok = cuda_ok(launch_write_header(dev_blob, h, stream), "header kernel");
         g_launches++;
     }
     if (out_kind == kMemHost) {

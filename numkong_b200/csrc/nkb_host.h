@@ -33,7 +33,13 @@ void fill_error_output(void *out, MemKind kind, uint64_t rows, uint64_t row_byte
 
 const uint8_t *resident_blob(const void *blob, MemKind kind, uint32_t magic, uint32_t dtype, uint64_t rows,
                              uint64_t depth, PackedHeader *header_out);
+// The same for a blob whose size the caller knows from its own geometry (microscaled blobs).
+const uint8_t *resident_blob_of_size(const void *blob, MemKind kind, uint32_t magic, uint32_t dtype, uint64_t rows,
+                                     uint64_t depth, uint64_t total_bytes, PackedHeader *header_out);
 void remember_blob(uint64_t nonce, uint64_t bytes, void *dev_ptr);
+uint64_t fresh_nonce();
+// Writes a blob's header on the stream.
+cudaError_t launch_write_header(void *blob, const PackedHeader &h, cudaStream_t stream);
 const void *resident_matrix(const void *src, MemKind kind, uint64_t rows, uint64_t row_bytes, uint64_t stride,
                             int slot, int piece_mode, uint64_t *pitch_out);
 

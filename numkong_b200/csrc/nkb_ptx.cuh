@@ -242,6 +242,41 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t 
 #undef NKB_UMMA_ASM
 }
 
+// ---------------------------------------------------------------- microscaled operands (kind::mxf4, one 2^X scale per 32 values)
+// 32-bit instruction descriptor of the block-scaled kinds (dense, K-major A and B, K = 64):
+//   [4,6) byte of B's scale word this step begins at, [7,10) A format (1 = e2m1), [10,12) B format (1 = e2m1),
+//   [17,23) N >> 3, [23] scale type (1 = power of two), [24,29) M >> 4, [29,31) byte of A's scale word.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t m, uint32_t n, uint32_t scale_byte) {
+    return (scale_byte << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (scale_byte << 29);
+}
+// D[128 x N] (+)= A . B^T over 64 values of depth. `a_scales` / `b_scales`: TMEM columns whose 32-bit cells hold four
+// consecutive scales of a row, rows 32 i .. 32 i + 31 in the lanes of column i (the same in every 32-lane quarter).
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                          uint32_t b_scales, uint32_t accumulate) {
+#define NKB_UMMA_MX_ASM(GROUP)                                                                                  \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                               \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" \
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory")
+    if constexpr (kCtaGroup == 1) NKB_UMMA_MX_ASM("1");
+    else NKB_UMMA_MX_ASM("2");
+#undef NKB_UMMA_MX_ASM
+}
+// Descriptor of a 512-byte scale tile in shared memory: 32 rows of 16 bytes, no swizzle, eight-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
+}
+// Copies one scale tile to four TMEM columns, into all four 32-lane quarters. Runs in order with the MMAs the same thread issues.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (kCtaGroup == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
