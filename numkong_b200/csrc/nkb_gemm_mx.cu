@@ -22,6 +22,7 @@ constexpr int kBM = 128;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kStepBytes = 32;       // bytes of depth (64 values) one MMA consumes
+constexpr uint32_t kMxChunkLines = kMxChunkBytes / 128;  // a chunk as rows of 128 bytes: 128 of codes, 8 of scales
 constexpr uint32_t kGroupM = 8;      // row tiles walked before the next column tile
 
 struct MxGemmDev {
@@ -33,6 +34,9 @@ struct MxGemmDev {
     uint32_t group_blocks;           // row blocks of 128 per packed matrix
     const MxRowTile *tiles;
     const int32_t *tile_count, *row_dest;
+    uint32_t a_row_major;            // A's codes are read from the caller's rows, only its scales are in tile form
+    const uint8_t *a_scales;         // scale tiles of A's first chunk, and the bytes from one chunk's to the next
+    uint64_t a_scale_step;
     unsigned int *error_word;
     uint32_t wait_us[kWaitSites];
 };
@@ -258,6 +262,294 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// CTA pairs (cta_group::2): two CTAs on neighbouring SMs share a 256 x 256 tile. Each loads its own 128 rows of A and half of
+// B's rows; the leader issues. All loads count on the leader's barriers, hence tensor maps: chunks seen as rows of 128 bytes. Every
+// CTA applies the scales of all of B's rows to its own half of the accumulator.
+//
+// TMEM holds two accumulators of 256 columns and the scales by letting the accumulators overlap: [0, 256) and
+// [512 - scales - 256, 512 - scales). The epilogue reads the columns they share first and then lets the next tile's MMAs
+// start, so they wait for a part of a read-out instead of all of it.
+//
+// The scales reach TMEM from registers: four warps per CTA, one for each 32-lane quarter, load a chunk's scale tiles two chunks
+// ahead and store them (tcgen05.st) beside the MMAs. tcgen05.cp, which the single-CTA kernel uses, runs in the queue of the MMAs and
+// costs them about 46 cycles a tile, six tiles a chunk: 253 us against 215 without any at 8192 x 8192 x 8192.
+constexpr int kPairStages = 5;
+constexpr int kPairScaleWarps = 4;
+constexpr int kPairThreads = kThreads + 32 * kPairScaleWarps;
+constexpr int kPairScaleCols = 24;                                // 8 for 128 rows of A, 16 for 256 of B
+constexpr int kPairSecond = 512 - 2 * kPairScaleCols - 256;       // first column of the second accumulator; two chunks' scales behind it
+constexpr int kPairBOffset = kBM * 128;
+constexpr int kPairStageBytes = 2 * kBM * 128;                    // A codes, B codes
+constexpr int kPairBarrierOffset = kPairStages * kPairStageBytes;
+constexpr int kPairStagingPitch = 144;
+constexpr int kPairStagingOffset = kPairBarrierOffset + 256;
+constexpr int kPairSmem = kPairStagingOffset + kEpilogueWarps * 32 * kPairStagingPitch + 1024;
+static_assert(kPairSecond >= 256 - 64, "the shared columns are the last / first 64 of the two accumulators at most");
+
+struct PairMaps {
+    CUtensorMap a, b;
+};
+
+// The (tile, depth block) sequence of one pair.
+struct PairWalk {
+    uint32_t tile, kb, mt, nt;
+    __device__ PairWalk(const MxGemmDev &p, uint32_t pair) : tile(pair), kb(0), mt(0), nt(0) { if (valid(p)) tile_coords(tile, p.tiles_m, p.tiles_n, mt, nt); }
+    __device__ bool valid(const MxGemmDev &p) const { return tile < p.tiles_m * p.tiles_n; }
+    __device__ void next(const MxGemmDev &p, uint32_t num_pairs) {
+        if (++kb < p.kblocks) return;
+        kb = 0;
+        tile += num_pairs;
+        if (valid(p)) tile_coords(tile, p.tiles_m, p.tiles_n, mt, nt);
+    }
+};
+
+template <bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
+    constexpr int kStages = kPairStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bar_base = smem_base + kPairBarrierOffset;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * kStages + a); };
+    auto scale_bar = [&](uint32_t b) { return bar_base + 8u * (2 * kStages + 2 + b); };  // a chunk's scales are in TMEM of both CTAs
+    const uint32_t shared_read_bar = bar_base + 8u * (2 * kStages + 4);  // the tile before is read, of this one the shared columns
+    const uint32_t drain_bar = bar_base + 8u * (2 * kStages + 5);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kPairBarrierOffset + 8 * (2 * kStages + 6));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const uint32_t tiles_m = p.tiles_m, num_tiles = tiles_m * p.tiles_n;
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&maps.a);
+        prefetch_tensormap(&maps.b);
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(scale_bar(a), 2 * kPairScaleWarps); }
+        mbar_init(shared_read_bar, 2 * kEpilogueWarps);
+        mbar_init(drain_bar, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc<2>(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+        tmem_relinquish<2>();
+    }
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0, issued = 0;
+            bool ok = true;
+            for (PairWalk w(p, pair); w.valid(p); w.next(p, num_pairs)) {
+                if (!mbar_wait<true>(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
+                const uint32_t dst = smem_base + stage * kPairStageBytes, full = map_to_cta(full_bar(stage), 0);
+                if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * kPairStageBytes);
+                const uint32_t a_block = w.mt * 2u + rank, b_block = w.nt * 2u + rank;
+                if (p.a_row_major) tma_load_2d_pair(dst, &maps.a, (int)(w.kb * 128u), (int)(a_block * kBM), full);
+                else tma_load_2d_pair(dst, &maps.a, 0, (int)((a_block * p.kblocks + w.kb) * kMxChunkLines), full);
+                tma_load_2d_pair(dst + kPairBOffset, &maps.b, 0, (int)((b_block * p.kblocks + w.kb) * kMxChunkLines), full);
+                ++issued;
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) {
+                // Both CTAs' copies count on the leader's barriers: the leader waits for them, the follower sleeps (its last
+                // copy is at least one wait limit old, and neither CTA retires before the cluster barrier).
+                if (rank == 0) {
+                    int s = stage;
+                    uint32_t ph = phase;
+                    for (uint32_t i = 0; i < issued && i < (uint32_t)kStages; ++i) {
+                        if (s == 0) { s = kStages; ph ^= 1u; }
+                        --s;
+                        if (!mbar_wait<true>(full_bar(s), ph, 6, p.error_word, p.wait_us[6])) break;
+                    }
+                } else {
+                    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int stage = 0;
+            uint32_t phase = 0, seq = 0, chunk = 0;
+            bool ok = true;
+            for (uint32_t tile = pair; tile < num_tiles && ok; tile += num_pairs, ++seq) {
+                if (seq > 0 && !mbar_wait<true>(shared_read_bar, (seq - 1u) & 1u, 2, p.error_word, p.wait_us[2])) { ok = false; break; }
+                tc_fence_after_sync();
+                const uint32_t buf = seq & 1u, d_tmem = tmem_base + buf * kPairSecond;
+                for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++chunk) {
+                    if (!mbar_wait<true>(scale_bar(chunk & 1u), (chunk >> 1) & 1u, 3, p.error_word, p.wait_us[3]) ||
+                        !mbar_wait<true>(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint32_t src = smem_base + stage * kPairStageBytes;
+                    const uint64_t a_desc = make_smem_desc_sw128(src), b_desc = make_smem_desc_sw128(src + kPairBOffset);
+                    const uint32_t scales_a = tmem_base + kPairSecond + 256 + (chunk & 1u) * kPairScaleCols, scales_b = scales_a + 8;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_mxf4<2>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(256, 256, (k & 1) * 2), scales_a + (k >> 1) * 4,
+                                     scales_b + (k >> 1) * 8, (kb | (uint32_t)k) != 0u);
+                    umma_commit_pair(empty_bar(stage), 3);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) umma_commit_pair(tmem_full_bar(buf), 3);
+            }
+            umma_commit_pair(drain_bar, 1);
+            mbar_wait<true>(drain_bar, 0u, 5, p.error_word, p.wait_us[5]);
+        }
+    } else if (warp >= 2 + kEpilogueWarps) {
+        // ------------------------------------------------------------ scales: this warp's 32-lane quarter of TMEM
+        const uint32_t column = tmem_base + (((uint32_t)warp & 3u) * 32u << 16) + kPairSecond + 256;
+        const uint32_t a_last = (p.m + kBM - 1) / kBM - 1, b_last = p.group_blocks - 1;
+        // Lane r of every quarter holds line r of each tile: A for both halves of the chunk's depth, B for both halves of its rows.
+        auto load = [&](const PairWalk &w, uint4 (&r)[6]) {
+            const uint64_t a_chunk = (uint64_t)min(w.mt * 2u + rank, a_last) * p.kblocks + w.kb;
+            const uint4 *a = reinterpret_cast<const uint4 *>(p.a_scales + a_chunk * p.a_scale_step) + lane;
+            r[0] = __ldg(a);
+            r[1] = __ldg(a + 32);
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                const uint64_t b_chunk = (uint64_t)min(w.nt * 2u + j, b_last) * p.kblocks + w.kb;
+                const uint4 *b = reinterpret_cast<const uint4 *>(p.b_chunks + b_chunk * kMxChunkBytes + kMxCodeBytes) + lane;
+                r[2 + j] = __ldg(b);
+                r[4 + j] = __ldg(b + 32);
+            }
+        };
+        uint32_t chunk = 0;
+        int freed = 0;            // stage of the chunk whose scales are overwritten next
+        uint32_t freed_phase = 0;
+        auto store = [&](const uint4 (&r)[6]) {
+            if (chunk >= 2) {  // the MMAs of two chunks ago have read theirs
+                if (!__all_sync(0xffffffffu, mbar_wait<true>(empty_bar(freed), freed_phase, 2, p.error_word, p.wait_us[2]))) return false;
+                if (++freed == kStages) { freed = 0; freed_phase ^= 1u; }
+                tc_fence_after_sync();
+            }
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const uint32_t w[8] = {r[2 * i].x, r[2 * i].y, r[2 * i].z, r[2 * i].w, r[2 * i + 1].x, r[2 * i + 1].y, r[2 * i + 1].z, r[2 * i + 1].w};
+                tmem_st_32x8(column + (chunk & 1u) * kPairScaleCols + i * 8, w);
+            }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(scale_bar(chunk & 1u), 0));
+            ++chunk;
+            return true;
+        };
+        PairWalk ahead(p, pair);
+        uint4 even[6], odd[6];
+        bool has_even = ahead.valid(p), has_odd = false;
+        if (has_even) { load(ahead, even); ahead.next(p, num_pairs); }
+        has_odd = ahead.valid(p);
+        if (has_odd) { load(ahead, odd); ahead.next(p, num_pairs); }
+        while (has_even) {
+            if (!store(even)) break;
+            if ((has_even = ahead.valid(p))) { load(ahead, even); ahead.next(p, num_pairs); }
+            if (!has_odd || !store(odd)) break;
+            if ((has_odd = ahead.valid(p))) { load(ahead, odd); ahead.next(p, num_pairs); }
+        }
+    } else {
+        const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
+        uint8_t *staging = smem_gen + kPairStagingOffset + (warp - 2) * 32 * kPairStagingPitch;
+        uint32_t seq = 0;
+        for (uint32_t tile = pair; tile < num_tiles; tile += num_pairs, ++seq) {
+            uint32_t mt, nt;
+            tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+            const uint32_t buf = seq & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait<true>(tmem_full_bar(buf), (seq >> 1) & 1u, 4, p.error_word, p.wait_us[4]))) break;
+            tc_fence_after_sync();
+            const uint32_t row = mt * 256u + rank * 128u + quarter * 32u + lane;
+            const int64_t dest = row < p.m ? (int64_t)row : -1;
+            // 64 columns at a time. Those shared with the other accumulator - the last of the first, the first of the second - come first.
+            const uint32_t first = buf == 0 ? 64u : 0u;
+            const bool shares = half == 1u - buf;
+            auto arrive = [&]() {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(shared_read_bar, 0));
+            };
+            if (!shares) arrive();
+#pragma unroll 1
+            for (uint32_t part = 0; part < 2; ++part) {
+                const uint32_t in_half = part == 0 ? first : 64u - first;
+                uint32_t acc[64];
+                const uint32_t from = tmem_base + ((quarter * 32u) << 16) + buf * kPairSecond + half * 128u + in_half;
+                tmem_ld_32x32(from, *reinterpret_cast<uint32_t(*)[32]>(&acc[0]));
+                tmem_ld_32x32(from + 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[32]));
+                tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[0]));
+                tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[32]));
+                if (shares && part == 0) arrive();
+                store_rows<kBf16, 64>(acc, p, dest, nt * 256u + half * 128u + in_half, staging, kPairStagingPitch, lane);
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync_all();  // neither CTA retires while its partner reads its shared memory or signals its barriers
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc<2>(tmem_base, 512);
+    }
+}
+
+int sm_count() {
+    static int cached[64] = {0};
+    int d = 0;
+    cudaGetDevice(&d);
+    if (d < 0 || d >= 64) d = 0;
+    if (!cached[d]) {
+        int n = 0;
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d);
+        cached[d] = n > 0 ? n : 148;
+    }
+    return cached[d];
+}
+int usable_sms() { return sm_budget() > 0 && sm_budget() < sm_count() ? sm_budget() : sm_count(); }
+
+// Rows of 128 bytes, `box_rows` of them per copy.
+bool line_map(CUtensorMap &map, const void *base, uint64_t lines, uint32_t box_rows) {
+    cuuint64_t dims[2] = {128, lines};
+    cuuint64_t strides[1] = {128};
+    cuuint32_t box[2] = {128, box_rows}, steps[2] = {1, 1};
+    return get_encode_tiled()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool kBf16>
+cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t stream) {
+    auto kernel = gemm_mx_pair_kernel<kBf16>;
+    static int max_pairs[64] = {0};
+    int d = 0;
+    cudaGetDevice(&d);
+    if (d < 0 || d >= 64) d = 0;
+    if (max_pairs[d] == 0) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * (sm_count() / 2));
+        cfg.blockDim = dim3(kPairThreads);
+        cfg.dynamicSmemBytes = kPairSmem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) { cudaGetLastError(); n = sm_count() / 2; }
+        max_pairs[d] = n;
+    }
+    uint32_t pairs = dev.tiles_m * dev.tiles_n, most = (uint32_t)max_pairs[d];
+    if (usable_sms() > 1 && (uint32_t)usable_sms() / 2 < most) most = (uint32_t)usable_sms() / 2;
+    if (pairs > most) pairs = most;
+    kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(maps, dev);
+    return cudaGetLastError();
+}
+
 template <int kBN, int kStages, bool kBf16>
 cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
     using P = Plan<kBN, kStages>;
@@ -270,20 +562,25 @@ cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream
         if (e != cudaSuccess) return e;
         configured[d] = true;
     }
-    int sms = 0;
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d);
-    if (sms <= 0) sms = 148;
-    if (sm_budget() > 0 && sm_budget() < sms) sms = sm_budget();
-    const uint32_t grid = (uint32_t)(max_tiles < (uint64_t)sms ? max_tiles : (uint64_t)sms);
+    const uint32_t grid = (uint32_t)(max_tiles < (uint64_t)usable_sms() ? max_tiles : (uint64_t)usable_sms());
     kernel<<<grid, kThreads, P::kTotal, stream>>>(dev);
     return cudaGetLastError();
 }
 
 } // namespace
 
+bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t k) {
+    return ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 2;
+}
+
+static bool use_pairs(const MxGemmArgs &args) { return args.tiles == nullptr && gemm_mx_reads_rows(args.m, args.n, args.k); }
+
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     if (args.m == 0 || args.n == 0) return cudaSuccess;
     if (args.m > 0x7fffff00ull || args.n > 0x7fffff00ull || args.k > 0x7fffff00ull) return cudaErrorInvalidValue;
+    // Tensor maps address lines of 128 bytes with 31-bit coordinates.
+    const uint64_t most_chunks = 0x7fffff00ull / (kMxChunkBytes / 128);
+    if ((args.m / 128 + 2) * (args.k / 256 + 1) > most_chunks || (args.n / 128 + 2) * (args.k / 256 + 1) > most_chunks) return cudaErrorInvalidValue;
     constexpr int kBN = 128, kStages = 5;
     MxGemmDev dev;
     dev.a_chunks = static_cast<const uint8_t *>(args.a_chunks);
@@ -301,6 +598,30 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.row_dest = args.row_dest;
     dev.error_word = args.error_word;
     wait_limits_us(dev.wait_us);
+    dev.a_row_major = args.a_codes != nullptr;
+    dev.a_scales = dev.a_chunks + (args.a_codes ? 0u : kMxCodeBytes);
+    dev.a_scale_step = args.a_codes ? kMxScaleBytes : kMxChunkBytes;
+    if (use_pairs(args)) {
+        if (!get_encode_tiled()) return cudaErrorNotSupported;
+        dev.tiles_m = (uint32_t)((args.m + 255) / 256);
+        dev.tiles_n = (uint32_t)((args.n + 255) / 256);
+        PairMaps maps;
+        const uint64_t a_chunks = (args.m + 127) / 128 * dev.kblocks, b_lines = (uint64_t)dev.group_blocks * dev.kblocks * kMxChunkLines;
+        bool ok;
+        if (args.a_codes) {
+            cuuint64_t dims[2] = {(args.k + 1) / 2, args.m}, strides[1] = {args.a_codes_stride};
+            cuuint32_t box[2] = {128, kBM}, steps[2] = {1, 1};
+            ok = get_encode_tiled()(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(args.a_codes), dims, strides, box, steps,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        } else {
+            ok = line_map(maps.a, args.a_chunks, a_chunks * kMxChunkLines, 128);
+        }
+        ok = ok && line_map(maps.b, args.b_chunks, b_lines, 128);
+        if (!ok) return cudaErrorInvalidValue;
+        return args.c_bf16 ? launch_pair<true>(maps, dev, stream) : launch_pair<false>(maps, dev, stream);
+    }
+    if (args.a_codes) return cudaErrorInvalidValue;
     const uint64_t tiles = (args.tiles ? args.max_tiles : dev.tiles_m) * (uint64_t)dev.tiles_n;
     if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
     return args.c_bf16 ? launch<kBN, kStages, true>(dev, tiles, stream) : launch<kBN, kStages, false>(dev, tiles, stream);

@@ -50,13 +50,18 @@ cudaError_t launch_mx_dequantise(uint32_t type, const void *codes, uint64_t code
 cudaError_t launch_mx_tile(const void *codes, uint64_t codes_stride, const void *scales, uint64_t scales_stride, uint64_t groups,
                            uint64_t width, uint64_t depth, bool pad_rows, void *chunks, cudaStream_t stream);
 
+// Row-major scales -> scale tiles alone, 1024 bytes per 128 rows x 256 values.
+cudaError_t launch_mx_tile_scales(const void *scales, uint64_t scales_stride, uint64_t rows, uint64_t depth, void *tiles, cudaStream_t stream);
+
 // One row tile (128 rows of A in tile form) of a grouped product.
 struct MxRowTile {
     int32_t group;  // packed matrix its rows multiply
     int32_t rows;   // valid rows, 1 .. 128
 };
 struct MxGemmArgs {
-    const void *a_chunks;
+    const void *a_chunks;              // A in tile form; with `a_codes` set, its scale tiles alone
+    const void *a_codes = nullptr;     // A's row-major codes (16-byte aligned, stride too), see gemm_mx_reads_rows
+    uint64_t a_codes_stride = 0;
     const void *b_chunks;
     void *c;
     uint64_t c_stride;
@@ -68,6 +73,8 @@ struct MxGemmArgs {
     uint64_t max_tiles = 0;            // row tiles there may be at most
     unsigned int *error_word = nullptr;
 };
+// Whether a product of this size reads A's codes from the caller's rows when they are aligned.
+bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t k);
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream);
 
 // ---- routing and the experts' products ----

@@ -159,9 +159,15 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     else if (ok) {
         uint8_t *chunks = workspace_or_scratch(workspace, chunk_bytes(m, k));
         ok = chunks != nullptr;
+        bool rows_in_place = false;
+        const uint8_t *cd = nullptr;
         if (ok && codes) {
-            const uint8_t *cd = ops.in(codes, m, (k + 1) / 2, codes_stride), *sd = cd ? ops.in(scales, m, kblocks, scales_stride) : nullptr;
-            ok = sd && cuda_ok(launch_mx_tile(cd, codes_stride, sd, scales_stride, 1, m, k, false, chunks, stream), "tile kernel");
+            cd = ops.in(codes, m, (k + 1) / 2, codes_stride);
+            const uint8_t *sd = cd ? ops.in(scales, m, kblocks, scales_stride) : nullptr;
+            if (m == 1) codes_stride = round_up((k + 1) / 2, 16);
+            rows_in_place = sd && gemm_mx_reads_rows(m, n, k) && ((reinterpret_cast<uintptr_t>(cd) | codes_stride) & 15u) == 0;
+            if (rows_in_place) ok = cuda_ok(launch_mx_tile_scales(sd, scales_stride, m, k, chunks, stream), "scale tile kernel");
+            else ok = sd && cuda_ok(launch_mx_tile(cd, codes_stride, sd, scales_stride, 1, m, k, false, chunks, stream), "tile kernel");
         } else if (ok) {
             const uint8_t *ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
             ok = ad && cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, a_stride, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
@@ -169,6 +175,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
         if (ok) {
             MxGemmArgs args;
             args.a_chunks = chunks; args.b_chunks = blob + g.payload_offset;
+            if (rows_in_place) { args.a_codes = cd; args.a_codes_stride = codes_stride; }
             args.c = c_dev; args.c_stride = c_stride; args.c_bf16 = c_type == kBF16;
             args.m = m; args.n = n; args.k = k; args.error_word = err;
             ok = cuda_ok(launch_gemm_mx(args, stream), "mxfp4 GEMM kernel");

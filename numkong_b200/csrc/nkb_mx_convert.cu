@@ -205,6 +205,33 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, ui
     }
 }
 
+// Scale tiles alone: one thread per 16-byte line, i.e. four scales of the rows r, r + 32, r + 64 and r + 96 of a chunk. The
+// threads of a warp walk the words of one row, so that the reads are whole lines.
+__global__ void __launch_bounds__(kThreads) tile_scales_kernel(const uint8_t *scales, uint64_t scales_stride, uint64_t rows, uint64_t depth,
+                                                               uint64_t row_blocks, uint32_t words, uint8_t *tiles) {
+    const uint64_t row_scales = (depth + kMxBlock - 1) / kMxBlock, items = row_blocks * 32 * words;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(scales) | scales_stride) & 3u) == 0;
+    for (uint64_t item = (uint64_t)blockIdx.x * kThreads + threadIdx.x; item < items; item += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t line = item / words;
+        const uint32_t word = (uint32_t)(item - line * words), r = (uint32_t)(line & 31u);
+        const uint64_t block = line >> 5, first = (uint64_t)word * 4;
+        uint32_t w[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint64_t row = block * kChunkRows + g * 32 + r;
+            w[g] = 0x7f7f7f7fu;
+            if (row < rows) {
+                const uint8_t *s = scales + row * scales_stride + first;
+                if (aligned && first + 4 <= row_scales) w[g] = __ldg(reinterpret_cast<const uint32_t *>(s));
+                else
+                    for (int i = 0; i < 4; ++i)
+                        if (first + i < row_scales) w[g] = (w[g] & ~(255u << (8 * i))) | ((uint32_t)s[i] << (8 * i));
+            }
+        }
+        *reinterpret_cast<uint4 *>(tiles + (block * (words / 2) + word / 2) * kMxScaleBytes + (word & 1u) * 512 + r * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 uint32_t grid_for(uint64_t warps) {
     const uint64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
     return (uint32_t)(blocks < 148ull * 8 * 4 ? (blocks ? blocks : 1) : 148ull * 8 * 4);
@@ -254,6 +281,14 @@ cudaError_t launch_mx_dequantise(uint32_t type, const void *codes, uint64_t code
     case kF16: dequantise_kernel<kF16><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, rows, depth, dst, x_stride); break;
     default: return cudaErrorInvalidValue;
     }
+    return cudaGetLastError();
+}
+
+cudaError_t launch_mx_tile_scales(const void *scales, uint64_t scales_stride, uint64_t rows, uint64_t depth, void *tiles, cudaStream_t stream) {
+    const uint64_t row_blocks = (rows + kChunkRows - 1) / kChunkRows;
+    const uint32_t words = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues) * 2;
+    tile_scales_kernel<<<grid_for(row_blocks * words), kThreads, 0, stream>>>(static_cast<const uint8_t *>(scales), scales_stride, rows, depth, row_blocks, words,
+                                                                              static_cast<uint8_t *>(tiles));
     return cudaGetLastError();
 }
 

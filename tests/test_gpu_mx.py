@@ -130,6 +130,26 @@ def test_product(m, n, k, cells):
     check_product(a, b, k, got, cells)
 
 
+@pytest.mark.parametrize("cells", ["f32", "bf16"])
+@pytest.mark.parametrize("rows_aligned", [True, False])
+@pytest.mark.parametrize("m,n,k", [(2304, 2304, 256), (2400, 2100, 520), (100, 19000, 321), (1, 19001, 300), (19001, 3, 1030), (5000, 1025, 2049)])
+def test_large_product(m, n, k, rows_aligned, cells):
+    """Sizes that fill the GPU with 256 x 256 tiles, with whole and with ragged edges, A's rows on and off 16-byte boundaries."""
+    a, b = random_mx(m, k, m + k), random_mx(n, k, n + k + 1)
+    bytes_a = a[0].shape[1]
+    held = np.zeros((m, -(-bytes_a // 16) * 16 + (0 if rows_aligned else 1)), np.uint8)
+    held[:, :bytes_a] = a[0]
+    packed = nk.dots_pack(nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), k))
+    x = nk.MxMatrix(torch.from_numpy(held).cuda()[:, :bytes_a], torch.from_numpy(a[1]).cuda(), k)
+    got = nk.dots_packed(x, packed, out_dtype=cells)
+    assert nk.synchronize() == 0
+    check_product(a, b, k, got, cells)
+    if rows_aligned and cells == "f32":  # the same bits as a float matrix of these values quantised on the way, and as few rows alone
+        assert torch.equal(nk.dots_packed(nk.mx_dequantise(x), packed), nk.dots_packed(nk.mx_quantise(nk.mx_dequantise(x)), packed))
+        few = nk.MxMatrix(x.codes[m // 2:m // 2 + 3], x.scales[m // 2:m // 2 + 3], k)
+        assert torch.equal(nk.dots_packed(few, packed), got[m // 2:m // 2 + 3])
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("m,n,k", [(1, 300, 512), (5, 128, 100), (70, 200, 321), (257, 384, 1024)])
 def test_product_of_floats_quantises_first(m, n, k, name):
