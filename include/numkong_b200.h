@@ -370,6 +370,10 @@ NKB_API char const *nkb_last_error(void);
  *  per-thread staging buffers pass from one call to the next, so a switch puts the new stream behind the work this thread
  *  already enqueued on the old one (an event wait on the device; the host does not block). */
 NKB_API void nkb_set_stream(void *cuda_stream);
+/** Enqueues the calling thread's next calls of the nkb_mx_*, nkb_dots_*_mxfp4, nkb_route* and nkb_experts_* families on
+ *  another stream until it is called again with `on` 0, without ordering the two streams: for callers whose operands and
+ *  workspaces follow that stream by themselves. Calls without a workspace, and all other entry points, want nkb_set_stream. */
+NKB_API void nkb_borrow_stream(void *cuda_stream, int on);
 /** Waits for the calling thread's stream and returns the device error word: 0, or 0x80000000 | site << 16 | block of the
  *  first bounded pipeline wait that gave up on this GPU since the last report (sites: 1 loader waiting for a free stage,
  *  2 / 3 MMA issuer waiting for a drained accumulator / a loaded stage, 4 epilogue waiting for a finished accumulator,

@@ -54,6 +54,16 @@ def _is_torch(x: Any) -> bool:
     return type(x).__module__.startswith("torch")
 
 
+_torch_names_of: dict = {}  # torch dtype -> its name, filled as types are met: spelling a dtype out costs a microsecond
+
+
+def _torch_name(dtype: Any) -> str:
+    name = _torch_names_of.get(dtype)
+    if name is None:
+        name = _torch_names_of[dtype] = str(dtype).replace("torch.", "")
+    return name
+
+
 _CAI_TYPES = {"<f2": "f16", "<f4": "f32", "<f8": "f64", "|i1": "i8", "|u1": "u8"}  # other element types need dtype=...
 
 
@@ -116,14 +126,14 @@ class _View:
                 raise ValueError("expected a 2-D matrix")
             if x.stride(1) != 1 and x.shape[1] > 1:
                 raise ValueError("rows must be contiguous (column-major inputs are not supported)")
-            name = dtype or _TORCH_NAMES.get(str(x.dtype))
+            name = dtype or _TORCH_NAMES.get("torch." + _torch_name(x.dtype))
             if name is None:
                 raise TypeError(f"unsupported torch dtype {x.dtype}")
             self.is_cuda = x.is_cuda
             self.ptr = x.data_ptr()
-            self.rows, self.cols = int(x.shape[0]), int(x.shape[1])
-            self.stride = int(x.stride(0)) * x.element_size() if self.rows > 1 else self.cols * x.element_size()
+            self.rows, self.cols = x.shape
             item = x.element_size()
+            self.stride = x.stride(0) * item if self.rows > 1 else self.cols * item
         else:
             x = np.asarray(x)
             self.obj = x
@@ -620,38 +630,53 @@ def merge_topk(values: Any, ids: Any, top: Optional[int] = None):
 _thread = threading.local()  # .stream: what this thread gave set_stream
 
 
-class _enqueue:
-    """Around the calls below: the GPU of the tensor they work on is made current, and a thread that has not chosen a
-    stream with set_stream enqueues on torch's current one, where the tensors come from and the results go."""
+class _torch:
+    """What the calls below need of torch, looked up when the first tensor arrives."""
+    ready = False
 
-    def __init__(self, x: Any):
-        self.device = x.device if _is_torch(x) and x.is_cuda else None
+    @classmethod
+    def load(cls):
+        import torch
+        cls.module, cls.empty, cls.current_device = torch, torch.empty, torch.cuda.current_device
+        cls.types = {name: getattr(torch, of) for name, of in _CAST_TORCH.items() if hasattr(torch, of)}
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a tenth of the public way's three microseconds
+        cls.stream = staticmethod(raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+        cls.ready = True
+        return cls
 
-    def __enter__(self):
-        self.guard, self.switched = None, False
-        if self.device is not None:
-            import torch
-            if self.device.index != torch.cuda.current_device():
-                self.guard = torch.cuda.device(self.device)
-                self.guard.__enter__()
-            if not getattr(_thread, "stream", 0):
-                stream = torch.cuda.current_stream().cuda_stream
-                if stream:
-                    lib.nkb_set_stream(stream)
-                    self.switched = True
 
-    def __exit__(self, *_):
-        if self.switched:
-            lib.nkb_set_stream(None)
-        if self.guard is not None:
-            self.guard.__exit__(None, None, None)
+def _cuda(x: Any) -> bool:
+    return _is_torch(x) and x.is_cuda
+
+
+def _enqueue(x: Any, call: Any, *arguments: Any) -> None:
+    """Makes a library call that works on `x`: with the GPU of a CUDA tensor current, and for a thread that has not chosen a
+    stream with set_stream on torch's current one, where the tensors come from and the results go."""
+    if not _cuda(x):
+        call(*arguments)
+        return
+    t = _torch if _torch.ready else _torch.load()
+    index = x.get_device()
+    if index != t.current_device():
+        with t.module.cuda.device(index):
+            _enqueue(x, call, *arguments)
+        return
+    stream = 0 if getattr(_thread, "stream", 0) else t.stream(index)
+    if not stream:
+        call(*arguments)
+        return
+    lib.nkb_borrow_stream(stream, 1)
+    try:
+        call(*arguments)
+    finally:
+        lib.nkb_borrow_stream(None, 0)
 
 
 def _like(x: Any, shape: Tuple[int, ...], name: str):
     """A new array of element type `name` where `x` lives; bf16 is uint16 storage in NumPy."""
     if _is_torch(x):
-        import torch
-        return torch.empty(shape, dtype=getattr(torch, _CAST_TORCH[name]), device=x.device)
+        t = _torch if _torch.ready else _torch.load()
+        return t.empty(shape, dtype=t.types[name], device=x.device)
     return np.empty(shape, dtype=_CAST_NUMPY[name])
 
 
@@ -659,20 +684,21 @@ def _workspace(x: Any, nbytes: int):
     """(buffer, pointer) of a call's workspace: a tensor of the caller's allocator for CUDA operands, none (the library's own
     staging memory) otherwise - for host operands, and on a stream chosen with set_stream that is not torch's current one: the
     allocator would hand the memory on when the call returns, in an order that stream does not follow."""
-    if _is_torch(x) and x.is_cuda:
-        import torch
-        if getattr(_thread, "stream", 0) not in (0, torch.cuda.current_stream(x.device).cuda_stream):
-            return None, None
-        buffer = torch.empty(nbytes + 256, dtype=torch.uint8, device=x.device)
-        return buffer, (buffer.data_ptr() + 255) // 256 * 256
-    return None, None
+    if not _cuda(x):
+        return None, None
+    t = _torch if _torch.ready else _torch.load()
+    chosen = getattr(_thread, "stream", 0)
+    if chosen and chosen != t.stream(x.get_device()):
+        return None, None
+    buffer = t.empty(nbytes + 256, dtype=t.types["u8"], device=x.device)
+    return buffer, (buffer.data_ptr() + 255) // 256 * 256
 
 
 def _checked(x: Any, shape: Tuple[int, ...], names: Tuple[str, ...], what: str, like: Any = None):
     """`x` as a dense array of the given shape and one of the given types, where `like` lives."""
     if not _is_torch(x):
         x = np.asarray(x)
-    name = str(x.dtype).replace("torch.", "")
+    name = _torch_name(x.dtype) if _is_torch(x) else x.dtype.name
     if name not in names or tuple(x.shape) != shape:
         raise ValueError(f"{what} must be {' or '.join(names)} of shape {shape}, got {name} of shape {tuple(x.shape)}")
     if not (x.is_contiguous() if _is_torch(x) else x.flags.c_contiguous):
@@ -700,11 +726,20 @@ class MxMatrix:
             raise ValueError(f"depth {self.depth} needs rows of {(self.depth + 1) // 2} code bytes and {(self.depth + 31) // 32} scale bytes")
         if _is_torch(c.obj) != _is_torch(s.obj) or (_is_torch(c.obj) and c.obj.device != s.obj.device):
             raise ValueError("codes and scales must live in the same place")
-        self.codes, self.scales, self.rows, self._c, self._s = c.obj, s.obj, c.rows, c, s
+        self.codes, self.scales, self.rows = c.obj, s.obj, c.rows
+        self._parts = c.ptr, c.stride, s.ptr, s.stride
+
+    @classmethod
+    def _of(cls, codes: Any, scales: Any, depth: int) -> "MxMatrix":
+        """Of two dense arrays of the right shapes."""
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.rows, self.depth = codes, scales, codes.shape[0], depth
+        self._parts = _ptr(codes), codes.shape[1], _ptr(scales), scales.shape[1]
+        return self
 
     @property
     def is_cuda(self) -> bool:
-        return self._c.is_cuda
+        return _cuda(self.codes)
 
     def __repr__(self) -> str:
         return f"MxMatrix(rows={self.rows}, depth={self.depth})"
@@ -715,11 +750,10 @@ def mx_quantise(x: Any, *, dtype: Optional[str] = None) -> MxMatrix:
     2^(floor(log2(largest)) - 2), each value to the nearest code, ties to the even code, beyond 6 scales to 6. A block that
     holds an infinity or a NaN becomes NaN."""
     v = _float_view(x, dtype, "mx_quantise")
-    codes, scales = _like(v.obj, (v.rows, (v.cols + 1) // 2), "u8"), _like(v.obj, (v.rows, (v.cols + 31) // 32), "u8")
-    with _enqueue(v.obj):
-        lib.nkb_mx_quantise(v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, _ptr(codes), codes.shape[1], _ptr(scales), scales.shape[1])
+    q = MxMatrix._of(_like(v.obj, (v.rows, (v.cols + 1) // 2), "u8"), _like(v.obj, (v.rows, (v.cols + 31) // 32), "u8"), v.cols)
+    _enqueue(v.obj, lib.nkb_mx_quantise, v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, *q._parts)
     check("mx_quantise")
-    return MxMatrix(codes, scales, v.cols)
+    return q
 
 
 def mx_dequantise(q: MxMatrix, to_dtype: str = "f32"):
@@ -729,9 +763,7 @@ def mx_dequantise(q: MxMatrix, to_dtype: str = "f32"):
     if to_dtype not in ("f32", "f16", "bf16"):
         raise TypeError(f"cannot write {to_dtype!r}")
     out = _like(q.codes, (q.rows, q.depth), to_dtype)
-    with _enqueue(q.codes):
-        lib.nkb_mx_dequantise(q._c.ptr, q._c.stride, q._s.ptr, q._s.stride, q.rows, q.depth, _ptr(out), DTYPE_CODES[to_dtype],
-                              q.depth * DTYPE_BYTES[to_dtype])
+    _enqueue(q.codes, lib.nkb_mx_dequantise, *q._parts, q.rows, q.depth, _ptr(out), DTYPE_CODES[to_dtype], q.depth * DTYPE_BYTES[to_dtype])
     check("mx_dequantise")
     return out
 
@@ -743,8 +775,7 @@ def _pack_mx(b: MxMatrix, groups: int) -> PackedMatrix:
     width = b.rows // groups
     nbytes = int(lib.nkb_dots_packed_size_mxfp4(groups, width, b.depth))
     buf = _like(b.codes, (nbytes,), "u8")
-    with _enqueue(b.codes):
-        lib.nkb_dots_pack_mxfp4(b._c.ptr, b._c.stride, b._s.ptr, b._s.stride, groups, width, b.depth, _ptr(buf))
+    _enqueue(b.codes, lib.nkb_dots_pack_mxfp4, *b._parts, groups, width, b.depth, _ptr(buf))
     check("dots_pack")
     return PackedMatrix(buf, "mxfp4", width, b.depth, groups)
 
@@ -756,9 +787,10 @@ def _mx_result(x: Any, rows: int, width: int, out: Any, out_dtype: str):
     if out is None:
         return _like(x, (rows, width), out_dtype), width * DTYPE_BYTES[out_dtype]
     v = _View(out, out_dtype)
-    if (v.rows, v.cols) != (rows, width) or str(v.obj.dtype).replace("torch.", "") not in ("float32", "bfloat16", "uint16"):
+    kind = _torch_name(v.obj.dtype) if _is_torch(v.obj) else v.obj.dtype.name
+    if (v.rows, v.cols) != (rows, width) or kind not in ("float32", "bfloat16", "uint16"):
         raise ValueError("out has the wrong shape or cell type")
-    if v.is_cuda and (not _is_torch(x) or x.device != v.obj.device):
+    if v.is_cuda and (not _is_torch(x) or not _is_torch(v.obj) or x.device != v.obj.device):
         raise ValueError("out must live where the other operands live")
     return v.obj, v.stride
 
@@ -772,14 +804,12 @@ def _packed_mx(a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], out
         raise ValueError(f"depth mismatch: a has {depth} dimensions, packed matrix has depth {packed.depth}")
     x = v.codes if isinstance(v, MxMatrix) else v.obj
     result, stride = _mx_result(x, v.rows, packed.width, out, out_dtype)
-    workspace, ws = _workspace(x, lib.nkb_dots_workspace_mxfp4(v.rows, depth))
-    with _enqueue(x):
-        if isinstance(v, MxMatrix):
-            lib.nkb_dots_packed_mxfp4(v._c.ptr, v._c.stride, v._s.ptr, v._s.stride, _ptr(packed.buffer), _ptr(result), DTYPE_CODES[out_dtype],
-                                      v.rows, packed.width, depth, stride, ws)
-        else:
-            lib.nkb_dots_packed_quantised_mxfp4(v.ptr, DTYPE_CODES[v.dtype], v.stride, _ptr(packed.buffer), _ptr(result),
-                                                DTYPE_CODES[out_dtype], v.rows, packed.width, depth, stride, ws)
+    workspace, ws = _workspace(x, (v.rows + 127) // 128 * ((depth + 255) // 256) * 17408)  # nkb_dots_workspace_mxfp4
+    rest = _ptr(packed.buffer), _ptr(result), DTYPE_CODES[out_dtype], v.rows, packed.width, depth, stride, ws
+    if isinstance(v, MxMatrix):
+        _enqueue(x, lib.nkb_dots_packed_mxfp4, *v._parts, *rest)
+    else:
+        _enqueue(x, lib.nkb_dots_packed_quantised_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, *rest)
     check("dots_packed")
     return result
 
@@ -800,9 +830,8 @@ def route(logits: Any, top: int, *, bias: Any = None, score: str = "softmax", gr
     if bias is not None:
         bias = _checked(bias, (v.cols,), ("float32",), "bias", v.obj)
     weights, ids = _like(v.obj, (v.rows, int(top)), "f32"), _like(v.obj, (v.rows, int(top)), "i32")
-    with _enqueue(v.obj):
-        lib.nkb_route(v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, None if bias is None else _ptr(bias), _SCORES[score], groups,
-                      groups if top_groups is None else top_groups, top, int(renormalise), scale, _ptr(weights), _ptr(ids))
+    _enqueue(v.obj, lib.nkb_route, v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, None if bias is None else _ptr(bias), _SCORES[score],
+             groups, groups if top_groups is None else top_groups, top, int(renormalise), scale, _ptr(weights), _ptr(ids))
     check("route")
     return weights, ids
 
@@ -818,9 +847,8 @@ def route_gradient(weights_grad: Any, ids: Any, logits: Any, *, score: str = "so
     ids = _checked(ids, (v.rows, top), ("int32",), "ids", v.obj)
     weights_grad = _checked(weights_grad, (v.rows, top), ("float32",), "weights_grad", v.obj)
     grad = _like(v.obj, (v.rows, v.cols), "f32")
-    with _enqueue(v.obj):
-        lib.nkb_route_gradient(_ptr(weights_grad), _ptr(ids), v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, _SCORES[score], top,
-                               int(renormalise), scale, _ptr(grad))
+    _enqueue(v.obj, lib.nkb_route_gradient, _ptr(weights_grad), _ptr(ids), v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, _SCORES[score],
+             top, int(renormalise), scale, _ptr(grad))
     check("route_gradient")
     return grad
 
@@ -853,10 +881,8 @@ def experts_packed(x: Any, ids: Any, packed: PackedMatrix, *, weights: Any = Non
         out = _checked(out, (tokens, top, packed.width), ("float32", "bfloat16", "uint16"), "out", v.obj).reshape(rows, packed.width)
     result, stride = _mx_result(v.obj, rows, packed.width, out, out_dtype)
     workspace, ws = _workspace(v.obj, lib.nkb_experts_workspace_mxfp4(tokens, top, packed.groups, packed.width, v.depth, int(weights is not None)))
-    with _enqueue(v.obj):
-        lib.nkb_experts_packed_mxfp4(v.ptr, DTYPE_CODES[v.dtype], v.stride, int(per_slot), _ptr(ids), tokens, top, _ptr(packed.buffer),
-                                     packed.groups, packed.width, v.depth, None if weights is None else _ptr(weights), _ptr(result),
-                                     DTYPE_CODES[out_dtype], stride, ws)
+    _enqueue(v.obj, lib.nkb_experts_packed_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, int(per_slot), _ptr(ids), tokens, top, _ptr(packed.buffer),
+             packed.groups, packed.width, v.depth, None if weights is None else _ptr(weights), _ptr(result), DTYPE_CODES[out_dtype], stride, ws)
     check("experts_packed")
     return result if weights is not None else result.reshape(tokens, top, packed.width)
 

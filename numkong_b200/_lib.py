@@ -95,6 +95,7 @@ def _load() -> ctypes.CDLL:
     lib.nkb_peer_barrier.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int, ctypes.c_uint32]
     u32, i32, f32 = ctypes.c_uint32, ctypes.c_int, ctypes.c_float
     for name, result, arguments in (
+        ("nkb_borrow_stream", None, [vp, i32]),
         ("nkb_mx_quantise", None, [vp, u32, sz, sz, sz, vp, sz, vp, sz]),
         ("nkb_mx_dequantise", None, [vp, sz, vp, sz, sz, sz, vp, u32, sz]),
         ("nkb_dots_packed_size_mxfp4", sz, [sz, sz, sz]),

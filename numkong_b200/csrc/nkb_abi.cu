@@ -219,7 +219,7 @@ void fill_error_output(void *out, MemKind kind, uint64_t rows, uint64_t row_byte
     if (kind == kMemHost) {
         for (uint64_t r = 0; r < rows; ++r) std::memset(static_cast<uint8_t *>(out) + r * stride, 0xFF, row_bytes);
     } else {
-        cudaMemset2DAsync(out, stride, 0xFF, row_bytes, rows, t_ctx.stream);
+        cudaMemset2DAsync(out, stride, 0xFF, row_bytes, rows, current_stream());
         cudaGetLastError();
     }
 }
@@ -691,6 +691,10 @@ NKB_API void nkb_set_stream(void *cuda_stream) {
         cudaGetLastError();
     }
     t_ctx.stream = next;
+}
+NKB_API void nkb_borrow_stream(void *cuda_stream, int on) {
+    t_ctx.override_stream = static_cast<cudaStream_t>(cuda_stream);
+    t_ctx.use_override = on != 0;
 }
 NKB_API uint32_t nkb_synchronize(void) {
     clear_error();

@@ -21,7 +21,6 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kStepBytes = 32;       // bytes of depth (64 values) one MMA consumes
 constexpr uint32_t kMxChunkLines = kMxChunkBytes / 128;  // a chunk as rows of 128 bytes: 128 of codes, 8 of scales
 constexpr uint32_t kGroupM = 8;      // row tiles walked before the next column tile
 
@@ -41,15 +40,21 @@ struct MxGemmDev {
     uint32_t wait_us[kWaitSites];
 };
 
-template <int kBN, int kStages>
+// Shared memory of the single-CTA kernel. The MMA always reads 128 rows of A; with kARows = 16 a stage holds 16 of them and the rest of
+// what it reads is the stages behind (and 14 KiB of slack): rows of the accumulator nobody looks at. That leaves room for more
+// stages of B, which is what a product with few rows waits for.
+template <int kBN, int kARows>
 struct Plan {
-    static constexpr int kBBytes = kBN * 128;
-    static constexpr int kScaleOffset = kBM * 128 + kBBytes;           // A codes, B codes, A scales, B scales
-    static constexpr int kStageBytes = kScaleOffset + kMxScaleBytes + kBN / 128 * kMxScaleBytes;
-    static constexpr int kBarrierOffset = kStages * kStageBytes;
+    static constexpr int kABytes = kARows * 128, kBBytes = kBN * 128;
+    static constexpr int kStageBytes = kBBytes + 2 * kMxScaleBytes;    // B codes, A scales, B scales; A's codes have a ring of their own
+    static constexpr int kRoom = 176 * 1024 - (kBM - kARows) * 128;
+    static constexpr int kStages = kRoom / (kStageBytes + kABytes) < 16 ? kRoom / (kStageBytes + kABytes) : 16;
+    static constexpr int kBRing = kStages * kABytes + (kBM - kARows) * 128;
+    static constexpr int kBarrierOffset = kBRing + kStages * kStageBytes;
     static constexpr int kStagingPitch = 144;                          // bytes per staged row: 128 and one 16-byte piece against bank conflicts
-    static constexpr int kStagingOffset = kBarrierOffset + 256;
+    static constexpr int kStagingOffset = kBarrierOffset + 512;
     static constexpr int kTotal = kStagingOffset + kEpilogueWarps * 32 * kStagingPitch + 1024;
+    static_assert(kBRing % 1024 == 0 && kStageBytes % 1024 == 0 && kTotal <= 227 * 1024, "aligned operands that fit");
 };
 
 __device__ __forceinline__ void tile_coords(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t &mt, uint32_t &nt) {
@@ -60,13 +65,15 @@ __device__ __forceinline__ void tile_coords(uint32_t tile, uint32_t tiles_m, uin
     if (group & 1u) nt = tiles_n - 1u - nt;  // the packed rows touched last are still in L2
 }
 
-// Stores this thread's row x kCols f32 accumulators: 128 bytes of a row at a time go through the warp's staging block, so that
-// each store instruction writes whole 128-byte lines. `dest` is this lane's destination row, negative for none.
+// Stores this thread's row x kCols f32 accumulators: up to 128 bytes of a row at a time go through the warp's staging block, so
+// that a store instruction writes whole lines. `dest` is this lane's destination row, negative for none. Rows that do not lie on
+// 16-byte boundaries (an odd width) are written a row at a time, in words as far as their cells make whole ones.
 template <bool kBf16, int kCols>
 __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const MxGemmDev &p, int64_t dest, uint32_t col_base, uint8_t *staging, int pitch, int lane) {
-    constexpr int kPieceCols = kBf16 ? 64 : 32;  // columns in 128 bytes
     constexpr int kCell = kBf16 ? 2 : 4;
-    static_assert(kCols % kPieceCols == 0, "whole pieces");
+    constexpr int kPieceCols = kCols * kCell < 128 ? kCols : 128 / kCell;
+    constexpr int kQuads = kPieceCols * kCell / 16;  // 16-byte parts of a staged row
+    static_assert(kCols % kPieceCols == 0 && kQuads >= 2, "whole pieces");
     if (!__any_sync(0xffffffffu, dest >= 0)) return;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.c) | p.c_stride) & 15u) == 0;
 #pragma unroll
@@ -74,39 +81,48 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const M
         const uint32_t col0 = col_base + c * kPieceCols;
         if (col0 >= p.n) break;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < kQuads; ++q) {
             uint4 v;
             if constexpr (kBf16) {
                 uint32_t w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(acc[c * 64 + q * 8 + 2 * j]), __uint_as_float(acc[c * 64 + q * 8 + 2 * j + 1]));
+                    const int at = c * kPieceCols + q * 8 + 2 * j;
+                    const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(acc[at]), __uint_as_float(acc[at + 1]));
                     w[j] = *reinterpret_cast<const uint32_t *>(&two);
                 }
                 v = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
-                v = make_uint4(acc[c * 32 + q * 4], acc[c * 32 + q * 4 + 1], acc[c * 32 + q * 4 + 2], acc[c * 32 + q * 4 + 3]);
+                const int at = c * kPieceCols + q * 4;
+                v = make_uint4(acc[at], acc[at + 1], acc[at + 2], acc[at + 3]);
             }
             *reinterpret_cast<uint4 *>(staging + lane * pitch + q * 16) = v;
         }
         __syncwarp();
+        const uint32_t cells = min((uint32_t)kPieceCols, p.n - col0);
+        if (aligned && cells == kPieceCols) {
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-            const int r = it * 4 + lane / 8, q = lane % 8;
-            const int64_t row = __shfl_sync(0xffffffffu, dest, r);
-            const uint32_t col = col0 + q * (16 / kCell);
-            if (row >= 0 && col < p.n) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(staging + r * pitch + q * 16);
-                uint8_t *dst = p.c + (uint64_t)row * p.c_stride + (uint64_t)col * kCell;
-                if (aligned && col + 16 / kCell <= p.n) __stcs(reinterpret_cast<uint4 *>(dst), v);
-                else {
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int j = 0; j < 16 / kCell; ++j)
-                        if (col + j < p.n) {
-                            if constexpr (kBf16) *reinterpret_cast<uint16_t *>(dst + 2 * j) = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-                            else *reinterpret_cast<uint32_t *>(dst + 4 * j) = w[j];
-                        }
+            for (int it = 0; it < kQuads; ++it) {
+                const int r = it * (32 / kQuads) + lane / kQuads, q = lane % kQuads;
+                const int64_t row = __shfl_sync(0xffffffffu, dest, r);
+                if (row >= 0)
+                    __stcs(reinterpret_cast<uint4 *>(p.c + (uint64_t)row * p.c_stride + (uint64_t)col0 * kCell) + q, *reinterpret_cast<const uint4 *>(staging + r * pitch + q * 16));
+            }
+        } else {
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+                const int64_t row = __shfl_sync(0xffffffffu, dest, r);
+                if (row < 0) continue;
+                uint8_t *dst = p.c + (uint64_t)row * p.c_stride + (uint64_t)col0 * kCell;
+                if constexpr (kBf16) {
+                    const uint16_t *from = reinterpret_cast<const uint16_t *>(staging + r * pitch);
+                    const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(dst) >> 1) & 1u;  // one cell before the first whole word
+                    const uint32_t at = odd + 2 * lane;
+                    if (at + 1 < cells) *reinterpret_cast<uint32_t *>(dst + 2 * at) = (uint32_t)from[at] | ((uint32_t)from[at + 1] << 16);
+                    else if (at < cells) *reinterpret_cast<uint16_t *>(dst + 2 * at) = from[at];
+                    if (odd && lane == 0) *reinterpret_cast<uint16_t *>(dst) = from[0];
+                } else if ((uint32_t)lane < cells) {
+                    *reinterpret_cast<uint32_t *>(dst + 4 * lane) = *reinterpret_cast<const uint32_t *>(staging + r * pitch + 4 * lane);
                 }
             }
         }
@@ -114,13 +130,30 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const M
     }
 }
 
-template <int kBN, int kStages, bool kBf16>
+// The (tile, depth block) sequence of one CTA or CTA pair out of `step`.
+struct Walk {
+    uint32_t tile, kb, mt, nt, tiles_m, tiles_n, kblocks, step;
+    __device__ Walk(uint32_t first, uint32_t step_, uint32_t tiles_m_, uint32_t tiles_n_, uint32_t kblocks_)
+        : tile(first), kb(0), mt(0), nt(0), tiles_m(tiles_m_), tiles_n(tiles_n_), kblocks(kblocks_), step(step_) { locate(); }
+    __device__ bool valid() const { return tile < tiles_m * tiles_n; }
+    __device__ void locate() { if (valid()) tile_coords(tile, tiles_m, tiles_n, mt, nt); }
+    __device__ void next() {
+        if (++kb < kblocks) return;
+        kb = 0;
+        tile += step;
+        locate();
+    }
+};
+
+template <int kBN, int kARows, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p) {
-    using P = Plan<kBN, kStages>;
+    using P = Plan<kBN, kARows>;
+    constexpr int kStages = P::kStages;
     constexpr int kColsPerThread = kBN / 2;
-    constexpr int kScaleCols = 8 + kBN / 16;                 // one chunk's scales: two words per row of A and of B
-    constexpr int kTmemCols = 512;
+    constexpr int kScaleCols = 16;                           // one chunk's scales: eight columns for 128 rows of A, eight for the row block of B
+    constexpr int kTmemCols = 2 * kBN + kScaleCols <= 256 ? 256 : 512;
     static_assert(2 * kBN + kScaleCols <= kTmemCols, "two accumulators and the scales fit TMEM");
+    static_assert(kBN == 64 || kBN == 128, "a tile's scales begin on an even TMEM column");
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -150,38 +183,41 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tiles_m = p.tile_count ? (uint32_t)*p.tile_count : p.tiles_m;
     const uint32_t num_tiles = tiles_m * p.tiles_n;
+    auto rows_of = [&](uint32_t mt) { return p.tiles ? (uint32_t)p.tiles[mt].rows : min(p.m - mt * kBM, (uint32_t)kBM); };
 
     if (warp == 0) {
         if (lane == 0) {
+            // Only the row groups of eight that hold valid rows of A are fetched.
+            auto load_b = [&](const Walk &w, int stage) {
+                const uint32_t group = p.tiles ? (uint32_t)p.tiles[w.mt].group : 0u;
+                const uint32_t block = w.nt * kBN / 128u, sub = w.nt * kBN % 128u;
+                const uint8_t *b = p.b_chunks + (((uint64_t)group * p.group_blocks + block) * p.kblocks + w.kb) * kMxChunkBytes;
+                const uint32_t dst = smem_base + P::kBRing + stage * P::kStageBytes;
+                mbar_expect_tx(full_bar(stage), (rows_of(w.mt) + 7u) / 8u * 1024u + P::kBBytes + 2 * kMxScaleBytes);
+                bulk_load(dst, b + sub * 128u, P::kBBytes, full_bar(stage));
+                bulk_load(dst + P::kBBytes + kMxScaleBytes, b + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
+            };
+            auto load_a = [&](const Walk &w, int stage) {
+                const uint8_t *a = p.a_chunks + ((uint64_t)w.mt * p.kblocks + w.kb) * kMxChunkBytes;
+                bulk_load(smem_base + stage * P::kABytes, a, (rows_of(w.mt) + 7u) / 8u * 1024u, full_bar(stage));
+                bulk_load(smem_base + P::kBRing + stage * P::kStageBytes + P::kBBytes, a + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
+            };
             int stage = 0;
             uint32_t phase = 0, issued = 0;
             bool ok = true;
-            for (uint32_t tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-                uint32_t mt, nt;
-                tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
-                const uint32_t rows = p.tiles ? (uint32_t)p.tiles[mt].rows : min(p.m - mt * kBM, (uint32_t)kBM);
-                const uint32_t group = p.tiles ? (uint32_t)p.tiles[mt].group : 0u;
-                // Only the row groups of eight that hold valid rows are fetched; what the rest of the buffer holds ends up in
-                // rows of the accumulator that nobody reads.
-                const uint32_t a_bytes = (rows + 7u) / 8u * 1024u;
-                const uint32_t block0 = nt * (kBN / 128), blocks = min((uint32_t)(kBN / 128), p.group_blocks - block0);
-                const uint8_t *a_src = p.a_chunks + (uint64_t)mt * p.kblocks * kMxChunkBytes;
-                const uint8_t *b_src = p.b_chunks + ((uint64_t)group * p.group_blocks + block0) * p.kblocks * kMxChunkBytes;
-                for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+            Walk w(blockIdx.x, gridDim.x, tiles_m, p.tiles_n, p.kblocks);
+            // The packed matrix does not depend on the kernel before, which is still quantising A.
+            Walk early = w;
+            for (int s = 0; s < kStages && early.valid(); ++s, early.next()) load_b(early, s);
+            wait_for_previous_kernel();
+            for (; w.valid(); w.next()) {
+                if (issued >= (uint32_t)kStages) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
-                    const uint32_t dst = smem_base + stage * P::kStageBytes;
-                    mbar_expect_tx(full_bar(stage), a_bytes + kMxScaleBytes + blocks * kMxChunkBytes);
-                    const uint8_t *a = a_src + (uint64_t)kb * kMxChunkBytes;
-                    bulk_load(dst, a, a_bytes, full_bar(stage));
-                    bulk_load(dst + P::kScaleOffset, a + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
-                    for (uint32_t j = 0; j < blocks; ++j) {
-                        const uint8_t *b = b_src + ((uint64_t)j * p.kblocks + kb) * kMxChunkBytes;
-                        bulk_load(dst + kBM * 128 + j * kMxCodeBytes, b, kMxCodeBytes, full_bar(stage));
-                        bulk_load(dst + P::kScaleOffset + (1 + j) * kMxScaleBytes, b + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
-                    }
-                    ++issued;
-                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    load_b(w, stage);
                 }
+                load_a(w, stage);
+                ++issued;
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
             if (!ok) {  // copies in flight must land before the block may retire
                 int s = stage;
@@ -200,6 +236,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             bool ok = true;
             const uint32_t scales_a = tmem_base + 2 * kBN, scales_b = scales_a + 8;
             for (uint32_t tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++seq) {
+                uint32_t mt, nt;
+                tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+                const uint32_t b_column = scales_b + nt * kBN % 128u / 32u;  // the tile's rows inside the row block's scales
                 const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
                 if (!mbar_wait(tmem_empty_bar(buf), buf_phase ^ 1u, 2, p.error_word, p.wait_us[2])) { ok = false; break; }
                 tc_fence_after_sync();
@@ -207,19 +246,17 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
                 for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
                     if (!mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
                     tc_fence_after_sync();
-                    const uint32_t src = smem_base + stage * P::kStageBytes;
-                    const uint64_t a_desc = make_smem_desc_sw128(src), b_desc = make_smem_desc_sw128(src + kBM * 128);
+                    const uint32_t src = smem_base + P::kBRing + stage * P::kStageBytes;
+                    const uint64_t a_desc = make_smem_desc_sw128(smem_base + stage * P::kABytes), b_desc = make_smem_desc_sw128(src);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {  // two scale tiles, 128 values of depth each
-                        tmem_copy_scales<1>(scales_a + t * 4, make_smem_desc_scales(src + P::kScaleOffset + t * 512));
-#pragma unroll
-                        for (int j = 0; j < kBN / 128; ++j)
-                            tmem_copy_scales<1>(scales_b + t * (kBN / 32) + j * 4, make_smem_desc_scales(src + P::kScaleOffset + (1 + j) * kMxScaleBytes + t * 512));
+                        tmem_copy_scales<1>(scales_a + t * 4, make_smem_desc_scales(src + P::kBBytes + t * 512));
+                        tmem_copy_scales<1>(scales_b + t * 4, make_smem_desc_scales(src + P::kBBytes + kMxScaleBytes + t * 512));
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_mxf4<1>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(kBM, kBN, (k & 1) * 2),
-                                     scales_a + (k >> 1) * 4, scales_b + (k >> 1) * (kBN / 32), (kb | (uint32_t)k) != 0u);
+                        umma_mxf4<1>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(kBM, kBN, (k & 1) * 2), scales_a + (k >> 1) * 4,
+                                     b_column + (k >> 1) * 4, (kb | (uint32_t)k) != 0u);
                     umma_commit(empty_bar(stage));
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -236,17 +273,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             uint32_t mt, nt;
             tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
             const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
-            const uint32_t in_tile = quarter * 32u + lane;
-            const uint32_t rows = p.tiles ? (uint32_t)p.tiles[mt].rows : min(p.m - mt * kBM, (uint32_t)kBM);
+            const uint32_t in_tile = quarter * 32u + lane, rows = rows_of(mt);
             int64_t dest = -1;
             if (in_tile < rows) dest = p.row_dest ? (int64_t)p.row_dest[(uint64_t)mt * kBM + in_tile] : (int64_t)mt * kBM + in_tile;
             // The whole warp leaves together: the stores below synchronise it.
             if (!__all_sync(0xffffffffu, mbar_wait(tmem_full_bar(buf), buf_phase, 4, p.error_word, p.wait_us[4]))) break;
             tc_fence_after_sync();
             uint32_t acc[kColsPerThread];
+            const uint32_t from = tmem_base + ((quarter * 32u) << 16) + buf * kBN + half * kColsPerThread;
 #pragma unroll
-            for (int c = 0; c < kColsPerThread / 32; ++c)
-                tmem_ld_32x32(tmem_base + ((quarter * 32u) << 16) + buf * kBN + half * kColsPerThread + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[c * 32]));
+            for (int c = 0; c < kColsPerThread / 32; ++c) tmem_ld_32x32(from + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[c * 32]));
 #pragma unroll
             for (int c = 0; c < kColsPerThread / 32; ++c) tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[c * 32]));
             tc_fence_before_sync();
@@ -289,19 +325,6 @@ static_assert(kPairSecond >= 256 - 64, "the shared columns are the last / first 
 
 struct PairMaps {
     CUtensorMap a, b;
-};
-
-// The (tile, depth block) sequence of one pair.
-struct PairWalk {
-    uint32_t tile, kb, mt, nt;
-    __device__ PairWalk(const MxGemmDev &p, uint32_t pair) : tile(pair), kb(0), mt(0), nt(0) { if (valid(p)) tile_coords(tile, p.tiles_m, p.tiles_n, mt, nt); }
-    __device__ bool valid(const MxGemmDev &p) const { return tile < p.tiles_m * p.tiles_n; }
-    __device__ void next(const MxGemmDev &p, uint32_t num_pairs) {
-        if (++kb < p.kblocks) return;
-        kb = 0;
-        tile += num_pairs;
-        if (valid(p)) tile_coords(tile, p.tiles_m, p.tiles_n, mt, nt);
-    }
 };
 
 template <bool kBf16>
@@ -347,7 +370,8 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
             int stage = 0;
             uint32_t phase = 0, issued = 0;
             bool ok = true;
-            for (PairWalk w(p, pair); w.valid(p); w.next(p, num_pairs)) {
+            wait_for_previous_kernel();
+            for (Walk w(pair, num_pairs, tiles_m, p.tiles_n, p.kblocks); w.valid(); w.next()) {
                 if (!mbar_wait<true>(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
                 const uint32_t dst = smem_base + stage * kPairStageBytes, full = map_to_cta(full_bar(stage), 0);
                 if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * kPairStageBytes);
@@ -407,11 +431,11 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
         const uint32_t column = tmem_base + (((uint32_t)warp & 3u) * 32u << 16) + kPairSecond + 256;
         const uint32_t a_last = (p.m + kBM - 1) / kBM - 1, b_last = p.group_blocks - 1;
         // Lane r of every quarter holds line r of each tile: A for both halves of the chunk's depth, B for both halves of its rows.
-        auto load = [&](const PairWalk &w, uint4 (&r)[6]) {
+        auto load = [&](const Walk &w, uint4 (&r)[6]) {
             const uint64_t a_chunk = (uint64_t)min(w.mt * 2u + rank, a_last) * p.kblocks + w.kb;
             const uint4 *a = reinterpret_cast<const uint4 *>(p.a_scales + a_chunk * p.a_scale_step) + lane;
-            r[0] = __ldg(a);
-            r[1] = __ldg(a + 32);
+            r[0] = a[0];
+            r[1] = a[32];
 #pragma unroll
             for (uint32_t j = 0; j < 2; ++j) {
                 const uint64_t b_chunk = (uint64_t)min(w.nt * 2u + j, b_last) * p.kblocks + w.kb;
@@ -441,17 +465,18 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
             ++chunk;
             return true;
         };
-        PairWalk ahead(p, pair);
+        wait_for_previous_kernel();
+        Walk ahead(pair, num_pairs, tiles_m, p.tiles_n, p.kblocks);
         uint4 even[6], odd[6];
-        bool has_even = ahead.valid(p), has_odd = false;
-        if (has_even) { load(ahead, even); ahead.next(p, num_pairs); }
-        has_odd = ahead.valid(p);
-        if (has_odd) { load(ahead, odd); ahead.next(p, num_pairs); }
+        bool has_even = ahead.valid(), has_odd = false;
+        if (has_even) { load(ahead, even); ahead.next(); }
+        has_odd = ahead.valid();
+        if (has_odd) { load(ahead, odd); ahead.next(); }
         while (has_even) {
             if (!store(even)) break;
-            if ((has_even = ahead.valid(p))) { load(ahead, even); ahead.next(p, num_pairs); }
+            if ((has_even = ahead.valid())) { load(ahead, even); ahead.next(); }
             if (!has_odd || !store(odd)) break;
-            if ((has_odd = ahead.valid(p))) { load(ahead, odd); ahead.next(p, num_pairs); }
+            if ((has_odd = ahead.valid())) { load(ahead, odd); ahead.next(); }
         }
     } else {
         const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
@@ -520,6 +545,23 @@ bool line_map(CUtensorMap &map, const void *base, uint64_t lines, uint32_t box_r
                               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Launches as the dependent of the kernel before on the stream, which by construction is this library's own (it prepares A) and no
+// dependent itself: everything before that one has finished.
+template <typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), uint32_t grid, int threads, int smem, cudaStream_t stream, const Args &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <bool kBf16>
 cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t stream) {
     auto kernel = gemm_mx_pair_kernel<kBf16>;
@@ -546,14 +588,13 @@ cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t
     uint32_t pairs = dev.tiles_m * dev.tiles_n, most = (uint32_t)max_pairs[d];
     if (usable_sms() > 1 && (uint32_t)usable_sms() / 2 < most) most = (uint32_t)usable_sms() / 2;
     if (pairs > most) pairs = most;
-    kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(maps, dev);
-    return cudaGetLastError();
+    return launch_dependent(kernel, 2 * pairs, kPairThreads, kPairSmem, stream, maps, dev);
 }
 
-template <int kBN, int kStages, bool kBf16>
+template <int kBN, int kARows, bool kBf16>
 cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
-    using P = Plan<kBN, kStages>;
-    auto kernel = gemm_mx_kernel<kBN, kStages, kBf16>;
+    using P = Plan<kBN, kARows>;
+    auto kernel = gemm_mx_kernel<kBN, kARows, kBf16>;
     static bool configured[64] = {false};
     int d = 0;
     cudaGetDevice(&d);
@@ -563,8 +604,13 @@ cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream
         configured[d] = true;
     }
     const uint32_t grid = (uint32_t)(max_tiles < (uint64_t)usable_sms() ? max_tiles : (uint64_t)usable_sms());
-    kernel<<<grid, kThreads, P::kTotal, stream>>>(dev);
-    return cudaGetLastError();
+    return launch_dependent(kernel, grid, kThreads, P::kTotal, stream, dev);
+}
+
+template <int kARows, bool kBf16>
+cudaError_t launch_by_width(int bn, const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
+    if (bn == 64) return launch<64, kARows, kBf16>(dev, max_tiles, stream);
+    return launch<128, kARows, kBf16>(dev, max_tiles, stream);
 }
 
 } // namespace
@@ -581,7 +627,6 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     // Tensor maps address lines of 128 bytes with 31-bit coordinates.
     const uint64_t most_chunks = 0x7fffff00ull / (kMxChunkBytes / 128);
     if ((args.m / 128 + 2) * (args.k / 256 + 1) > most_chunks || (args.n / 128 + 2) * (args.k / 256 + 1) > most_chunks) return cudaErrorInvalidValue;
-    constexpr int kBN = 128, kStages = 5;
     MxGemmDev dev;
     dev.a_chunks = static_cast<const uint8_t *>(args.a_chunks);
     dev.b_chunks = static_cast<const uint8_t *>(args.b_chunks);
@@ -592,7 +637,6 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.kblocks = (uint32_t)((args.k + kMxChunkValues - 1) / kMxChunkValues);
     dev.group_blocks = (uint32_t)((args.n + kChunkRows - 1) / kChunkRows);
     dev.tiles_m = (uint32_t)((args.m + kBM - 1) / kBM);
-    dev.tiles_n = (uint32_t)((args.n + kBN - 1) / kBN);
     dev.tiles = args.tiles;
     dev.tile_count = args.tile_count;
     dev.row_dest = args.row_dest;
@@ -622,9 +666,16 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
         return args.c_bf16 ? launch_pair<true>(maps, dev, stream) : launch_pair<false>(maps, dev, stream);
     }
     if (args.a_codes) return cudaErrorInvalidValue;
-    const uint64_t tiles = (args.tiles ? args.max_tiles : dev.tiles_m) * (uint64_t)dev.tiles_n;
+    // Narrower tiles while the wide ones are fewer than the SMs: a product with few rows is bound by the packed matrix's bytes, and every SM
+    // that streams some of it counts. Sums run over the depth in the same order whatever the tile.
+    const uint64_t row_tiles = args.tiles ? args.max_tiles : dev.tiles_m;
+    int bn = 128;
+    if (row_tiles * ((args.n + bn - 1) / bn) * 4 < (uint64_t)usable_sms() * 3) bn = 64;
+    dev.tiles_n = (uint32_t)((args.n + bn - 1) / bn);
+    const uint64_t tiles = row_tiles * dev.tiles_n;
     if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-    return args.c_bf16 ? launch<kBN, kStages, true>(dev, tiles, stream) : launch<kBN, kStages, false>(dev, tiles, stream);
+    if (!args.tiles && args.m <= 16) return args.c_bf16 ? launch_by_width<16, true>(bn, dev, tiles, stream) : launch_by_width<16, false>(bn, dev, tiles, stream);
+    return args.c_bf16 ? launch_by_width<128, true>(bn, dev, tiles, stream) : launch_by_width<128, false>(bn, dev, tiles, stream);
 }
 
 } // namespace nkb

@@ -49,8 +49,12 @@ public:
         stride = pitch;
         return d;
     }
-    // Whether a packed blob or a workspace may be used here.
-    bool usable(const void *p) { return !p || place(p); }
+    // Where a packed blob or a workspace lives; false when it may not be used here.
+    bool look(const void *p, MemKind &kind) {
+        if (!place(p)) return false;
+        kind = on_device_ ? kMemDevice : kMemHost;
+        return true;
+    }
     // Vectors: one dense row.
     const uint8_t *in(const void *p, uint64_t bytes) { uint64_t s = bytes; return in(p, 1, bytes, s); }
     uint8_t *out(void *p, uint64_t bytes) { uint64_t s = bytes; return out(p, 1, bytes, s); }
@@ -107,9 +111,11 @@ uint64_t chunk_bytes(uint64_t rows, uint64_t depth) { return mx_geometry(1, rows
 
 constexpr uint64_t kMostRows = 0x7fffff00ull;  // indices inside the kernels are 32 bits wide
 
-uint8_t *workspace_or_scratch(void *workspace, uint64_t bytes) {
+uint8_t *workspace_or_scratch(Operands &ops, void *workspace, uint64_t bytes) {
     if (!workspace) return static_cast<uint8_t *>(scratch(kSlotA, bytes));
-    if (classify(workspace) != kMemDevice || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
+    MemKind kind;
+    if (!ops.look(workspace, kind)) return nullptr;
+    if (kind != kMemDevice || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
         refuse("the workspace must be device memory on a 256-byte boundary");
         return nullptr;
     }
@@ -148,8 +154,8 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(1, n, k);
-    const MemKind packed_kind = classify(packed);
-    if (!ops.usable(packed) || !ops.usable(workspace)) return fail();
+    MemKind packed_kind;
+    if (!ops.look(packed, packed_kind)) return fail();
     const uint8_t *blob = resident_blob_of_size(packed, packed_kind, kMagicMx, kMxfp4, n, k, g.total_bytes, nullptr);
     unsigned int *err = blob ? device_error_word() : nullptr;
     if (!err) { if (blob) refuse("could not allocate the device error word"); return fail(); }
@@ -157,7 +163,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     bool ok = c_dev != nullptr;
     if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_stride, 0, row_bytes, m, stream), "clear result");
     else if (ok) {
-        uint8_t *chunks = workspace_or_scratch(workspace, chunk_bytes(m, k));
+        uint8_t *chunks = workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
         ok = chunks != nullptr;
         bool rows_in_place = false;
         const uint8_t *cd = nullptr;
@@ -258,7 +264,8 @@ NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void
     h.nonce = fresh_nonce(); h.reserved[0] = groups;
     cudaStream_t stream = current_stream();
     Operands ops(stream);
-    if (!ops.usable(packed)) return;
+    MemKind looked;
+    if (!ops.look(packed, looked)) return;
     uint8_t *blob = static_cast<uint8_t *>(packed);
     if (out_kind == kMemHost) {
         void *d = nullptr;
@@ -370,8 +377,8 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(experts, width, depth);
-    const MemKind packed_kind = classify(b_packed);
-    if (!ops.usable(b_packed) || !ops.usable(workspace)) return fail();
+    MemKind packed_kind;
+    if (!ops.look(b_packed, packed_kind)) return fail();
     const uint8_t *blob = resident_blob_of_size(b_packed, packed_kind, kMagicMx, kMxfp4, experts * width, depth, g.total_bytes, nullptr);
     unsigned int *err = blob ? device_error_word() : nullptr;
     if (!err) { if (blob) refuse("could not allocate the device error word"); return fail(); }
@@ -380,7 +387,7 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
     if (ok && depth == 0) ok = cuda_ok(cudaMemset2DAsync(dst, out_stride, 0, row_bytes, rows, stream), "clear result");
     else if (ok) {
         const ExpertsLayout l = experts_layout(slots, experts, width, depth, weights != nullptr);
-        uint8_t *ws = workspace_or_scratch(workspace, l.total);
+        uint8_t *ws = workspace_or_scratch(ops, workspace, l.total);
         const int32_t *id = ws ? reinterpret_cast<const int32_t *>(ops.in(ids, slots * 4)) : nullptr;
         const uint8_t *xd = id ? ops.in(x, x_rows, depth * dtype_bytes(x_type), x_stride) : nullptr;
         const float *wd = xd && weights ? reinterpret_cast<const float *>(ops.in(weights, slots * 4)) : nullptr;

@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include "nkb_decode.cuh"
 #include "nkb_mx.h"
+#include "nkb_ptx.cuh"
 
 namespace nkb {
 
@@ -70,6 +71,7 @@ template <uint32_t kType, bool kTiled>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, uint64_t rows, uint64_t depth, uint64_t x_stride, RowMajorSink out,
                                                             uint8_t *chunks, uint32_t depth_blocks, const int32_t *row_dest, const int32_t *tile_count,
                                                             uint32_t divide) {
+    if constexpr (kTiled) allow_next_kernel();  // the product that reads the chunks may set itself up meanwhile
     if (kTiled && row_dest) rows = (uint64_t)*tile_count * kChunkRows;
     constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
@@ -176,6 +178,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
 __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
                                                         uint64_t width, uint64_t depth, uint64_t tiled_rows, uint32_t group_rows, uint8_t *chunks,
                                                         uint32_t depth_blocks) {
+    allow_next_kernel();
     const int lane = threadIdx.x & 31;
     const uint64_t row_bytes = (depth + 1) / 2, row_scales = (depth + kMxBlock - 1) / kMxBlock;
     const uint64_t items = tiled_rows * depth_blocks, step = (uint64_t)gridDim.x * (kThreads / 32);
@@ -209,6 +212,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, ui
 // threads of a warp walk the words of one row, so that the reads are whole lines.
 __global__ void __launch_bounds__(kThreads) tile_scales_kernel(const uint8_t *scales, uint64_t scales_stride, uint64_t rows, uint64_t depth,
                                                                uint64_t row_blocks, uint32_t words, uint8_t *tiles) {
+    allow_next_kernel();
     const uint64_t row_scales = (depth + kMxBlock - 1) / kMxBlock, items = row_blocks * 32 * words;
     const bool aligned = ((reinterpret_cast<uintptr_t>(scales) | scales_stride) & 3u) == 0;
     for (uint64_t item = (uint64_t)blockIdx.x * kThreads + threadIdx.x; item < items; item += (uint64_t)gridDim.x * kThreads) {
