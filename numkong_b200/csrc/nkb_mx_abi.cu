@@ -151,6 +151,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     if ((m > 1 && c_stride < row_bytes) || (reinterpret_cast<uintptr_t>(c) | c_stride) % cell) { refuse("mxfp4 product: rows of the result overlap or are not aligned to its cells"); return fail(); }
     const uint64_t kblocks = (k + kMxBlock - 1) / kMxBlock;
     if (m > 1 && (codes ? codes_stride < (k + 1) / 2 || scales_stride < kblocks : a_stride < k * dtype_bytes(a_type))) { refuse("mxfp4 product: rows of A overlap"); return fail(); }
+    if (!codes && (reinterpret_cast<uintptr_t>(a) | (m > 1 ? a_stride : 0)) % dtype_bytes(a_type)) { refuse("mxfp4 product: values of A are not aligned to their type"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(1, n, k);
@@ -176,7 +177,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
             else ok = sd && cuda_ok(launch_mx_tile(cd, codes_stride, sd, scales_stride, 1, m, k, false, chunks, stream), "tile kernel");
         } else if (ok) {
             const uint8_t *ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
-            ok = ad && cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, a_stride, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
+            ok = ad && cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
         }
         if (ok) {
             MxGemmArgs args;
@@ -211,6 +212,7 @@ NKB_API void nkb_mx_quantise(void const *x, uint32_t x_type, nk_size_t rows, nk_
     if (!float_type(x_type) || !x || !codes || !scales) { refuse("mx_quantise: unsupported element type or null pointer"); return fail(); }
     if (rows > kMostRows || depth > kMostRows) { refuse("mx_quantise: a size does not fit 31 bits"); return fail(); }
     if (rows > 1 && (x_stride < depth * dtype_bytes(x_type) || codes_stride < code_bytes || scales_stride < blocks)) { refuse("mx_quantise: rows overlap"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | x_stride) % dtype_bytes(x_type)) { refuse("mx_quantise: values are not aligned to their type"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *xd = ops.in(x, rows, depth * dtype_bytes(x_type), x_stride);
@@ -231,6 +233,7 @@ NKB_API void nkb_mx_dequantise(void const *codes, nk_size_t codes_stride, void c
     if (!x || !codes || !scales) { refuse("mx_dequantise: null pointer"); return fail(); }
     if (rows > kMostRows || depth > kMostRows) { refuse("mx_dequantise: a size does not fit 31 bits"); return fail(); }
     if (rows > 1 && (x_stride < row_bytes || codes_stride < code_bytes || scales_stride < blocks)) { refuse("mx_dequantise: rows overlap"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | x_stride) % dtype_bytes(x_type)) { refuse("mx_dequantise: values are not aligned to their type"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *cd = ops.in(codes, rows, code_bytes, codes_stride), *sd = cd ? ops.in(scales, rows, blocks, scales_stride) : nullptr;
@@ -373,7 +376,7 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
     if (experts == 0 || experts > kRouteMaxExperts) { refuse("experts: 1 to 1024 experts"); return fail(); }
     if (tokens > kMostRows || top > 1024 || slots > kMostRows / 2 || width > kMostRows || depth > kMostRows) { refuse("experts: a size does not fit 31 bits"); return fail(); }
     if ((x_rows > 1 && x_stride < depth * dtype_bytes(x_type)) || (rows > 1 && out_stride < row_bytes)) { refuse("experts: rows overlap"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(out) | out_stride) % cell || (reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) % 4) { refuse("experts: operands are not aligned to their elements"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | (x_rows > 1 ? x_stride : 0)) % dtype_bytes(x_type) || (reinterpret_cast<uintptr_t>(out) | out_stride) % cell || (reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) % 4) { refuse("experts: operands are not aligned to their elements"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(experts, width, depth);
@@ -403,7 +406,7 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
             args.m = slots; args.n = width; args.k = depth;
             args.tiles = tiles; args.tile_count = count; args.row_dest = dest; args.max_tiles = l.max_tiles; args.error_word = err;
             ok = cuda_ok(launch_expert_order(id, slots, (uint32_t)experts, tiles, count, dest, l.max_tiles, stream), "expert order kernel") &&
-                 cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, x_stride, l.max_tiles * kChunkRows, dest, count, per_slot ? 1u : (uint32_t)top, ws + l.chunks, stream), "quantise kernel") &&
+                 cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, x_rows > 1 ? x_stride : 0, l.max_tiles * kChunkRows, dest, count, per_slot ? 1u : (uint32_t)top, ws + l.chunks, stream), "quantise kernel") &&
                  cuda_ok(launch_gemm_mx(args, stream), "grouped mxfp4 GEMM kernel");
             if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, (uint32_t)experts, width, dst, out_type == kBF16, out_stride, stream), "combine kernel");
             else if (ok) ok = cuda_ok(launch_zero_unrouted(id, slots, (uint32_t)experts, dst, row_bytes, out_stride, stream), "zero kernel");
