@@ -13,33 +13,54 @@ namespace {
 
 constexpr int kOrderThreads = 1024;
 
+// One block: slots are counted per expert in shared memory, a scan over the experts gives every expert its tiles, and a second pass
+// over the slots takes the places. 16,384 slots of 32 experts.
 __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t *ids, uint32_t slots, uint32_t experts, MxRowTile *tiles,
                                                                      int32_t *tile_count, int32_t *row_dest) {
-    __shared__ uint32_t count[kRouteMaxExperts], first_tile[kRouteMaxExperts + 1], taken[kRouteMaxExperts];
-    for (uint32_t e = threadIdx.x; e < experts; e += kOrderThreads) { count[e] = 0; taken[e] = 0; }
+    static_assert(kRouteMaxExperts <= kOrderThreads, "one thread per expert");
+    __shared__ uint32_t count[kRouteMaxExperts], next_row[kRouteMaxExperts], warp_sums[kOrderThreads / 32];
+    const uint32_t t = threadIdx.x, lane = t & 31u;
+    if (t < experts) count[t] = 0;
     __syncthreads();
-    for (uint32_t s = threadIdx.x; s < slots; s += kOrderThreads) {
+    for (uint32_t s = t; s < slots; s += kOrderThreads) {
         const int32_t e = ids[s];
         if (e >= 0 && e < (int32_t)experts) atomicAdd(&count[e], 1u);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        uint32_t next = 0;
-        for (uint32_t e = 0; e < experts; ++e) { first_tile[e] = next; next += (count[e] + 127u) / 128u; }
-        first_tile[experts] = next;
-        *tile_count = (int32_t)next;
+    const uint32_t mine = t < experts ? count[t] : 0u, my_tiles = (mine + 127u) / 128u;
+    uint32_t through = my_tiles;  // inclusive sum over the experts
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, through, o);
+        if ((int)lane >= o) through += v;
+    }
+    if (lane == 31u) warp_sums[t >> 5] = through;
+    __syncthreads();
+    if (t < 32) {
+        uint32_t w = warp_sums[t];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, w, o);
+            if ((int)lane >= o) w += v;
+        }
+        warp_sums[t] = w;
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < experts; e += kOrderThreads)
-        for (uint32_t t = first_tile[e], left = count[e]; t < first_tile[e + 1]; ++t, left -= 128u) {
-            tiles[t].group = (int32_t)e;
-            tiles[t].rows = (int32_t)min(left, 128u);
-        }
-    for (uint32_t i = threadIdx.x; i < first_tile[experts] * 128u; i += kOrderThreads) row_dest[i] = -1;
+    if (t >= 32) through += warp_sums[(t >> 5) - 1];
+    if (t == kOrderThreads - 1) *tile_count = (int32_t)through;
+    if (t < experts) {
+        uint32_t tile = through - my_tiles, left = mine;
+        next_row[t] = tile * 128u;
+        for (; tile < through; ++tile, left -= 128u) tiles[tile] = {(int32_t)t, (int32_t)min(left, 128u)};
+    }
     __syncthreads();
-    for (uint32_t s = threadIdx.x; s < slots; s += kOrderThreads) {
+    // Rows behind an expert's last slot belong to nobody.
+    for (uint32_t e = t >> 5; e < experts; e += kOrderThreads / 32)
+        for (uint32_t r = count[e] + lane; r < (count[e] + 127u) / 128u * 128u; r += 32) row_dest[next_row[e] + r] = -1;
+    __syncthreads();
+    for (uint32_t s = t; s < slots; s += kOrderThreads) {
         const int32_t e = ids[s];
-        if (e >= 0 && e < (int32_t)experts) row_dest[first_tile[e] * 128u + atomicAdd(&taken[e], 1u)] = (int32_t)s;
+        if (e >= 0 && e < (int32_t)experts) row_dest[atomicAdd(&next_row[e], 1u)] = (int32_t)s;
     }
 }
 
@@ -52,19 +73,40 @@ __global__ void __launch_bounds__(256) zero_unrouted_kernel(const int32_t *ids, 
     }
 }
 
+// One block per token and stretch of columns: the token's ids and weights are the same for all its threads, and four columns a
+// thread keep `top` loads of 16 bytes in flight. Bound by memory: y is read once and the sums are written.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) combine_kernel(const float *y, const float *weights, const int32_t *ids, uint64_t tokens, uint32_t top, uint32_t experts,
-                                                      uint64_t width, uint8_t *out, uint64_t out_stride) {
-    const uint64_t items = tokens * width;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t t = i / width, c = i - t * width;
-        float sum = 0.0f;
-        for (uint32_t j = 0; j < top; ++j) {
-            const int32_t e = ids[t * top + j];
-            if (e >= 0 && e < (int32_t)experts) sum = fmaf(weights[t * top + j], y[(t * top + j) * width + c], sum);
+__global__ void __launch_bounds__(256) combine_kernel(const float *y, const float *weights, const int32_t *ids, uint32_t top, uint32_t experts,
+                                                      uint64_t width, uint8_t *out, uint64_t out_stride, bool vectors) {
+    const uint64_t t = blockIdx.x;
+    const float *rows = y + t * top * width;
+    const float *w = weights + t * top;
+    const int32_t *id = ids + t * top;
+    if (vectors) {
+        for (uint64_t c = ((uint64_t)blockIdx.y * 256 + threadIdx.x) * 4; c < width; c += (uint64_t)gridDim.y * 1024) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (uint32_t j = 0; j < top; ++j) {
+                if ((uint32_t)id[j] >= experts) continue;  // none below 0 either
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(rows + j * width + c));
+                const float f = w[j];
+                sum = make_float4(fmaf(f, v.x, sum.x), fmaf(f, v.y, sum.y), fmaf(f, v.z, sum.z), fmaf(f, v.w, sum.w));
+            }
+            if constexpr (kBf16) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+                *reinterpret_cast<uint2 *>(out + t * out_stride + c * 2) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+            } else {
+                *reinterpret_cast<float4 *>(out + t * out_stride + c * 4) = sum;
+            }
         }
-        if constexpr (kBf16) reinterpret_cast<__nv_bfloat16 *>(out + t * out_stride)[c] = __float2bfloat16_rn(sum);
-        else reinterpret_cast<float *>(out + t * out_stride)[c] = sum;
+    } else {
+        for (uint64_t c = (uint64_t)blockIdx.y * 256 + threadIdx.x; c < width; c += (uint64_t)gridDim.y * 256) {
+            float sum = 0.0f;
+            for (uint32_t j = 0; j < top; ++j)
+                if ((uint32_t)id[j] < experts) sum = fmaf(w[j], rows[j * width + c], sum);
+            if constexpr (kBf16) reinterpret_cast<__nv_bfloat16 *>(out + t * out_stride)[c] = __float2bfloat16_rn(sum);
+            else reinterpret_cast<float *>(out + t * out_stride)[c] = sum;
+        }
     }
 }
 
@@ -86,10 +128,12 @@ cudaError_t launch_zero_unrouted(const int32_t *ids, uint64_t slots, uint32_t ex
 
 cudaError_t launch_combine(const float *y, const float *weights, const int32_t *ids, uint64_t tokens, uint32_t top, uint32_t experts, uint64_t width,
                            void *out, bool bf16, uint64_t out_stride, cudaStream_t stream) {
-    const uint32_t grid = blocks_for((tokens * width + 255) / 256);
     uint8_t *dst = static_cast<uint8_t *>(out);
-    if (bf16) combine_kernel<true><<<grid, 256, 0, stream>>>(y, weights, ids, tokens, top, experts, width, dst, out_stride);
-    else combine_kernel<false><<<grid, 256, 0, stream>>>(y, weights, ids, tokens, top, experts, width, dst, out_stride);
+    const bool vectors = width % 4 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out) | (tokens > 1 ? out_stride : 0)) & 15u) == 0;
+    const uint64_t stretches = (width + (vectors ? 1023 : 255)) / (vectors ? 1024 : 256);
+    const dim3 grid((uint32_t)tokens, (uint32_t)(stretches < 4096 ? stretches : 4096));
+    if (bf16) combine_kernel<true><<<grid, 256, 0, stream>>>(y, weights, ids, top, experts, width, dst, out_stride, vectors);
+    else combine_kernel<false><<<grid, 256, 0, stream>>>(y, weights, ids, top, experts, width, dst, out_stride, vectors);
     return cudaGetLastError();
 }
 

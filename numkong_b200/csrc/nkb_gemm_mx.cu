@@ -3,13 +3,14 @@
 //
 //   C[i, j] = sum over blocks b of 2^(sa[i,b] + sb[j,b] - 254) * sum over the block's 32 values of a_l b_l
 //
-// tcgen05.mma.kind::mxf4 takes 64 values of depth a step and applies the scales inside: the scales come from TMEM, where
-// tcgen05.cp puts the chunk's scale tiles just before the chunk's MMAs (both run in the order one thread issues them).
+// tcgen05.mma.kind::mxf4 takes 64 values of depth a step and applies the scales inside: the scales come from TMEM. Four warps,
+// one for each 32-lane quarter, bring a chunk's scale tiles there through registers (tcgen05.st) beside the MMAs. tcgen05.cp would
+// bring them from shared memory in one instruction, but runs in the queue of the MMAs and costs them about 46 cycles a tile.
 // e2m1 products are multiples of 1/4 of at most 36, so a block's sum is exact and the accumulator only loses bits when the
 // block scales of a row spread over more than 2^10.
 //
-// One persistent CTA per SM, ten warps, as in the packed GEMM of the other types: warp 0 brings chunks to shared memory with
-// untiled bulk copies, warp 1 issues copies of scales and MMAs, warps 2..9 read the accumulators out and store the cells.
+// One persistent CTA per SM, fourteen warps: warp 0 brings chunks to shared memory with untiled bulk copies, warp 1 issues the
+// MMAs, warps 2..9 read the accumulators out and store the cells, warps 10..13 store scales.
 #include <cuda_bf16.h>
 #include "nkb_mx.h"
 #include "nkb_ptx.cuh"
@@ -20,7 +21,8 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kScaleWarps = 4;
+constexpr int kThreads = 64 + 32 * (kEpilogueWarps + kScaleWarps);
 constexpr uint32_t kMxChunkLines = kMxChunkBytes / 128;  // a chunk as rows of 128 bytes: 128 of codes, 8 of scales
 constexpr uint32_t kGroupM = 8;      // row tiles walked before the next column tile
 
@@ -150,9 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     using P = Plan<kBN, kARows>;
     constexpr int kStages = P::kStages;
     constexpr int kColsPerThread = kBN / 2;
-    constexpr int kScaleCols = 16;                           // one chunk's scales: eight columns for 128 rows of A, eight for the row block of B
-    constexpr int kTmemCols = 2 * kBN + kScaleCols <= 256 ? 256 : 512;
-    static_assert(2 * kBN + kScaleCols <= kTmemCols, "two accumulators and the scales fit TMEM");
+    constexpr int kScaleCols = 16;  // one chunk's scales: eight columns for 128 rows of A, eight for the row block of B
+    static_assert(2 * kBN + kStages * kScaleCols <= 512, "two accumulators and every stage's scales fit TMEM");
     static_assert(kBN == 64 || kBN == 128, "a tile's scales begin on an even TMEM column");
 
     extern __shared__ uint8_t smem_raw[];
@@ -161,20 +162,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     const uint32_t bar_base = smem_base + P::kBarrierOffset;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
-    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * kStages + a); };
-    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (2 * kStages + 2 + a); };
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + P::kBarrierOffset + 8 * (2 * kStages + 4));
-    const uint32_t drain_bar = bar_base + 8u * (2 * kStages + 5);
+    auto scale_bar = [&](int s) { return bar_base + 8u * (2 * kStages + s); };  // the stage's scales are in TMEM
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (3 * kStages + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (3 * kStages + 2 + a); };
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + P::kBarrierOffset + 8 * (3 * kStages + 4));
+    const uint32_t drain_bar = bar_base + 8u * (3 * kStages + 5);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), kScaleWarps); }
         for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(tmem_empty_bar(a), kEpilogueWarps * 32); }
         mbar_init(drain_bar, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t *>(tmem_slot)), kTmemCols);
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
         tmem_relinquish<1>();
     }
     tc_fence_before_sync();
@@ -234,29 +236,24 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             int stage = 0;
             uint32_t phase = 0, seq = 0;
             bool ok = true;
-            const uint32_t scales_a = tmem_base + 2 * kBN, scales_b = scales_a + 8;
             for (uint32_t tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++seq) {
                 uint32_t mt, nt;
                 tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
-                const uint32_t b_column = scales_b + nt * kBN % 128u / 32u;  // the tile's rows inside the row block's scales
+                const uint32_t b_column = 8u + nt * kBN % 128u / 32u;  // the tile's rows inside the row block's scales
                 const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
                 if (!mbar_wait(tmem_empty_bar(buf), buf_phase ^ 1u, 2, p.error_word, p.wait_us[2])) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + buf * kBN;
                 for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-                    if (!mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
+                    if (!mbar_wait(scale_bar(stage), phase, 3, p.error_word, p.wait_us[3]) ||
+                        !mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
                     tc_fence_after_sync();
-                    const uint32_t src = smem_base + P::kBRing + stage * P::kStageBytes;
+                    const uint32_t src = smem_base + P::kBRing + stage * P::kStageBytes, scales = tmem_base + 2 * kBN + stage * kScaleCols;
                     const uint64_t a_desc = make_smem_desc_sw128(smem_base + stage * P::kABytes), b_desc = make_smem_desc_sw128(src);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {  // two scale tiles, 128 values of depth each
-                        tmem_copy_scales<1>(scales_a + t * 4, make_smem_desc_scales(src + P::kBBytes + t * 512));
-                        tmem_copy_scales<1>(scales_b + t * 4, make_smem_desc_scales(src + P::kBBytes + kMxScaleBytes + t * 512));
-                    }
-#pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_mxf4<1>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(kBM, kBN, (k & 1) * 2), scales_a + (k >> 1) * 4,
-                                     b_column + (k >> 1) * 4, (kb | (uint32_t)k) != 0u);
+                        umma_mxf4<1>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(kBM, kBN, (k & 1) * 2), scales + (k >> 1) * 4,
+                                     scales + b_column + (k >> 1) * 4, (kb | (uint32_t)k) != 0u);
                     umma_commit(empty_bar(stage));
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -264,6 +261,28 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             }
             umma_commit(drain_bar);  // shared memory and TMEM are released below: the last MMAs must have retired
             mbar_wait(drain_bar, 0u, 5, p.error_word, p.wait_us[5]);
+        }
+    } else if (warp >= 2 + kEpilogueWarps) {
+        // ------------------------------------------------------------ scales: shared memory -> this warp's 32-lane quarter of TMEM
+        // A stage has TMEM columns of its own, free again when the stage is.
+        const uint32_t column = tmem_base + (((uint32_t)warp & 3u) * 32u << 16) + 2 * kBN;
+        int stage = 0;
+        uint32_t phase = 0;
+        for (Walk w(blockIdx.x, gridDim.x, tiles_m, p.tiles_n, p.kblocks); w.valid(); w.next()) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3]))) break;
+            tc_fence_after_sync();
+            const uint4 *tiles = reinterpret_cast<const uint4 *>(smem_gen + P::kBRing + stage * P::kStageBytes + P::kBBytes) + lane;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 lo = tiles[i * 64], hi = tiles[i * 64 + 32];
+                const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                tmem_st_32x8(column + stage * kScaleCols + i * 8, words);
+            }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(scale_bar(stage));
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
     } else {
         const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc<1>(tmem_base, kTmemCols);
+        tmem_dealloc<1>(tmem_base, 512);
     }
 }
 
@@ -307,12 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
 // [512 - scales - 256, 512 - scales). The epilogue reads the columns they share first and then lets the next tile's MMAs
 // start, so they wait for a part of a read-out instead of all of it.
 //
-// The scales reach TMEM from registers: four warps per CTA, one for each 32-lane quarter, load a chunk's scale tiles two chunks
-// ahead and store them (tcgen05.st) beside the MMAs. tcgen05.cp, which the single-CTA kernel uses, runs in the queue of the MMAs and
-// costs them about 46 cycles a tile, six tiles a chunk: 253 us against 215 without any at 8192 x 8192 x 8192.
+// The scale warps load a chunk's scale tiles from global memory two chunks ahead. With tcgen05.cp in their place (six tiles a
+// chunk) 8192 x 8192 x 8192 took 253 us, with no scales moved at all 215.
 constexpr int kPairStages = 5;
-constexpr int kPairScaleWarps = 4;
-constexpr int kPairThreads = kThreads + 32 * kPairScaleWarps;
 constexpr int kPairScaleCols = 24;                                // 8 for 128 rows of A, 16 for 256 of B
 constexpr int kPairSecond = 512 - 2 * kPairScaleCols - 256;       // first column of the second accumulator; two chunks' scales behind it
 constexpr int kPairBOffset = kBM * 128;
@@ -328,7 +344,7 @@ struct PairMaps {
 };
 
 template <bool kBf16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
     constexpr int kStages = kPairStages;
     extern __shared__ uint8_t smem_raw[];
@@ -350,7 +366,7 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
         prefetch_tensormap(&maps.a);
         prefetch_tensormap(&maps.b);
         for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(scale_bar(a), 2 * kPairScaleWarps); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(scale_bar(a), 2 * kScaleWarps); }
         mbar_init(shared_read_bar, 2 * kEpilogueWarps);
         mbar_init(drain_bar, 1);
         fence_mbar_init();
@@ -574,7 +590,7 @@ cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * (sm_count() / 2));
-        cfg.blockDim = dim3(kPairThreads);
+        cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = kPairSmem;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
@@ -588,7 +604,7 @@ cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t
     uint32_t pairs = dev.tiles_m * dev.tiles_n, most = (uint32_t)max_pairs[d];
     if (usable_sms() > 1 && (uint32_t)usable_sms() / 2 < most) most = (uint32_t)usable_sms() / 2;
     if (pairs > most) pairs = most;
-    return launch_dependent(kernel, 2 * pairs, kPairThreads, kPairSmem, stream, maps, dev);
+    return launch_dependent(kernel, 2 * pairs, kThreads, kPairSmem, stream, maps, dev);
 }
 
 template <int kBN, int kARows, bool kBf16>

@@ -7,7 +7,7 @@
 //
 // Tile form: a chunk is 128 rows x 256 values. Its first 16 KiB are the codes, 128 bytes per row, in the 128-byte-swizzled
 // K-major image tcgen05.mma reads (as in PackedHeader); then two 512-byte scale tiles, one per 128 values of depth, each the
-// image tcgen05.cp copies to TMEM: the four scales of row r at byte (r % 32) * 16 + (r / 32) * 4. One bulk copy brings a
+// image the MMA's scales take in TMEM: the four scales of row r at byte (r % 32) * 16 + (r / 32) * 4 (lane r % 32, column r / 32). One bulk copy brings a
 // chunk to shared memory with nothing left to rearrange. Chunks are ordered [row block][depth block], so that a CTA that
 // stays on one row block reads one contiguous stream.
 #pragma once

@@ -144,25 +144,36 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
             for (int u = 0; u < kAhead; ++u) {
                 if (u >= (int)count) break;
                 float v[8];
-#pragma unroll
-                for (int h = 0; h < kBytes / 2; ++h) {
-                    const uint32_t w[4] = {raw[u][h].x, raw[u][h].y, raw[u][h].z, raw[u][h].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (kType == kF32) v[4 * h + i] = __uint_as_float(w[i]);
-                        else { v[2 * i] = decode_bits<kType>(w[i] & 0xffffu); v[2 * i + 1] = decode_bits<kType>(w[i] >> 16); }
-                    }
-                }
                 uint32_t largest = 0;
+                if constexpr (kType == kBF16) {
+                    // Two values an instruction: the order of bf16 magnitudes is that of their bits, and scaling by a power of two is exact
+                    // (or ends below the smallest code).
+                    const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
+                    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+                    largest = max(m << 16, m & 0xffff0000u);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);
+                    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < kBytes / 2; ++h) {
+                        const uint32_t w[4] = {raw[u][h].x, raw[u][h].y, raw[u][h].z, raw[u][h].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kType == kF32) v[4 * h + i] = __uint_as_float(w[i]);
+                            else { v[2 * i] = decode_bits<kType>(w[i] & 0xffffu); v[2 * i + 1] = decode_bits<kType>(w[i] >> 16); }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);
+                }
                 largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                 largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
                 const uint32_t s = scale_byte(largest);
-                const float inverse = s == 255u ? 0.0f : inverse_scale(s);
+                const float inverse = inverse_scale(min(s, 253u));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = s == 255u ? 0.0f : v[i] * inverse;
-                store_chunk_row<kTiled>(encode8(v), piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
+                for (int i = 0; i < 8; ++i) v[i] *= inverse;
+                const uint32_t codes = s == 255u ? 0u : encode8(v);
+                store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
                 const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
                 if ((lane >> 3) == u) my_scale = mine;
             }

@@ -275,21 +275,6 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint
     else NKB_UMMA_MX_ASM("2");
 #undef NKB_UMMA_MX_ASM
 }
-// Descriptor of a 512-byte scale tile in shared memory: 32 rows of 16 bytes, no swizzle, eight-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    return d;
-}
-// Copies one scale tile to four TMEM columns, into all four 32-lane quarters. Runs in order with the MMAs the same thread issues.
-template <int kCtaGroup>
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-    if constexpr (kCtaGroup == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

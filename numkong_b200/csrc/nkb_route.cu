@@ -80,6 +80,50 @@ __device__ __forceinline__ float exp_difference(float a, float b) {
     return lost == lost ? fmaf(expf(d), lost, expf(d)) : expf(d);  // the correction is NaN where the difference overflows
 }
 
+// 1 / x for a positive x in the range of f32, to 46 bits: a 32-bit start and one step of Newton's.
+__device__ __forceinline__ double reciprocal(double x) {
+    const double r = (double)__frcp_rn((float)x);
+    return r * fma(-x, r, 2.0);
+}
+// A chosen expert's score, up to the softmax's common factor, from one 32-bit exponential (off by two half units at most, the
+// rest is 64 bits). Sigmoids of logits below -80 need the 64-bit exponential: see the callers.
+__device__ __forceinline__ double fast_score(bool sigmoid, float l, float most) {
+    return sigmoid ? reciprocal(1.0 + (double)expf(-l)) : (double)exp_difference(l, most);
+}
+
+// The logits lane * kPer .. of a token's row, -infinity where there is none or it is masked.
+template <uint32_t kType, int kPer>
+__device__ __forceinline__ void load_logits(const uint8_t *row, uint32_t experts, int lane, float (&l)[kPer]) {
+    constexpr int kBytes = kType == kF32 ? 4 : 2, kLaneBytes = kPer * kBytes, kVector = kLaneBytes < 16 ? kLaneBytes : 16;
+    const uint32_t first = lane * kPer;
+    if (kVector >= 4 && first + kPer <= experts && (reinterpret_cast<uintptr_t>(row) & (kVector - 1)) == 0) {
+        uint32_t w[(kLaneBytes + 3) / 4];
+        const uint8_t *from = row + first * kBytes;
+        if constexpr (kVector == 16) {
+#pragma unroll
+            for (int i = 0; i < kLaneBytes / 16; ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from) + i);
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+        } else if constexpr (kVector == 8) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from));
+            w[0] = v.x; w[1] = v.y;
+        } else if constexpr (kVector == 4) {
+            w[0] = __ldg(reinterpret_cast<const uint32_t *>(from));
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            float v;
+            if constexpr (kType == kF32) v = __uint_as_float(w[i]);
+            else v = decode_bits<kType>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+            l[i] = v == v ? fminf(v, FLT_MAX) : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) l[i] = first + i < experts ? load_logit<kType>(row, first + i) : -INFINITY;
+    }
+}
+
 // The choice in 64 bits, for the tokens whose keys 32 bits leave undecided. `keys`: room for one key per expert. Returns lane j's choice.
 template <uint32_t kType>
 __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, float top_logit, double *keys, int lane) {
@@ -135,27 +179,26 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     return chosen;
 }
 
-// One warp per token; lane i holds the experts i, i + 32, ... in registers (kPer of them) and every round of the selection is one
-// integer maximum over the warp and one minimum over the indices that reach it.
+// One warp per token; lane i holds the experts i * kPer .. in registers. A round of the selection is one integer maximum over the
+// warp and a ballot for the lowest lane that reaches it; that lane alone takes its expert out and looks for its next best.
 //
 // Keys are computed in 32 bits with a bound on their error. Where every decision (chosen against next, open group against closed) is
-// wider than that bound, or is a tie of equal inputs, the choice is the one 64 bits would make; the other tokens, about one in a
-// hundred on random logits, go through choose_exactly. Keys that are the logits themselves (no bias, no groups) are exact.
-// 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: the exact way for every token took 73 us.
+// wider than that bound, or is a tie of equal inputs, the choice is the one 64 bits would make; the other tokens, a few in a
+// thousand on random logits, go through choose_exactly. Keys that are the logits themselves (no bias, no groups) are exact.
+// Bound by instructions. 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token in 64 bits.
 template <uint32_t kType, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, float *weights, int32_t *ids) {
     extern __shared__ double keys_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool direct = p.bias == nullptr && p.groups == 1;
-    const uint32_t size = p.experts / p.groups;
+    const uint32_t size = p.experts / p.groups, lanes = size / kPer;
+    const bool whole_lanes = size % kPer == 0 && (lanes & (lanes - 1)) == 0;  // a group is a power of two of lanes
     float bias[kPer], most_bias = 0.0f;
-    uint32_t group[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const uint32_t e = i * 32 + lane;
+        const uint32_t e = lane * kPer + i;
         bias[i] = e < p.experts ? load_bias(p.bias, e) : -INFINITY;
         if (bias[i] > -INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
-        group[i] = e / size;
     }
     most_bias = warp_max(most_bias);
     // Relative error of a score: exp and division a few units, the softmax's sum one more per addition. Scores are at most 1, and the
@@ -164,20 +207,19 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
     for (uint32_t token = blockIdx.x * kWarps + warp; token < p.tokens; token += gridDim.x * kWarps) {
         const uint8_t *row = p.logits + token * p.stride;
         float logit[kPer], top_logit = -INFINITY;
+        load_logits<kType, kPer>(row, p.experts, lane, logit);
+        if (!p.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const uint32_t e = i * 32 + lane;
-            logit[i] = e < p.experts ? load_logit<kType>(row, e) : -INFINITY;
-            top_logit = fmaxf(top_logit, logit[i]);
+            for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
+            top_logit = warp_max(top_logit);
         }
-        if (!p.sigmoid) top_logit = warp_max(top_logit);
         uint32_t key[kPer];
         if (direct) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) key[i] = ordered(logit[i]);
         } else if (p.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY && bias[i] > -INFINITY ? ordered(__fdividef(1.0f, 1.0f + expf(-logit[i])) + bias[i]) : 0u;
+            for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY && bias[i] > -INFINITY ? ordered(__fdividef(1.0f, 1.0f + __expf(-logit[i])) + bias[i]) : 0u;
         } else {
             float part[kPer], total = 0.0f;
 #pragma unroll
@@ -191,18 +233,35 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
         bool sure = true;
         if (p.groups > 1) {
             float worth = -INFINITY;  // lane g: group g's
-            for (uint32_t g = 0; g < p.groups; ++g) {
+            if (whole_lanes) {
                 uint32_t first = 0, second = 0;
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
-                    const uint32_t k = group[i] == g ? key[i] : 0u;
-                    second = max(second, min(first, k));
-                    first = max(first, k);
+                    second = max(second, min(first, key[i]));
+                    first = max(first, key[i]);
                 }
-                const uint32_t best = __reduce_max_sync(0xffffffffu, first);
-                const int holder = __ffs(__ballot_sync(0xffffffffu, first == best)) - 1;
-                const uint32_t next = __reduce_max_sync(0xffffffffu, lane == holder ? second : first);
-                if (lane == (int)g) worth = next ? from_ordered(best) + from_ordered(next) : from_ordered(best);
+                for (uint32_t o = 1; o < lanes; o <<= 1) {
+                    const uint32_t f = __shfl_xor_sync(0xffffffffu, first, o), n = __shfl_xor_sync(0xffffffffu, second, o);
+                    second = max(min(first, f), max(second, n));
+                    first = max(first, f);
+                }
+                const float mine = second ? from_ordered(first) + from_ordered(second) : from_ordered(first);
+                worth = __shfl_sync(0xffffffffu, mine, lane * lanes);
+                if ((uint32_t)lane >= p.groups) worth = -INFINITY;
+            } else {
+                for (uint32_t g = 0; g < p.groups; ++g) {
+                    uint32_t first = 0, second = 0;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) {
+                        const uint32_t e = lane * kPer + i, k = e >= g * size && e < (g + 1) * size ? key[i] : 0u;
+                        second = max(second, min(first, k));
+                        first = max(first, k);
+                    }
+                    const uint32_t best = __reduce_max_sync(0xffffffffu, first);
+                    const int holder = __ffs(__ballot_sync(0xffffffffu, first == best)) - 1;
+                    const uint32_t next = __reduce_max_sync(0xffffffffu, lane == holder ? second : first);
+                    if (lane == (int)g) worth = next ? from_ordered(best) + from_ordered(next) : from_ordered(best);
+                }
             }
             uint32_t rank = 0;
             for (uint32_t g = 0; g < p.groups; ++g) {
@@ -215,61 +274,79 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             // A worth is off by twice a key's error and a rounding.
             if (most_closed > -INFINITY && !(least_open - most_closed > 6.0f * slack)) sure = false;
             const uint32_t open_groups = __ballot_sync(0xffffffffu, open);
+            if (whole_lanes) {
+                const uint32_t group = lane / lanes;
+                if (!((open_groups >> group) & 1u)) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (group[i] >= 32u || !((open_groups >> group[i]) & 1u)) key[i] = 0u;
+                    for (int i = 0; i < kPer; ++i) key[i] = 0u;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const uint32_t group = (lane * kPer + i) / size;
+                    if (group >= 32u || !((open_groups >> group) & 1u)) key[i] = 0u;
+                }
+            }
         }
-        int32_t chosen = -1, previous = -1;  // lane j: the expert of slot j
-        float previous_key = 0.0f;
+        int32_t chosen = -1;  // lane j: the expert of slot j
+        uint32_t previous = 0;
+        float previous_key = INFINITY;
         const uint32_t rounds = direct ? p.top : p.top + 1;  // the one behind the last choice has to be further off than the error, too
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine = max(mine, key[i]);
         for (uint32_t j = 0; j < rounds && sure; ++j) {
-            uint32_t best = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-            best = __reduce_max_sync(0xffffffffu, best);
+            const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
             if (best == 0) break;
-            uint32_t who = 0xffffffffu;
+            const int winner = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+            uint32_t who = 0;
+            if (lane == winner) {
+                bool found = false;
+                mine = 0;
 #pragma unroll
-            for (int i = kPer - 1; i >= 0; --i)
-                if (key[i] == best) who = i * 32 + lane;
-            who = __reduce_min_sync(0xffffffffu, who);
+                for (int i = 0; i < kPer; ++i) {
+                    const bool hit = !found && key[i] == best;
+                    if (hit) { who = lane * kPer + i; key[i] = 0u; found = true; }
+                    mine = max(mine, key[i]);
+                }
+            }
+            who = __shfl_sync(0xffffffffu, who, winner);
             if (!direct) {
                 const float k = from_ordered(best);
-                if (j > 0 && !(previous_key - k > 2.0f * slack))
+                if (!(previous_key - k > 2.0f * slack))
                     sure = load_logit<kType>(row, who) == load_logit<kType>(row, previous) && load_bias(p.bias, who) == load_bias(p.bias, previous);
                 previous_key = k;
-                previous = (int32_t)who;
+                previous = who;
             }
             if (lane == (int)j && j < p.top) chosen = (int32_t)who;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (i * 32 + lane == who) key[i] = 0u;
         }
         if (!sure) {
-            top_logit = warp_max(top_logit);
+            if (p.sigmoid) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
+                top_logit = warp_max(top_logit);
+            }
             chosen = choose_exactly<kType>(p, row, top_logit, keys_all + (size_t)warp * p.experts, lane);
             __syncwarp();
         }
-        // Weights in 64 bits: one exponential per lane.
         const float l = chosen >= 0 ? load_logit<kType>(row, chosen) : -INFINITY;
+        const bool near_zero = p.sigmoid && __any_sync(0xffffffffu, chosen >= 0 && l < -80.0f);
         double w = 0.0;
         if (p.renormalise) {
             // Scores as they are while they can be represented, ratios from differences of logarithms where they vanish.
             const float most = warp_max(l);
-            if (p.sigmoid && most > -700.0f) w = chosen >= 0 ? sigmoid64(l) : 0.0;
-            else if (p.sigmoid) w = chosen >= 0 ? exp(log_sigmoid(l) - log_sigmoid(most)) : 0.0;
-            else w = chosen >= 0 ? exp((double)l - most) : 0.0;
+            if (chosen >= 0) w = !near_zero ? fast_score(p.sigmoid, l, most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
             const double sum = warp_sum(w);
-            if (chosen >= 0) w /= sum;
+            if (chosen >= 0) w *= sum > 1e-30 ? reciprocal(sum) : 1.0 / sum;
         } else if (p.sigmoid) {
-            if (chosen >= 0) w = sigmoid64(l);
+            if (chosen >= 0) w = near_zero ? sigmoid64(l) : fast_score(true, l, 0.0f);
         } else {
             double total = 0.0;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 if (logit[i] > -INFINITY) total += (double)exp_difference(logit[i], top_logit);
             total = warp_sum(total);
-            if (chosen >= 0) w = exp((double)l - top_logit) / total;
+            if (chosen >= 0) w = (double)exp_difference(l, top_logit) * reciprocal(total);
         }
         if ((uint32_t)lane < p.top) {
             weights[(uint64_t)token * p.top + lane] = (float)(w * p.scale);
@@ -309,20 +386,21 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
             for (uint32_t i = lane; i < padded / 4; i += 32) reinterpret_cast<float4 *>(line)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         double d = 0.0;  // what this slot's logit gets through the slot itself
+        const bool near_limit = p.sigmoid && __any_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f);
         if (p.renormalise) {
             const float most = warp_max(l);
             double part = 0.0;
-            if (id >= 0) part = !p.sigmoid ? exp((double)l - most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
-            const double sum = warp_sum(part), u = id >= 0 ? part / sum : 0.0, mean = warp_sum(g * u);
+            if (id >= 0) part = !near_limit ? fast_score(p.sigmoid, l, most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
+            const double sum = warp_sum(part), u = id >= 0 ? part * (sum > 1e-30 ? reciprocal(sum) : 1.0 / sum) : 0.0, mean = warp_sum(g * u);
             d = u * (g - mean);
         } else if (id >= 0) {
-            d = p.sigmoid ? g * sigmoid64(l) : g * (exp((double)l - top_logit) / total);
+            d = p.sigmoid ? g * (near_limit ? sigmoid64(l) : fast_score(true, l, 0.0f)) : g * ((double)exp_difference(l, top_logit) * reciprocal(total));
         }
-        if (p.sigmoid && id >= 0) d *= sigmoid64(-(double)l);  // 1 - s
+        if (p.sigmoid && id >= 0) d *= near_limit ? sigmoid64(-(double)l) : fast_score(true, -l, 0.0f);  // 1 - s
         __syncwarp();
         if (dense) {
             const double spread = warp_sum(d);
-            const float per_part = total > 0.0 ? (float)(-spread / total) : 0.0f;
+            const float per_part = total > 0.0 ? (float)(-spread * reciprocal(total)) : 0.0f;
             for (uint32_t e = lane; e < p.experts; e += 32) line[e] *= per_part;
             __syncwarp();
         }
