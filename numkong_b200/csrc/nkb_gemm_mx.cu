@@ -189,19 +189,25 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
 
     if (warp == 0) {
         if (lane == 0) {
-            // Only the row groups of eight that hold valid rows of A are fetched.
+            // Only the row groups of eight that hold valid rows of A are fetched. A tile's rows and group are looked up once.
+            struct Tile { uint32_t tile, a_bytes, group; };
+            auto tile_of = [&](const Walk &w, Tile &t) -> const Tile & {
+                if (t.tile != w.tile) t = {w.tile, (rows_of(w.mt) + 7u) / 8u * 1024u, p.tiles ? (uint32_t)p.tiles[w.mt].group : 0u};
+                return t;
+            };
+            Tile b_tile{0xffffffffu, 0, 0}, a_tile{0xffffffffu, 0, 0};
             auto load_b = [&](const Walk &w, int stage) {
-                const uint32_t group = p.tiles ? (uint32_t)p.tiles[w.mt].group : 0u;
+                const Tile &t = tile_of(w, b_tile);
                 const uint32_t block = w.nt * kBN / 128u, sub = w.nt * kBN % 128u;
-                const uint8_t *b = p.b_chunks + (((uint64_t)group * p.group_blocks + block) * p.kblocks + w.kb) * kMxChunkBytes;
+                const uint8_t *b = p.b_chunks + (((uint64_t)t.group * p.group_blocks + block) * p.kblocks + w.kb) * kMxChunkBytes;
                 const uint32_t dst = smem_base + P::kBRing + stage * P::kStageBytes;
-                mbar_expect_tx(full_bar(stage), (rows_of(w.mt) + 7u) / 8u * 1024u + P::kBBytes + 2 * kMxScaleBytes);
+                mbar_expect_tx(full_bar(stage), t.a_bytes + P::kBBytes + 2 * kMxScaleBytes);
                 bulk_load(dst, b + sub * 128u, P::kBBytes, full_bar(stage));
                 bulk_load(dst + P::kBBytes + kMxScaleBytes, b + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
             };
             auto load_a = [&](const Walk &w, int stage) {
                 const uint8_t *a = p.a_chunks + ((uint64_t)w.mt * p.kblocks + w.kb) * kMxChunkBytes;
-                bulk_load(smem_base + stage * P::kABytes, a, (rows_of(w.mt) + 7u) / 8u * 1024u, full_bar(stage));
+                bulk_load(smem_base + stage * P::kABytes, a, tile_of(w, a_tile).a_bytes, full_bar(stage));
                 bulk_load(smem_base + P::kBRing + stage * P::kStageBytes + P::kBBytes, a + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
             };
             int stage = 0;

@@ -54,7 +54,6 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-__device__ __forceinline__ float warp_min(float v) { return -warp_max(-v); }
 // The largest key of the warp and its index; the lower index where keys are equal.
 __device__ __forceinline__ void warp_best(double &key, uint32_t &index) {
 #pragma unroll
@@ -64,13 +63,6 @@ __device__ __forceinline__ void warp_best(double &key, uint32_t &index) {
         if (k > key || (k == key && i < index)) { key = k; index = i; }
     }
 }
-// Order-preserving integer of a key, 0 for "none" (-infinity): one integer reduction finds a warp's largest.
-__device__ __forceinline__ uint32_t ordered(float f) {
-    const uint32_t u = __float_as_uint(f);
-    return f > -INFINITY ? ((u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;
-}
-__device__ __forceinline__ float from_ordered(uint32_t k) { return k ? selection_value(k) : -INFINITY; }
-
 __device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
 __device__ __forceinline__ double log_sigmoid(double l) { return fmin(l, 0.0) - log1p(exp(-fabs(l))); }
 
@@ -127,8 +119,9 @@ __device__ __forceinline__ void load_logits(const uint8_t *row, uint32_t experts
 // The choice in 64 bits, for the tokens whose keys 32 bits leave undecided. `keys`: room for one key per expert. Returns lane j's choice.
 template <uint32_t kType>
 __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, float top_logit, double *keys, int lane) {
+    const bool direct = p.bias == nullptr && p.groups == 1;  // scores grow with their logits
     double total = 0.0;
-    if (!p.sigmoid) {
+    if (!p.sigmoid && !direct) {
         for (uint32_t e = lane; e < p.experts; e += 32) {
             const float l = load_logit<kType>(row, e);
             if (l > -INFINITY) total += exp((double)l - top_logit);
@@ -137,7 +130,8 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     }
     for (uint32_t e = lane; e < p.experts; e += 32) {
         const float l = load_logit<kType>(row, e), b = load_bias(p.bias, e);
-        keys[e] = l > -INFINITY && b > -INFINITY ? (p.sigmoid ? sigmoid64(l) : exp((double)l - top_logit) / total) + b : -INFINITY;
+        if (direct) keys[e] = l;
+        else keys[e] = l > -INFINITY && b > -INFINITY ? (p.sigmoid ? sigmoid64(l) : exp((double)l - top_logit) / total) + b : -INFINITY;
     }
     __syncwarp();
     if (p.groups > 1) {
@@ -179,60 +173,94 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     return chosen;
 }
 
-// One warp per token; lane i holds the experts i * kPer .. in registers. A round of the selection is one integer maximum over the
-// warp and a ballot for the lowest lane that reaches it; that lane alone takes its expert out and looks for its next best.
+// One warp per token; lane i holds the experts i * kPer .. in registers.
 //
-// Keys are computed in 32 bits with a bound on their error. Where every decision (chosen against next, open group against closed) is
-// wider than that bound, or is a tie of equal inputs, the choice is the one 64 bits would make; the other tokens, a few in a
-// thousand on random logits, go through choose_exactly. Keys that are the logits themselves (no bias, no groups) are exact.
-// Bound by instructions. 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token in 64 bits.
+// A key and its expert share one 32-bit word: the key in fixed point above, 31 - e of the warp's width below, so that one integer
+// maximum over the warp finds the next choice and gives ties to the lower index. The fixed point comes from scores in 32 bits;
+// `slack` bounds, in its units, how far it is off. Where every decision (chosen against next, open group against closed) is wider
+// than that, or is a tie of equal inputs, the choice is the one 64 bits would make; the other tokens, a few in a thousand on
+// random logits, go through choose_exactly. Keys that are the logits themselves (no bias, no groups) are the upper bits of their
+// order-preserving integers, exact for 16-bit logits.
+//
+// Bound by instructions, about 600 a token. 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token
+// in 64 bits, 38 us with 32-bit keys whose expert was looked up in every round.
 template <uint32_t kType, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, float *weights, int32_t *ids) {
+    constexpr uint32_t kIndexBits = kPer == 1 ? 5 : kPer == 2 ? 6 : kPer == 4 ? 7 : kPer == 8 ? 8 : kPer == 16 ? 9 : 10;
+    constexpr uint32_t kWidth = 32 * kPer, kUnits = (1u << (32 - kIndexBits)) - 64;  // some room above for rounding
     extern __shared__ double keys_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool direct = p.bias == nullptr && p.groups == 1;
     const uint32_t size = p.experts / p.groups, lanes = size / kPer;
     const bool whole_lanes = size % kPer == 0 && (lanes & (lanes - 1)) == 0;  // a group is a power of two of lanes
-    float bias[kPer], most_bias = 0.0f;
+    // Scores lie in [0, 1], keys in [least bias, 1 + most bias]. zero_key: the units of a key of 0.
+    float bias[kPer], least = INFINITY, most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const uint32_t e = lane * kPer + i;
         bias[i] = e < p.experts ? load_bias(p.bias, e) : -INFINITY;
-        if (bias[i] > -INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
+        if (bias[i] > -INFINITY) { least = fminf(least, bias[i]); most = fmaxf(most, bias[i]); }
     }
-    most_bias = warp_max(most_bias);
-    // Relative error of a score: exp and division a few units, the softmax's sum one more per addition. Scores are at most 1, and the
-    // sum with the bias rounds once more.
-    const float slack = ((p.sigmoid ? 8.0f : (float)(kPer + 16)) + most_bias) * 0x1p-23f;
-    for (uint32_t token = blockIdx.x * kWarps + warp; token < p.tokens; token += gridDim.x * kWarps) {
+    least = -warp_max(-least);
+    most = warp_max(most);
+    if (!(least <= most)) least = most = 0.0f;  // every expert is barred
+    least = fminf(least, 0.0f);                 // so that a key of 0 is on the scale
+    const bool workable = direct || (fabsf(least) < 16.0f && fabsf(most) < 16.0f);  // wider biases leave the scale too coarse
+    const float per_key = (float)kUnits / (1.0f + (most - least)), zero_key = -least * per_key;
+    // A score is off by a few units of its last place (exp, division), the softmax's sum one more per addition; the sum with the bias and
+    // the step to fixed point round four times more.
+    const uint32_t slack = (uint32_t)(((p.sigmoid ? 8.0f : (float)(kPer + 16)) + fabsf(least) + fabsf(most)) * 0x1p-23f * per_key) + 8u;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) bias[i] = (bias[i] - least) * per_key;  // -infinity stays
+    float logit[kPer];
+    uint32_t token = blockIdx.x * kWarps + warp;
+    if (token < p.tokens) load_logits<kType, kPer>(p.logits + token * p.stride, p.experts, lane, logit);
+    for (; token < p.tokens;) {
         const uint8_t *row = p.logits + token * p.stride;
-        float logit[kPer], top_logit = -INFINITY;
-        load_logits<kType, kPer>(row, p.experts, lane, logit);
+        const uint32_t following = token + gridDim.x * kWarps;
+        float next[kPer];
+        if (following < p.tokens) load_logits<kType, kPer>(p.logits + following * p.stride, p.experts, lane, next);
+        float top_logit = -INFINITY;
         if (!p.sigmoid) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
             top_logit = warp_max(top_logit);
         }
         uint32_t key[kPer];
+        const uint32_t last = kWidth - 1 - lane * kPer;
         if (direct) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) key[i] = ordered(logit[i]);
-        } else if (p.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY && bias[i] > -INFINITY ? ordered(__fdividef(1.0f, 1.0f + __expf(-logit[i])) + bias[i]) : 0u;
+            for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY ? (selection_key(logit[i]) & ~(kWidth - 1)) | (last - i) : 0u;
         } else {
-            float part[kPer], total = 0.0f;
+            float scaled = per_key;
+            float part[kPer];
+            if (p.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) { part[i] = logit[i] > -INFINITY ? expf(logit[i] - top_logit) : 0.0f; total += part[i]; }
+                for (int i = 0; i < kPer; ++i) part[i] = __fdividef(1.0f, 1.0f + __expf(-logit[i]));
+            } else {
+                float total = 0.0f;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            const float inverse = 1.0f / total;
+                for (int i = 0; i < kPer; ++i) { part[i] = expf(logit[i] - top_logit); if (logit[i] > -INFINITY) total += part[i]; }
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY && bias[i] > -INFINITY ? ordered(part[i] * inverse + bias[i]) : 0u;
+                for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                scaled = __fdividef(per_key, total);
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const float units = fmaf(part[i], scaled, bias[i]);
+                // One unit up: 0 stands for no key.
+                key[i] = logit[i] > -INFINITY && units > -INFINITY ? ((__float2uint_rz(units) + 1u) << kIndexBits) | (last - i) : 0u;
+            }
         }
-        bool sure = true;
+        bool sure = workable;
         if (p.groups > 1) {
-            float worth = -INFINITY;  // lane g: group g's
+            uint32_t worth = 0;  // lane g: group g's, in units; 0 where nobody is left
+            const uint32_t alone = (uint32_t)zero_key;  // keeps sums of one and of two keys comparable
+            auto worth_of = [&](uint32_t first, uint32_t second) {
+                if (first == 0) return 0u;
+                const uint32_t a = first >> kIndexBits, b = second ? second >> kIndexBits : alone;
+                return (a >> 1) + (b >> 1) + 1u;  // half units: the sum fits 32 bits
+            };
             if (whole_lanes) {
                 uint32_t first = 0, second = 0;
 #pragma unroll
@@ -245,9 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                     second = max(min(first, f), max(second, n));
                     first = max(first, f);
                 }
-                const float mine = second ? from_ordered(first) + from_ordered(second) : from_ordered(first);
-                worth = __shfl_sync(0xffffffffu, mine, lane * lanes);
-                if ((uint32_t)lane >= p.groups) worth = -INFINITY;
+                worth = __shfl_sync(0xffffffffu, worth_of(first, second), lane * lanes);
             } else {
                 for (uint32_t g = 0; g < p.groups; ++g) {
                     uint32_t first = 0, second = 0;
@@ -257,26 +283,25 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                         second = max(second, min(first, k));
                         first = max(first, k);
                     }
-                    const uint32_t best = __reduce_max_sync(0xffffffffu, first);
-                    const int holder = __ffs(__ballot_sync(0xffffffffu, first == best)) - 1;
-                    const uint32_t next = __reduce_max_sync(0xffffffffu, lane == holder ? second : first);
-                    if (lane == (int)g) worth = next ? from_ordered(best) + from_ordered(next) : from_ordered(best);
+                    const uint32_t best = __reduce_max_sync(0xffffffffu, first);  // keys differ from one another in their experts
+                    const uint32_t behind = __reduce_max_sync(0xffffffffu, first == best ? second : first);
+                    if (lane == (int)g) worth = worth_of(best, behind);
                 }
             }
+            if ((uint32_t)lane >= p.groups) worth = 0;
             uint32_t rank = 0;
             for (uint32_t g = 0; g < p.groups; ++g) {
-                const float other = __shfl_sync(0xffffffffu, worth, g);
+                const uint32_t other = __shfl_sync(0xffffffffu, worth, g);
                 rank += other > worth || (other == worth && (int)g < lane);
             }
             const bool open = (uint32_t)lane < p.groups && rank < p.top_groups;
-            const float least_open = warp_min(open ? worth : INFINITY);
-            const float most_closed = warp_max((uint32_t)lane < p.groups && !open ? worth : -INFINITY);
-            // A worth is off by twice a key's error and a rounding.
-            if (most_closed > -INFINITY && !(least_open - most_closed > 6.0f * slack)) sure = false;
+            const uint32_t least_open = __reduce_min_sync(0xffffffffu, open ? worth : 0xffffffffu);
+            const uint32_t most_closed = __reduce_max_sync(0xffffffffu, open ? 0u : worth);
+            // A worth is off by two keys' errors, halved, and its roundings.
+            if (most_closed != 0 && least_open - most_closed <= 2 * slack + 4) sure = false;
             const uint32_t open_groups = __ballot_sync(0xffffffffu, open);
             if (whole_lanes) {
-                const uint32_t group = lane / lanes;
-                if (!((open_groups >> group) & 1u)) {
+                if (!((open_groups >> (lane / lanes)) & 1u)) {
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) key[i] = 0u;
                 }
@@ -289,35 +314,22 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             }
         }
         int32_t chosen = -1;  // lane j: the expert of slot j
-        uint32_t previous = 0;
-        float previous_key = INFINITY;
-        const uint32_t rounds = direct ? p.top : p.top + 1;  // the one behind the last choice has to be further off than the error, too
-        uint32_t mine = 0;
+        uint32_t before = 0xffffffffu;  // the word before; the one behind the last choice has to be further off than the error, too
+        for (uint32_t j = 0; j <= p.top && sure; ++j) {
+            uint32_t mine = key[0];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) mine = max(mine, key[i]);
-        for (uint32_t j = 0; j < rounds && sure; ++j) {
+            for (int i = 1; i < kPer; ++i) mine = max(mine, key[i]);
             const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
             if (best == 0) break;
-            const int winner = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
-            uint32_t who = 0;
-            if (lane == winner) {
-                bool found = false;
-                mine = 0;
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const bool hit = !found && key[i] == best;
-                    if (hit) { who = lane * kPer + i; key[i] = 0u; found = true; }
-                    mine = max(mine, key[i]);
-                }
+            for (int i = 0; i < kPer; ++i)
+                if (key[i] == best) key[i] = 0u;
+            const uint32_t who = kWidth - 1 - (best & (kWidth - 1));
+            if (j > 0 && (before >> kIndexBits) - (best >> kIndexBits) <= (direct ? 0u : 2 * slack)) {
+                const uint32_t previous = kWidth - 1 - (before & (kWidth - 1));
+                sure = load_logit<kType>(row, who) == load_logit<kType>(row, previous) && load_bias(p.bias, who) == load_bias(p.bias, previous);
             }
-            who = __shfl_sync(0xffffffffu, who, winner);
-            if (!direct) {
-                const float k = from_ordered(best);
-                if (!(previous_key - k > 2.0f * slack))
-                    sure = load_logit<kType>(row, who) == load_logit<kType>(row, previous) && load_bias(p.bias, who) == load_bias(p.bias, previous);
-                previous_key = k;
-                previous = who;
-            }
+            before = best;
             if (lane == (int)j && j < p.top) chosen = (int32_t)who;
         }
         if (!sure) {
@@ -334,8 +346,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
         double w = 0.0;
         if (p.renormalise) {
             // Scores as they are while they can be represented, ratios from differences of logarithms where they vanish.
-            const float most = warp_max(l);
-            if (chosen >= 0) w = !near_zero ? fast_score(p.sigmoid, l, most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
+            const float largest = p.sigmoid && !near_zero ? 0.0f : warp_max(l);
+            if (chosen >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
             const double sum = warp_sum(w);
             if (chosen >= 0) w *= sum > 1e-30 ? reciprocal(sum) : 1.0 / sum;
         } else if (p.sigmoid) {
@@ -352,6 +364,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             weights[(uint64_t)token * p.top + lane] = (float)(w * p.scale);
             ids[(uint64_t)token * p.top + lane] = chosen;
         }
+        token = following;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) logit[i] = next[i];
     }
 }
 
@@ -364,13 +379,28 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
     const uint32_t padded = (p.experts + 3) / 4 * 4;
     float *line = rows_all + (size_t)warp * padded;
     const bool dense = !p.sigmoid && !p.renormalise;
-    for (uint32_t token = blockIdx.x * kWarps + warp; token < p.tokens; token += gridDim.x * kWarps) {
+    const uint32_t step = gridDim.x * kWarps;
+    // The slots of the token after this one are on their way while this one is worked on, and so are the logits they name.
+    struct Slot { int32_t id; float grad, logit; };
+    auto load_slot = [&](uint32_t token, Slot &s) {
+        s = {-1, 0.0f, -INFINITY};
+        if (token < p.tokens && (uint32_t)lane < p.top) {
+            s.id = ids[(uint64_t)token * p.top + lane];
+            s.grad = weights_grad[(uint64_t)token * p.top + lane];
+        }
+    };
+    auto load_named = [&](uint32_t token, Slot &s) {
+        if (s.id >= 0 && s.id < (int32_t)p.experts) s.logit = load_logit<kType>(p.logits + token * p.stride, s.id);
+    };
+    Slot slot, ahead;
+    load_slot(blockIdx.x * kWarps + warp, slot);
+    load_named(blockIdx.x * kWarps + warp, slot);
+    for (uint32_t token = blockIdx.x * kWarps + warp; token < p.tokens; token += step) {
         const uint8_t *row = p.logits + token * p.stride;
-        int32_t id = (uint32_t)lane < p.top ? ids[(uint64_t)token * p.top + lane] : -1;
-        if (id >= (int32_t)p.experts) id = -1;
-        const float l = id >= 0 ? load_logit<kType>(row, id) : -INFINITY;
-        if (l == -INFINITY) id = -1;  // a masked expert has score 0 whatever its logit: no gradient
-        const double g = id >= 0 ? (double)weights_grad[(uint64_t)token * p.top + lane] * p.scale : 0.0;
+        load_slot(token + step, ahead);
+        const float l = slot.logit;
+        const int32_t id = l > -INFINITY ? slot.id : -1;  // a masked expert has score 0 whatever its logit: no gradient
+        const double g = id >= 0 ? (double)slot.grad * p.scale : 0.0;
         float top_logit = -INFINITY;
         double total = 0.0;
         if (dense) {
@@ -415,6 +445,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
             d = sum;
         }
         if (id >= 0 && __ffs(same) - 1 == lane) line[id] += (float)d;
+        load_named(token + step, ahead);
+        slot = ahead;
         __syncwarp();
         float *out = logits_grad + (uint64_t)token * p.experts;
         if ((p.experts & 3u) == 0 && (reinterpret_cast<uintptr_t>(logits_grad) & 15u) == 0)

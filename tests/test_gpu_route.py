@@ -98,6 +98,40 @@ def test_masked_logits(case):
     assert (ids[1] >= 0).sum() == 2
 
 
+@pytest.mark.parametrize("offset,spread", [(5.0, 0.1), (-5.0, 0.1), (0.0, 30.0), (1e8, 0.0), (0.0, 1e30), (-1e-30, 0.0)])
+def test_biases_of_any_size(offset, spread):
+    """Biases beyond the scores' range, far from zero, all of one sign, infinite."""
+    x = np.random.default_rng(11).standard_normal((40, 96)).astype(np.float32)
+    bias = (offset + spread * np.random.default_rng(12).standard_normal(96)).astype(np.float32)
+    for case in (dict(top=6, score="sigmoid"), dict(top=6), dict(top=5, groups=8, top_groups=3, score="sigmoid"), dict(top=5, groups=6, top_groups=2)):
+        run(torch.from_numpy(x), x, dict(case, bias=True), bias)
+        barred = bias.copy()
+        barred[::5], barred[1] = -np.inf, np.inf
+        run(torch.from_numpy(x), x, dict(case, bias=True), barred)
+
+
+def test_groups_with_one_expert_left():
+    x = np.random.default_rng(13).standard_normal((64, 64)).astype(np.float32)
+    x[:, 1:8] = -np.inf                 # one left in the first group
+    x[::2, 8:16] = -np.inf              # none in the second
+    x[::3, 17:24] = np.nan
+    bias = (0.3 * np.random.default_rng(14).standard_normal(64)).astype(np.float32)
+    for shift in (-0.5, 0.0, 2.0):
+        for score in ("softmax", "sigmoid"):
+            run(torch.from_numpy(x), x, dict(top=9, groups=8, top_groups=5, score=score, bias=True), bias + np.float32(shift))
+    run(torch.from_numpy(x), x, dict(top=9, groups=8, top_groups=5), None)
+
+
+def test_f32_logits_that_differ_in_their_last_bits():
+    """Without a bias the choice is the logits' own order, to the last bit, at every size and sign."""
+    rng = np.random.default_rng(15)
+    base = np.repeat(rng.standard_normal((60, 8)).astype(np.float32) * 50, 16, axis=1)
+    x = base.view(np.int32) + rng.permuted(np.tile(np.arange(128, dtype=np.int32) % 16, (60, 1)), axis=1)
+    x = x.view(np.float32)
+    for score in ("softmax", "sigmoid"):
+        run(torch.from_numpy(x), x, dict(top=20, score=score), None)
+
+
 def test_scores_too_small_to_represent_renormalise():
     x = np.full((3, 16), -200, np.float32)
     x[1, 4], x[2] = -190, -1e4
