@@ -12,7 +12,9 @@
 // One persistent CTA per SM, fourteen warps: warp 0 brings chunks to shared memory with untiled bulk copies, warp 1 issues the
 // MMAs, warps 2..9 read the accumulators out and store the cells, warps 10..13 store scales.
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "nkb_mx.h"
+#include "nkb_mx_encode.cuh"
 #include "nkb_ptx.cuh"
 
 namespace nkb {
@@ -38,6 +40,9 @@ struct MxGemmDev {
     uint32_t a_row_major;            // A's codes are read from the caller's rows, only its scales are in tile form
     const uint8_t *a_scales;         // scale tiles of A's first chunk, and the bytes from one chunk's to the next
     uint64_t a_scale_step;
+    const uint8_t *x;                // float rows of A the kernel quantises itself (m <= 16), their stride, type and length
+    uint64_t x_stride;
+    uint32_t x_type, k;
     unsigned int *error_word;
     uint32_t wait_us[kWaitSites];
 };
@@ -77,6 +82,7 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const M
     constexpr int kQuads = kPieceCols * kCell / 16;  // 16-byte parts of a staged row
     static_assert(kCols % kPieceCols == 0 && kQuads >= 2, "whole pieces");
     if (!__any_sync(0xffffffffu, dest >= 0)) return;
+    uint8_t *const my_row = dest >= 0 ? p.c + (uint64_t)dest * p.c_stride : nullptr;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.c) | p.c_stride) & 15u) == 0;
 #pragma unroll
     for (int c = 0; c < kCols / kPieceCols; ++c) {
@@ -106,25 +112,34 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const M
 #pragma unroll
             for (int it = 0; it < kQuads; ++it) {
                 const int r = it * (32 / kQuads) + lane / kQuads, q = lane % kQuads;
-                const int64_t row = __shfl_sync(0xffffffffu, dest, r);
-                if (row >= 0)
-                    __stcs(reinterpret_cast<uint4 *>(p.c + (uint64_t)row * p.c_stride + (uint64_t)col0 * kCell) + q, *reinterpret_cast<const uint4 *>(staging + r * pitch + q * 16));
+                uint8_t *row = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), r));
+                if (row) __stcs(reinterpret_cast<uint4 *>(row + (uint64_t)col0 * kCell) + q, *reinterpret_cast<const uint4 *>(staging + r * pitch + q * 16));
             }
         } else {
+            // Whole pieces without a branch, so that several rows are on their way at once: every lane writes a word, of a bf16 row that begins
+            // in the middle of one the 31 words inside and two single cells at its ends.
+            const bool whole = cells == kPieceCols;
+            constexpr int kWords = kPieceCols * kCell / 4;
 #pragma unroll 4
             for (int r = 0; r < 32; ++r) {
-                const int64_t row = __shfl_sync(0xffffffffu, dest, r);
-                if (row < 0) continue;
-                uint8_t *dst = p.c + (uint64_t)row * p.c_stride + (uint64_t)col0 * kCell;
+                uint8_t *dst = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), r));
+                const bool there = dst != nullptr;
+                dst += (uint64_t)col0 * kCell;
+                const uint32_t *from = reinterpret_cast<const uint32_t *>(staging + r * pitch);
                 if constexpr (kBf16) {
-                    const uint16_t *from = reinterpret_cast<const uint16_t *>(staging + r * pitch);
-                    const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(dst) >> 1) & 1u;  // one cell before the first whole word
-                    const uint32_t at = odd + 2 * lane;
-                    if (at + 1 < cells) *reinterpret_cast<uint32_t *>(dst + 2 * at) = (uint32_t)from[at] | ((uint32_t)from[at + 1] << 16);
-                    else if (at < cells) *reinterpret_cast<uint16_t *>(dst + 2 * at) = from[at];
-                    if (odd && lane == 0) *reinterpret_cast<uint16_t *>(dst) = from[0];
-                } else if ((uint32_t)lane < cells) {
-                    *reinterpret_cast<uint32_t *>(dst + 4 * lane) = *reinterpret_cast<const uint32_t *>(staging + r * pitch + 4 * lane);
+                    const bool odd = reinterpret_cast<uintptr_t>(dst) & 2u;  // one cell before the first whole word
+                    const uint32_t w0 = from[min(lane, kWords - 1)], w1 = from[min(lane + 1, kWords - 1)];
+                    const uint32_t word = odd ? __funnelshift_r(w0, w1, 16) : w0;
+                    if (whole) {
+                        if (there && lane < kWords - (odd ? 1 : 0)) *reinterpret_cast<uint32_t *>(dst + (odd ? 2 : 0) + 4 * lane) = word;
+                        if (there && odd && (lane == 0 || lane == kWords - 1))
+                            *reinterpret_cast<uint16_t *>(dst + (lane == 0 ? 0 : 4 * kWords - 2)) = (uint16_t)(lane == 0 ? w0 : w0 >> 16);
+                    } else if (there) {
+                        for (uint32_t c2 = 2 * lane; c2 < min(cells, 2 * lane + 2); ++c2)
+                            *reinterpret_cast<uint16_t *>(dst + 2 * c2) = (uint16_t)(c2 & 1 ? w0 >> 16 : w0);
+                    }
+                } else if (there && (uint32_t)lane < cells) {
+                    *reinterpret_cast<uint32_t *>(dst + 4 * lane) = from[min(lane, kWords - 1)];
                 }
             }
         }
@@ -147,8 +162,41 @@ struct Walk {
     }
 };
 
-template <int kBN, int kARows, bool kBf16>
+// Eight values of row `row` from `first` on, zeros past the end.
+template <uint32_t kType>
+__device__ __forceinline__ void load_row8(const MxGemmDev &p, uint32_t row, uint32_t first, uint4 (&raw)[2]) {
+    constexpr int kBytes = kType == kF32 ? 4 : 2;
+    const uint8_t *from = p.x + row * p.x_stride + (uint64_t)first * kBytes;
+    raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
+    if (first + 8 <= p.k && (reinterpret_cast<uintptr_t>(from) & 15u) == 0) {
+        raw[0] = __ldg(reinterpret_cast<const uint4 *>(from));
+        if constexpr (kType == kF32) raw[1] = __ldg(reinterpret_cast<const uint4 *>(from) + 1);
+    } else {
+        uint32_t w[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first + i < p.k) {
+                if constexpr (kType == kF32) w[i] = __ldg(reinterpret_cast<const uint32_t *>(from) + i);
+                else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(from) + i) << (16 * (i & 1));
+            }
+        raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+template <uint32_t kType>
+__device__ __forceinline__ uint32_t quantise_row8(const uint4 (&raw)[2], uint32_t &scale) {
+    float v[8];
+    uint32_t largest;
+    if constexpr (kType == kF32) largest = unpack8<kType>(raw, v);
+    else largest = unpack8<kType>({raw[0]}, v);
+    return quantise8(v, largest, scale);
+}
+
+// With kOwnA the epilogue warps quantise A's few rows chunk by chunk into the ring while the packed matrix streams in: one launch and
+// no workspace, at the price of every CTA doing it again.
+template <int kBN, int kARows, bool kOwnA, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p) {
+    static_assert(!kOwnA || kARows == 2 * kEpilogueWarps, "two rows a warp");
     using P = Plan<kBN, kARows>;
     constexpr int kStages = P::kStages;
     constexpr int kColsPerThread = kBN / 2;
@@ -170,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), kScaleWarps); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), kOwnA ? 1 + kEpilogueWarps : 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), kScaleWarps); }
         for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(tmem_empty_bar(a), kEpilogueWarps * 32); }
         mbar_init(drain_bar, 1);
         fence_mbar_init();
@@ -201,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
                 const uint32_t block = w.nt * kBN / 128u, sub = w.nt * kBN % 128u;
                 const uint8_t *b = p.b_chunks + (((uint64_t)t.group * p.group_blocks + block) * p.kblocks + w.kb) * kMxChunkBytes;
                 const uint32_t dst = smem_base + P::kBRing + stage * P::kStageBytes;
-                mbar_expect_tx(full_bar(stage), t.a_bytes + P::kBBytes + 2 * kMxScaleBytes);
+                mbar_expect_tx(full_bar(stage), (kOwnA ? 0u : t.a_bytes + kMxScaleBytes) + P::kBBytes + kMxScaleBytes);
                 bulk_load(dst, b + sub * 128u, P::kBBytes, full_bar(stage));
                 bulk_load(dst + P::kBBytes + kMxScaleBytes, b + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
             };
@@ -217,13 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             // The packed matrix does not depend on the kernel before, which is still quantising A.
             Walk early = w;
             for (int s = 0; s < kStages && early.valid(); ++s, early.next()) load_b(early, s);
-            wait_for_previous_kernel();
+            if constexpr (!kOwnA) wait_for_previous_kernel();
             for (; w.valid(); w.next()) {
                 if (issued >= (uint32_t)kStages) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
                     load_b(w, stage);
                 }
-                load_a(w, stage);
+                if constexpr (!kOwnA) load_a(w, stage);
                 ++issued;
                 if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
@@ -293,10 +341,48 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     } else {
         const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
         uint8_t *staging = smem_gen + P::kStagingOffset + (warp - 2) * 32 * P::kStagingPitch;
-        uint32_t seq = 0;
+        uint32_t seq = 0, phase = 0;
+        int stage = 0;
         for (uint32_t tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++seq) {
             uint32_t mt, nt;
             tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+            if constexpr (kOwnA) {
+                bool ok = true;
+                auto own = [&](auto type) {
+                    constexpr uint32_t kType = decltype(type)::value;
+                    const uint32_t rows[2] = {(uint32_t)warp - 2u, (uint32_t)warp - 2u + kEpilogueWarps};
+                    uint4 raw[2][2], next[2][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (rows[h] < p.m) load_row8<kType>(p, rows[h], lane * 8, raw[h]);
+                    for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (rows[h] < p.m && kb + 1 < p.kblocks) load_row8<kType>(p, rows[h], (kb + 1) * kMxChunkValues + lane * 8, next[h]);
+                        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1]))) { ok = false; break; }
+                        uint8_t *codes = smem_gen + stage * P::kABytes, *scales = smem_gen + P::kBRing + stage * P::kStageBytes + P::kBBytes;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t r = rows[h];
+                            if (r >= p.m) continue;
+                            uint32_t s;
+                            const uint32_t word = quantise_row8<kType>(raw[h], s);
+                            *reinterpret_cast<uint32_t *>(codes + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = word;
+                            if ((lane & 3) == 0) scales[(lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)s;
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) raw[h][q] = next[h][q];
+                        }
+                        fence_proxy_async_smem();  // the MMA reads the codes through the other proxy
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full_bar(stage));
+                        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    }
+                };
+                if (p.x_type == kBF16) own(std::integral_constant<uint32_t, kBF16>{});
+                else if (p.x_type == kF16) own(std::integral_constant<uint32_t, kF16>{});
+                else own(std::integral_constant<uint32_t, kF32>{});
+                if (!ok) break;
+            }
             const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
             const uint32_t in_tile = quarter * 32u + lane, rows = rows_of(mt);
             int64_t dest = -1;
@@ -613,10 +699,10 @@ cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t
     return launch_dependent(kernel, 2 * pairs, kThreads, kPairSmem, stream, maps, dev);
 }
 
-template <int kBN, int kARows, bool kBf16>
+template <int kBN, int kARows, bool kOwnA, bool kBf16>
 cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
     using P = Plan<kBN, kARows>;
-    auto kernel = gemm_mx_kernel<kBN, kARows, kBf16>;
+    auto kernel = gemm_mx_kernel<kBN, kARows, kOwnA, kBf16>;
     static bool configured[64] = {false};
     int d = 0;
     cudaGetDevice(&d);
@@ -626,13 +712,18 @@ cudaError_t launch(const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream
         configured[d] = true;
     }
     const uint32_t grid = (uint32_t)(max_tiles < (uint64_t)usable_sms() ? max_tiles : (uint64_t)usable_sms());
-    return launch_dependent(kernel, grid, kThreads, P::kTotal, stream, dev);
+    if constexpr (kOwnA) {
+        kernel<<<grid, kThreads, P::kTotal, stream>>>(dev);
+        return cudaGetLastError();
+    } else {
+        return launch_dependent(kernel, grid, kThreads, P::kTotal, stream, dev);
+    }
 }
 
-template <int kARows, bool kBf16>
-cudaError_t launch_by_width(int bn, const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
-    if (bn == 64) return launch<64, kARows, kBf16>(dev, max_tiles, stream);
-    return launch<128, kARows, kBf16>(dev, max_tiles, stream);
+template <int kARows, bool kOwnA>
+cudaError_t launch_by_width(int bn, bool bf16, const MxGemmDev &dev, uint64_t max_tiles, cudaStream_t stream) {
+    if (bn == 64) return bf16 ? launch<64, kARows, kOwnA, true>(dev, max_tiles, stream) : launch<64, kARows, kOwnA, false>(dev, max_tiles, stream);
+    return bf16 ? launch<128, kARows, kOwnA, true>(dev, max_tiles, stream) : launch<128, kARows, kOwnA, false>(dev, max_tiles, stream);
 }
 
 } // namespace
@@ -641,7 +732,9 @@ bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t k) {
     return ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 2;
 }
 
-static bool use_pairs(const MxGemmArgs &args) { return args.tiles == nullptr && gemm_mx_reads_rows(args.m, args.n, args.k); }
+bool gemm_mx_quantises(uint64_t m) { return m <= 16; }
+
+static bool use_pairs(const MxGemmArgs &args) { return args.tiles == nullptr && args.x == nullptr && gemm_mx_reads_rows(args.m, args.n, args.k); }
 
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     if (args.m == 0 || args.n == 0) return cudaSuccess;
@@ -662,8 +755,13 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.tiles = args.tiles;
     dev.tile_count = args.tile_count;
     dev.row_dest = args.row_dest;
+    dev.x = static_cast<const uint8_t *>(args.x);
+    dev.x_stride = args.x_stride;
+    dev.x_type = args.x_type;
+    dev.k = (uint32_t)args.k;
     dev.error_word = args.error_word;
     wait_limits_us(dev.wait_us);
+    if (args.x && !gemm_mx_quantises(args.m)) return cudaErrorInvalidValue;
     dev.a_row_major = args.a_codes != nullptr;
     dev.a_scales = dev.a_chunks + (args.a_codes ? 0u : kMxCodeBytes);
     dev.a_scale_step = args.a_codes ? kMxScaleBytes : kMxChunkBytes;
@@ -696,8 +794,9 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.tiles_n = (uint32_t)((args.n + bn - 1) / bn);
     const uint64_t tiles = row_tiles * dev.tiles_n;
     if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-    if (!args.tiles && args.m <= 16) return args.c_bf16 ? launch_by_width<16, true>(bn, dev, tiles, stream) : launch_by_width<16, false>(bn, dev, tiles, stream);
-    return args.c_bf16 ? launch_by_width<128, true>(bn, dev, tiles, stream) : launch_by_width<128, false>(bn, dev, tiles, stream);
+    if (args.x) return launch_by_width<16, true>(bn, args.c_bf16, dev, tiles, stream);
+    if (!args.tiles && args.m <= 16) return launch_by_width<16, false>(bn, args.c_bf16, dev, tiles, stream);
+    return launch_by_width<128, false>(bn, args.c_bf16, dev, tiles, stream);
 }
 
 } // namespace nkb

@@ -63,6 +63,9 @@ struct MxGemmArgs {
     const void *a_codes = nullptr;     // A's row-major codes (16-byte aligned, stride too), see gemm_mx_reads_rows
     uint64_t a_codes_stride = 0;
     const void *b_chunks;
+    const void *x = nullptr;           // or float rows of A, quantised inside: see gemm_mx_quantises
+    uint64_t x_stride = 0;
+    uint32_t x_type = 0;
     void *c;
     uint64_t c_stride;
     bool c_bf16;                       // cells: bf16 (rounded to nearest even) or f32
@@ -75,6 +78,8 @@ struct MxGemmArgs {
 };
 // Whether a product of this size reads A's codes from the caller's rows when they are aligned.
 bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t k);
+// Whether a product with this many rows takes float rows as they are.
+bool gemm_mx_quantises(uint64_t m);
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream);
 
 // ---- routing and the experts' products ----

@@ -164,9 +164,11 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     bool ok = c_dev != nullptr;
     if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_stride, 0, row_bytes, m, stream), "clear result");
     else if (ok) {
-        uint8_t *chunks = workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
-        ok = chunks != nullptr;
+        const bool inside = !codes && gemm_mx_quantises(m);
+        uint8_t *chunks = inside ? nullptr : workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
+        ok = inside || chunks;
         bool rows_in_place = false;
+        const uint8_t *ad = nullptr;
         const uint8_t *cd = nullptr;
         if (ok && codes) {
             cd = ops.in(codes, m, (k + 1) / 2, codes_stride);
@@ -176,17 +178,19 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
             if (rows_in_place) ok = cuda_ok(launch_mx_tile_scales(sd, scales_stride, m, k, chunks, stream), "scale tile kernel");
             else ok = sd && cuda_ok(launch_mx_tile(cd, codes_stride, sd, scales_stride, 1, m, k, false, chunks, stream), "tile kernel");
         } else if (ok) {
-            const uint8_t *ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
-            ok = ad && cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
+            ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
+            ok = ad != nullptr;
+            if (ok && !inside) ok = cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
         }
         if (ok) {
             MxGemmArgs args;
             args.a_chunks = chunks; args.b_chunks = blob + g.payload_offset;
+            if (inside) { args.x = ad; args.x_stride = m > 1 ? a_stride : 0; args.x_type = a_type; }
             if (rows_in_place) { args.a_codes = cd; args.a_codes_stride = codes_stride; }
             args.c = c_dev; args.c_stride = c_stride; args.c_bf16 = c_type == kBF16;
             args.m = m; args.n = n; args.k = k; args.error_word = err;
             ok = cuda_ok(launch_gemm_mx(args, stream), "mxfp4 GEMM kernel");
-            g_launches += 2;
+            g_launches += inside ? 1 : 2;
         }
     }
     if (ok && packed_kind == kMemHost && !ops.on_host()) ok = cuda_ok(cudaStreamSynchronize(stream), "mxfp4 product");

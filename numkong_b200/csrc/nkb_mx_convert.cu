@@ -6,12 +6,14 @@
 // nearest, ties to the even code. X comes from the exponent field of t alone and the division is a multiplication with a
 // power of two, so nothing before the one rounding is inexact. A block that holds an infinity or a NaN gets the NaN scale and
 // zero codes.
+// (nkb_mx_encode.cuh).
 //
-// All three kernels are bound by memory: 2 (4) bytes in and 0.53 bytes out per bf16 (f32) value, or the other way round.
+// All kernels here are bound by memory: 2 (4) bytes in and 0.53 bytes out per bf16 (f32) value, or the other way round.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "nkb_decode.cuh"
 #include "nkb_mx.h"
+#include "nkb_mx_encode.cuh"
 #include "nkb_ptx.cuh"
 
 namespace nkb {
@@ -25,26 +27,6 @@ struct RowMajorSink {
     uint8_t *codes, *scales;
     uint64_t codes_stride, scales_stride;
 };
-
-__device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits) {
-    const uint32_t e = largest_bits >> 23;           // biased exponent of the largest magnitude; 255: not finite
-    return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
-}
-// 1 / scale as an f32: 2^(127 - s), a normal number for every s a finite block can get (0 .. 252).
-__device__ __forceinline__ float inverse_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
-
-// Eight values over their scale -> eight codes, value 0 in the lowest four bits.
-__device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-    return r;
-}
 
 constexpr int kAhead = 4;  // chunk rows (256 values) a warp has in flight
 
@@ -144,35 +126,8 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
             for (int u = 0; u < kAhead; ++u) {
                 if (u >= (int)count) break;
                 float v[8];
-                uint32_t largest = 0;
-                if constexpr (kType == kBF16) {
-                    // Two values an instruction: the order of bf16 magnitudes is that of their bits, and scaling by a power of two is exact
-                    // (or ends below the smallest code).
-                    const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
-                    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-                    largest = max(m << 16, m & 0xffff0000u);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-                } else {
-#pragma unroll
-                    for (int h = 0; h < kBytes / 2; ++h) {
-                        const uint32_t w[4] = {raw[u][h].x, raw[u][h].y, raw[u][h].z, raw[u][h].w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if constexpr (kType == kF32) v[4 * h + i] = __uint_as_float(w[i]);
-                            else { v[2 * i] = decode_bits<kType>(w[i] & 0xffffu); v[2 * i + 1] = decode_bits<kType>(w[i] >> 16); }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);
-                }
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                const uint32_t s = scale_byte(largest);
-                const float inverse = inverse_scale(min(s, 253u));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= inverse;
-                const uint32_t codes = s == 255u ? 0u : encode8(v);
+                uint32_t s;
+                const uint32_t largest = unpack8<kType>(raw[u], v), codes = quantise8(v, largest, s);
                 store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
                 const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
                 if ((lane >> 3) == u) my_scale = mine;

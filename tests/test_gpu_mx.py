@@ -151,7 +151,7 @@ def test_large_product(m, n, k, rows_aligned, cells):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,n,k", [(1, 300, 512), (5, 128, 100), (70, 200, 321), (257, 384, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 512), (5, 128, 100), (9, 70, 255), (16, 20000, 777), (17, 300, 777), (70, 200, 321), (257, 384, 1024)])
 def test_product_of_floats_quantises_first(m, n, k, name):
     x, _ = stored(wide_values(m, k, m, -6, 6), name)
     b = random_mx(n, k, n)
@@ -162,6 +162,28 @@ def test_product_of_floats_quantises_first(m, n, k, name):
     assert torch.equal(got, two)
     q = nk.mx_quantise(x)
     check_product((q.codes.cpu().numpy(), q.scales.cpu().numpy()), b, k, got, "f32")
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
+def test_few_float_rows_off_their_boundaries(name):
+    """Up to 16 float rows are quantised inside the product: strides and offsets of every kind, rows of infinities and NaN."""
+    n, k = 200, 515
+    b = random_mx(n, k, 3)
+    packed = nk.dots_pack(nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), k))
+    for rows in (1, 2, 8, 13, 16):
+        wide = np.zeros((rows, k + 9), np.float32)
+        wide[:, 4:4 + k] = wide_values(rows, k, rows, -6, 6)
+        t = stored(wide, name)[0].cuda()
+        for first in (4, 3):
+            x = t[:, first:first + k]
+            got, two = nk.dots_packed(x, packed), nk.dots_packed(nk.mx_quantise(x), packed)
+            assert nk.synchronize() == 0
+            assert torch.equal(got, two)
+    x = torch.ones(3, k, device="cuda", dtype=TORCH[name])
+    x[1, 40], x[2, 7] = float("inf"), float("nan")
+    got = nk.dots_packed(x, packed)
+    assert nk.synchronize() == 0
+    assert got[0].isfinite().all() and got[1].isnan().all() and got[2].isnan().all()
 
 
 def test_rows_do_not_depend_on_one_another():
