@@ -804,7 +804,7 @@ def _packed_mx(a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], out
         raise ValueError(f"depth mismatch: a has {depth} dimensions, packed matrix has depth {packed.depth}")
     x = v.codes if isinstance(v, MxMatrix) else v.obj
     result, stride = _mx_result(x, v.rows, packed.width, out, out_dtype)
-    if isinstance(v, MxMatrix) or v.rows > 16:  # up to 16 float rows are quantised inside the product
+    if isinstance(v, MxMatrix) or v.rows > 2:  # one or two float rows are quantised inside the product
         workspace, ws = _workspace(x, (v.rows + 127) // 128 * ((depth + 255) // 256) * 17408)  # nkb_dots_workspace_mxfp4
     else:
         workspace = ws = None

@@ -1,8 +1,8 @@
 // What surrounds the grouped product of the experts: the order of the slots by expert, zero rows for slots without one, and
 // the weighted sum of a token's rows.
 //
-// A slot is one (token, choice) pair. The product wants every expert's slots in row tiles of up to 128, so the slots are
-// counted per expert, each expert gets ceil(count / 128) tiles, and each slot a place in its expert's tiles. Which place does
+// A slot is one (token, choice) pair. The product wants every expert's slots in row tiles of up to 128 (or 256), so the slots are
+// counted per expert, each expert gets the tiles its count fills, and each slot a place in its expert's tiles. Which place does
 // not matter to the result: rows of a product do not depend on one another.
 #include <cuda_bf16.h>
 #include "nkb_mx.h"
@@ -16,7 +16,7 @@ constexpr int kOrderThreads = 1024;
 // One block: slots are counted per expert in shared memory, a scan over the experts gives every expert its tiles, and a second pass
 // over the slots takes the places. 16,384 slots of 32 experts.
 __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t *ids, uint32_t slots, uint32_t experts, MxRowTile *tiles,
-                                                                     int32_t *tile_count, int32_t *row_dest) {
+                                                                     int32_t *tile_count, int32_t *row_dest, uint32_t tile_rows) {
     static_assert(kRouteMaxExperts <= kOrderThreads, "one thread per expert");
     __shared__ uint32_t count[kRouteMaxExperts], next_row[kRouteMaxExperts], warp_sums[kOrderThreads / 32];
     const uint32_t t = threadIdx.x, lane = t & 31u;
@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
         if (e >= 0 && e < (int32_t)experts) atomicAdd(&count[e], 1u);
     }
     __syncthreads();
-    const uint32_t mine = t < experts ? count[t] : 0u, my_tiles = (mine + 127u) / 128u;
+    const uint32_t mine = t < experts ? count[t] : 0u, my_tiles = (mine + tile_rows - 1u) / tile_rows;
     uint32_t through = my_tiles;  // inclusive sum over the experts
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -50,13 +50,13 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     if (t == kOrderThreads - 1) *tile_count = (int32_t)through;
     if (t < experts) {
         uint32_t tile = through - my_tiles, left = mine;
-        next_row[t] = tile * 128u;
-        for (; tile < through; ++tile, left -= 128u) tiles[tile] = {(int32_t)t, (int32_t)min(left, 128u)};
+        next_row[t] = tile * tile_rows;
+        for (; tile < through; ++tile, left -= tile_rows) tiles[tile] = {(int32_t)t, (int32_t)min(left, tile_rows)};
     }
     __syncthreads();
     // Rows behind an expert's last slot belong to nobody.
     for (uint32_t e = t >> 5; e < experts; e += kOrderThreads / 32)
-        for (uint32_t r = count[e] + lane; r < (count[e] + 127u) / 128u * 128u; r += 32) row_dest[next_row[e] + r] = -1;
+        for (uint32_t r = count[e] + lane; r < (count[e] + tile_rows - 1u) / tile_rows * tile_rows; r += 32) row_dest[next_row[e] + r] = -1;
     __syncthreads();
     for (uint32_t s = t; s < slots; s += kOrderThreads) {
         const int32_t e = ids[s];
@@ -115,9 +115,9 @@ uint32_t blocks_for(uint64_t n) { return (uint32_t)(n < 148ull * 32 ? (n ? n : 1
 } // namespace
 
 cudaError_t launch_expert_order(const int32_t *ids, uint64_t slots, uint32_t experts, MxRowTile *tiles, int32_t *tile_count, int32_t *row_dest,
-                                uint64_t max_tiles, cudaStream_t stream) {
+                                uint64_t max_tiles, uint32_t tile_rows, cudaStream_t stream) {
     if (slots > 0x7fffff00ull || max_tiles > 0x00ffffffull) return cudaErrorInvalidValue;
-    expert_order_kernel<<<1, kOrderThreads, 0, stream>>>(ids, (uint32_t)slots, experts, tiles, tile_count, row_dest);
+    expert_order_kernel<<<1, kOrderThreads, 0, stream>>>(ids, (uint32_t)slots, experts, tiles, tile_count, row_dest, tile_rows);
     return cudaGetLastError();
 }
 

@@ -9,8 +9,8 @@
 // e2m1 products are multiples of 1/4 of at most 36, so a block's sum is exact and the accumulator only loses bits when the
 // block scales of a row spread over more than 2^10.
 //
-// One persistent CTA per SM, fourteen warps: warp 0 brings chunks to shared memory with untiled bulk copies, warp 1 issues the
-// MMAs, warps 2..9 read the accumulators out and store the cells, warps 10..13 store scales.
+// One persistent CTA per SM: warp 0 brings B to shared memory with untiled bulk copies and warp 14 brings A, warp 1 issues the MMAs,
+// warps 2..9 read the accumulators out and store the cells, warps 10..13 store scales.
 #include <cuda_bf16.h>
 #include <type_traits>
 #include "nkb_mx.h"
@@ -24,12 +24,13 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kEpilogueWarps = 8;
 constexpr int kScaleWarps = 4;
-constexpr int kThreads = 64 + 32 * (kEpilogueWarps + kScaleWarps);
-constexpr uint32_t kMxChunkLines = kMxChunkBytes / 128;  // a chunk as rows of 128 bytes: 128 of codes, 8 of scales
+constexpr int kThreads = 64 + 32 * (kEpilogueWarps + kScaleWarps + 1);
+constexpr int kSecondLoader = 2 + kEpilogueWarps + kScaleWarps;  // warp that fetches A
 constexpr uint32_t kGroupM = 8;      // row tiles walked before the next column tile
 
 struct MxGemmDev {
-    const uint8_t *a_chunks, *b_chunks;
+    const uint8_t *a_codes, *a_scales;  // tile form: codes and scales of the first chunk; with a_row_major only the scales
+    const uint8_t *b_codes, *b_scales;
     uint8_t *c;
     uint64_t c_stride;
     uint32_t m, n, kblocks;
@@ -37,31 +38,34 @@ struct MxGemmDev {
     uint32_t group_blocks;           // row blocks of 128 per packed matrix
     const MxRowTile *tiles;
     const int32_t *tile_count, *row_dest;
-    uint32_t a_row_major;            // A's codes are read from the caller's rows, only its scales are in tile form
-    const uint8_t *a_scales;         // scale tiles of A's first chunk, and the bytes from one chunk's to the next
-    uint64_t a_scale_step;
-    const uint8_t *x;                // float rows of A the kernel quantises itself (m <= 16), their stride, type and length
+    uint32_t a_row_major;            // A's codes are read from the caller's rows
+    uint32_t a_blocks;               // row blocks A's buffers hold
+    const uint8_t *x;                // float rows of A the kernel quantises itself, their stride, type and length
     uint64_t x_stride;
     uint32_t x_type, k;
     unsigned int *error_word;
     uint32_t wait_us[kWaitSites];
 };
 
-// Shared memory of the single-CTA kernel. The MMA always reads 128 rows of A; with kARows = 16 a stage holds 16 of them and the rest of
-// what it reads is the stages behind (and 14 KiB of slack): rows of the accumulator nobody looks at. That leaves room for more
-// stages of B, which is what a product with few rows waits for.
+// Shared memory of the single-CTA kernel: a ring of stages with the codes of A and B, and a ring of groups of four chunks' scales
+// (a bulk copy costs its issuer about 110 cycles whatever its size, so scales come four chunks at a time). The MMA always reads 128 rows of
+// A; with kARows = 16 a stage holds 16 of them and the rest of what it reads is the stages behind (and 14 KiB of slack): rows of the
+// accumulator nobody looks at. That leaves room for more stages of B, which is what a product with few rows waits for.
+constexpr uint32_t kScaleGroup = 4, kScaleRing = 3;
 template <int kBN, int kARows>
 struct Plan {
     static constexpr int kABytes = kARows * 128, kBBytes = kBN * 128;
-    static constexpr int kStageBytes = kBBytes + 2 * kMxScaleBytes;    // B codes, A scales, B scales; A's codes have a ring of their own
-    static constexpr int kRoom = 176 * 1024 - (kBM - kARows) * 128;
-    static constexpr int kStages = kRoom / (kStageBytes + kABytes) < 16 ? kRoom / (kStageBytes + kABytes) : 16;
+    static constexpr int kScaleBytes = kScaleRing * 2 * kScaleGroup * kMxScaleBytes;  // per group: A's tiles, B's tiles
+    static constexpr int kStagingPitch = 144;  // bytes per staged row: 128 and one 16-byte piece against bank conflicts
+    static constexpr int kStagingBytes = kEpilogueWarps * 32 * kStagingPitch;
+    static constexpr int kRoom = 227 * 1024 - 1024 - 512 - kStagingBytes - kScaleBytes - (kBM - kARows) * 128;
+    static constexpr int kStages = kRoom / (kBBytes + kABytes) < 16 ? kRoom / (kBBytes + kABytes) : 16;
     static constexpr int kBRing = kStages * kABytes + (kBM - kARows) * 128;
-    static constexpr int kBarrierOffset = kBRing + kStages * kStageBytes;
-    static constexpr int kStagingPitch = 144;                          // bytes per staged row: 128 and one 16-byte piece against bank conflicts
+    static constexpr int kScaleOffset = kBRing + kStages * kBBytes;
+    static constexpr int kBarrierOffset = kScaleOffset + kScaleBytes;
     static constexpr int kStagingOffset = kBarrierOffset + 512;
-    static constexpr int kTotal = kStagingOffset + kEpilogueWarps * 32 * kStagingPitch + 1024;
-    static_assert(kBRing % 1024 == 0 && kStageBytes % 1024 == 0 && kTotal <= 227 * 1024, "aligned operands that fit");
+    static constexpr int kTotal = kStagingOffset + kStagingBytes + 1024;
+    static_assert(kBRing % 1024 == 0 && kTotal <= 227 * 1024, "aligned operands that fit");
 };
 
 __device__ __forceinline__ void tile_coords(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t &mt, uint32_t &nt) {
@@ -147,18 +151,32 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[kCols], const M
     }
 }
 
-// The (tile, depth block) sequence of one CTA or CTA pair out of `step`.
+// The (tile, depth block) sequence of one CTA or CTA pair out of `step`, with the rows and the packed matrix of its tile.
+template <int kTileRows>
 struct Walk {
-    uint32_t tile, kb, mt, nt, tiles_m, tiles_n, kblocks, step;
-    __device__ Walk(uint32_t first, uint32_t step_, uint32_t tiles_m_, uint32_t tiles_n_, uint32_t kblocks_)
-        : tile(first), kb(0), mt(0), nt(0), tiles_m(tiles_m_), tiles_n(tiles_n_), kblocks(kblocks_), step(step_) { locate(); }
-    __device__ bool valid() const { return tile < tiles_m * tiles_n; }
-    __device__ void locate() { if (valid()) tile_coords(tile, tiles_m, tiles_n, mt, nt); }
-    __device__ void next() {
-        if (++kb < kblocks) return;
+    const MxGemmDev &p;
+    uint32_t tile, kb, mt, nt, tiles_m, step, rows, group;
+    __device__ Walk(const MxGemmDev &p_, uint32_t first, uint32_t step_, uint32_t tiles_m_)
+        : p(p_), tile(first), kb(0), mt(0), nt(0), tiles_m(tiles_m_), step(step_), rows(0), group(0) { locate(); }
+    __device__ bool valid() const { return tile < tiles_m * p.tiles_n; }
+    __device__ void locate() {
+        if (!valid()) return;
+        tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+        if (p.tiles) {
+            const int2 t = *reinterpret_cast<const int2 *>(p.tiles + mt);
+            group = (uint32_t)t.x;
+            rows = (uint32_t)t.y;
+        } else {
+            rows = min(p.m - mt * kTileRows, (uint32_t)kTileRows);
+        }
+    }
+    __device__ void next_tile() {
         kb = 0;
         tile += step;
         locate();
+    }
+    __device__ void next() {
+        if (++kb == p.kblocks) next_tile();
     }
 };
 
@@ -192,11 +210,16 @@ __device__ __forceinline__ uint32_t quantise_row8(const uint4 (&raw)[2], uint32_
     return quantise8(v, largest, scale);
 }
 
-// With kOwnA the epilogue warps quantise A's few rows chunk by chunk into the ring while the packed matrix streams in: one launch and
-// no workspace, at the price of every CTA doing it again.
+// How kOwnA shares the chunks out: `width` warps, two rows each, work on one chunk, so that `sets` chunks are in hand at a time.
+struct OwnShare {
+    uint32_t width, sets;
+    __host__ __device__ explicit OwnShare(uint32_t m) : width((m + 1) / 2), sets(kEpilogueWarps / ((m + 1) / 2)) {}
+};
+
+// With kOwnA the epilogue warps quantise A's few rows chunk by chunk into the rings while the packed matrix streams in: one launch
+// and no workspace, at the price of every CTA doing it again.
 template <int kBN, int kARows, bool kOwnA, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p) {
-    static_assert(!kOwnA || kARows == 2 * kEpilogueWarps, "two rows a warp");
     using P = Plan<kBN, kARows>;
     constexpr int kStages = P::kStages;
     constexpr int kColsPerThread = kBN / 2;
@@ -210,15 +233,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     const uint32_t bar_base = smem_base + P::kBarrierOffset;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
-    auto scale_bar = [&](int s) { return bar_base + 8u * (2 * kStages + s); };  // the stage's scales are in TMEM
-    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (3 * kStages + a); };
-    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (3 * kStages + 2 + a); };
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + P::kBarrierOffset + 8 * (3 * kStages + 4));
-    const uint32_t drain_bar = bar_base + 8u * (3 * kStages + 5);
+    auto scale_full_bar = [&](uint32_t g) { return bar_base + 8u * (2 * kStages + g); };
+    auto scale_empty_bar = [&](uint32_t g) { return bar_base + 8u * (2 * kStages + kScaleRing + g); };
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * kStages + 2 * kScaleRing + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (2 * kStages + 2 * kScaleRing + 2 + a); };
+    const uint32_t drain_bar = bar_base + 8u * (2 * kStages + 2 * kScaleRing + 4);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + P::kBarrierOffset + 8 * (2 * kStages + 2 * kScaleRing + 5));
+    static_assert(8 * (2 * kStages + 2 * kScaleRing + 6) <= 512, "barriers fit");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), kOwnA ? 1 + kEpilogueWarps : 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), kScaleWarps); }
+        // A stage is full when B's loader, A's loader or quantisers and the scale warps have arrived.
+        const uint32_t fillers = (kOwnA ? 1 + OwnShare(p.m).width : 2) + kScaleWarps;
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), fillers); mbar_init(empty_bar(s), 1); }
+        for (uint32_t g = 0; g < kScaleRing; ++g) { mbar_init(scale_full_bar(g), kOwnA ? 1 + kEpilogueWarps : 2); mbar_init(scale_empty_bar(g), kScaleWarps); }
         for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(tmem_empty_bar(a), kEpilogueWarps * 32); }
         mbar_init(drain_bar, 1);
         fence_mbar_init();
@@ -232,161 +260,179 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tiles_m = p.tile_count ? (uint32_t)*p.tile_count : p.tiles_m;
-    const uint32_t num_tiles = tiles_m * p.tiles_n;
-    auto rows_of = [&](uint32_t mt) { return p.tiles ? (uint32_t)p.tiles[mt].rows : min(p.m - mt * kBM, (uint32_t)kBM); };
 
-    if (warp == 0) {
-        if (lane == 0) {
-            // Only the row groups of eight that hold valid rows of A are fetched. A tile's rows and group are looked up once.
-            struct Tile { uint32_t tile, a_bytes, group; };
-            auto tile_of = [&](const Walk &w, Tile &t) -> const Tile & {
-                if (t.tile != w.tile) t = {w.tile, (rows_of(w.mt) + 7u) / 8u * 1024u, p.tiles ? (uint32_t)p.tiles[w.mt].group : 0u};
-                return t;
-            };
-            Tile b_tile{0xffffffffu, 0, 0}, a_tile{0xffffffffu, 0, 0};
-            auto load_b = [&](const Walk &w, int stage) {
-                const Tile &t = tile_of(w, b_tile);
-                const uint32_t block = w.nt * kBN / 128u, sub = w.nt * kBN % 128u;
-                const uint8_t *b = p.b_chunks + (((uint64_t)t.group * p.group_blocks + block) * p.kblocks + w.kb) * kMxChunkBytes;
-                const uint32_t dst = smem_base + P::kBRing + stage * P::kStageBytes;
-                mbar_expect_tx(full_bar(stage), (kOwnA ? 0u : t.a_bytes + kMxScaleBytes) + P::kBBytes + kMxScaleBytes);
-                bulk_load(dst, b + sub * 128u, P::kBBytes, full_bar(stage));
-                bulk_load(dst + P::kBBytes + kMxScaleBytes, b + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
-            };
-            auto load_a = [&](const Walk &w, int stage) {
-                const uint8_t *a = p.a_chunks + ((uint64_t)w.mt * p.kblocks + w.kb) * kMxChunkBytes;
-                bulk_load(smem_base + stage * P::kABytes, a, tile_of(w, a_tile).a_bytes, full_bar(stage));
-                bulk_load(smem_base + P::kBRing + stage * P::kStageBytes + P::kBBytes, a + kMxCodeBytes, kMxScaleBytes, full_bar(stage));
-            };
-            int stage = 0;
-            uint32_t phase = 0, issued = 0;
-            bool ok = true;
-            Walk w(blockIdx.x, gridDim.x, tiles_m, p.tiles_n, p.kblocks);
-            // The packed matrix does not depend on the kernel before, which is still quantising A.
-            Walk early = w;
-            for (int s = 0; s < kStages && early.valid(); ++s, early.next()) load_b(early, s);
-            if constexpr (!kOwnA) wait_for_previous_kernel();
-            for (; w.valid(); w.next()) {
-                if (issued >= (uint32_t)kStages) {
-                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
-                    load_b(w, stage);
-                }
-                if constexpr (!kOwnA) load_a(w, stage);
-                ++issued;
-                if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    // One loader for each operand: its scales four chunks at a time, its codes chunk by chunk.
+    auto run_loader = [&](uint32_t scale_part, auto scale_source, auto code_bytes, auto code_copy) {
+        int stage = 0;
+        uint32_t phase = 0, group = 0, group_phase = 0, issued = 0, groups = 0;
+        bool ok = true;
+        for (Walk<kBM> w(p, blockIdx.x, gridDim.x, tiles_m); w.valid(); w.next()) {
+            if (w.kb % kScaleGroup == 0) {
+                if (!mbar_wait(scale_empty_bar(group), group_phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
+                const uint32_t bytes = min(kScaleGroup, p.kblocks - w.kb) * kMxScaleBytes;
+                mbar_expect_tx(scale_full_bar(group), bytes);
+                bulk_load(smem_base + P::kScaleOffset + (2 * group + scale_part) * kScaleGroup * kMxScaleBytes, scale_source(w), bytes, scale_full_bar(group));
+                ++groups;
+                if (++group == kScaleRing) { group = 0; group_phase ^= 1u; }
             }
-            if (!ok) {  // copies in flight must land before the block may retire
-                int s = stage;
-                uint32_t ph = phase;
-                for (uint32_t i = 0; i < issued && i < (uint32_t)kStages; ++i) {
-                    if (s == 0) { s = kStages; ph ^= 1u; }
-                    --s;
-                    if (!mbar_wait(full_bar(s), ph, 6, p.error_word, p.wait_us[6])) break;
-                }
+            if (!mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
+            mbar_expect_tx(full_bar(stage), code_bytes(w));
+            code_copy(w, stage);
+            ++issued;
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) {  // copies in flight must land before the block may retire
+            for (uint32_t i = 0; i < issued && i < (uint32_t)kStages; ++i) {
+                if (stage == 0) { stage = kStages; phase ^= 1u; }
+                --stage;
+                if (!mbar_wait(full_bar(stage), phase, 6, p.error_word, p.wait_us[6])) break;
+            }
+            for (uint32_t i = 0; i < groups && i < kScaleRing; ++i) {
+                if (group == 0) { group = kScaleRing; group_phase ^= 1u; }
+                --group;
+                if (!mbar_wait(scale_full_bar(group), group_phase, 6, p.error_word, p.wait_us[6])) break;
             }
         }
-    } else if (warp == 1) {
+    };
+
+    if (warp == 0) {
+        // The packed matrix does not depend on the kernel before, which may still be quantising A.
         if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0, seq = 0;
-            bool ok = true;
-            for (uint32_t tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++seq) {
-                uint32_t mt, nt;
-                tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
-                const uint32_t b_column = 8u + nt * kBN % 128u / 32u;  // the tile's rows inside the row block's scales
-                const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
-                if (!mbar_wait(tmem_empty_bar(buf), buf_phase ^ 1u, 2, p.error_word, p.wait_us[2])) { ok = false; break; }
+            auto chunk = [&](const Walk<kBM> &w) { return ((uint64_t)w.group * p.group_blocks + w.nt * kBN / 128u) * p.kblocks + w.kb; };
+            run_loader(1, [&](const Walk<kBM> &w) { return p.b_scales + chunk(w) * kMxScaleBytes; }, [&](const Walk<kBM> &) { return (uint32_t)P::kBBytes; },
+                       [&](const Walk<kBM> &w, int stage) {
+                           bulk_load(smem_base + P::kBRing + stage * P::kBBytes, p.b_codes + chunk(w) * kMxCodeBytes + w.nt * kBN % 128u * 128u, P::kBBytes, full_bar(stage));
+                       });
+        }
+    } else if (warp == kSecondLoader) {
+        if (!kOwnA && lane == 0) {
+            wait_for_previous_kernel();
+            auto chunk = [&](const Walk<kBM> &w) { return (uint64_t)w.mt * p.kblocks + w.kb; };
+            auto bytes = [&](const Walk<kBM> &w) { return (w.rows + 7u) / 8u * 1024u; };  // the row groups of eight that hold valid rows
+            run_loader(0, [&](const Walk<kBM> &w) { return p.a_scales + chunk(w) * kMxScaleBytes; }, bytes,
+                       [&](const Walk<kBM> &w, int stage) { bulk_load(smem_base + stage * P::kABytes, p.a_codes + chunk(w) * kMxCodeBytes, bytes(w), full_bar(stage)); });
+        }
+    } else if (warp == 1) {
+        // The whole warp walks, one lane issues (see elect_one).
+        uint32_t stage = 0, phase = 0, seq = 0;
+        bool ok = true;
+        const uint32_t num_tiles = tiles_m * p.tiles_n;
+        for (uint32_t tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++seq) {
+            uint32_t mt, nt;
+            tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+            const uint32_t b_column = 8u + nt * kBN % 128u / 32u;  // the tile's rows inside the row block's scales
+            const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(buf), buf_phase ^ 1u, 2, p.error_word, p.wait_us[2]))) { ok = false; break; }
+            tc_fence_after_sync();
+            const uint32_t d_tmem = tmem_base + buf * kBN;
+            for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+                if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3]))) { ok = false; break; }
                 tc_fence_after_sync();
-                const uint32_t d_tmem = tmem_base + buf * kBN;
-                for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-                    if (!mbar_wait(scale_bar(stage), phase, 3, p.error_word, p.wait_us[3]) ||
-                        !mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
-                    tc_fence_after_sync();
-                    const uint32_t src = smem_base + P::kBRing + stage * P::kStageBytes, scales = tmem_base + 2 * kBN + stage * kScaleCols;
-                    const uint64_t a_desc = make_smem_desc_sw128(smem_base + stage * P::kABytes), b_desc = make_smem_desc_sw128(src);
+                const uint32_t scales = tmem_base + 2 * kBN + stage * kScaleCols;
+                const uint64_t a_desc = make_smem_desc_sw128(smem_base + stage * P::kABytes), b_desc = make_smem_desc_sw128(smem_base + P::kBRing + stage * P::kBBytes);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         umma_mxf4<1>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(kBM, kBN, (k & 1) * 2), scales + (k >> 1) * 4,
                                      scales + b_column + (k >> 1) * 4, (kb | (uint32_t)k) != 0u);
                     umma_commit(empty_bar(stage));
-                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    if (kb + 1 == p.kblocks) umma_commit(tmem_full_bar(buf));
                 }
-                if (ok) umma_commit(tmem_full_bar(buf));
+                __syncwarp();
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
-            umma_commit(drain_bar);  // shared memory and TMEM are released below: the last MMAs must have retired
-            mbar_wait(drain_bar, 0u, 5, p.error_word, p.wait_us[5]);
         }
+        if (elect_one()) umma_commit(drain_bar);  // shared memory and TMEM are released below: the last MMAs must have retired
+        __syncwarp();
+        mbar_wait(drain_bar, 0u, 5, p.error_word, p.wait_us[5]);
+        __syncwarp();
     } else if (warp >= 2 + kEpilogueWarps) {
         // ------------------------------------------------------------ scales: shared memory -> this warp's 32-lane quarter of TMEM
         // A stage has TMEM columns of its own, free again when the stage is.
         const uint32_t column = tmem_base + (((uint32_t)warp & 3u) * 32u << 16) + 2 * kBN;
         int stage = 0;
-        uint32_t phase = 0;
-        for (Walk w(blockIdx.x, gridDim.x, tiles_m, p.tiles_n, p.kblocks); w.valid(); w.next()) {
-            if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, 3, p.error_word, p.wait_us[3]))) break;
+        uint32_t phase = 0, group = 0, group_phase = 0;
+        for (Walk<kBM> w(p, blockIdx.x, gridDim.x, tiles_m); w.valid(); w.next()) {
+            const uint32_t in_group = w.kb % kScaleGroup;
+            bool ok = in_group != 0 || mbar_wait(scale_full_bar(group), group_phase, 3, p.error_word, p.wait_us[3]);
+            ok = ok && mbar_wait(empty_bar(stage), phase ^ 1u, 2, p.error_word, p.wait_us[2]);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after_sync();
-            const uint4 *tiles = reinterpret_cast<const uint4 *>(smem_gen + P::kBRing + stage * P::kStageBytes + P::kBBytes) + lane;
+            const uint4 *tiles = reinterpret_cast<const uint4 *>(smem_gen + P::kScaleOffset + (2 * group * kScaleGroup + in_group) * kMxScaleBytes) + lane;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint4 lo = tiles[i * 64], hi = tiles[i * 64 + 32];
+                const uint4 lo = tiles[i * kScaleGroup * kMxScaleBytes / 16], hi = tiles[i * kScaleGroup * kMxScaleBytes / 16 + 32];
                 const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                 tmem_st_32x8(column + stage * kScaleCols + i * 8, words);
             }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(scale_bar(stage));
+            const bool last = in_group == kScaleGroup - 1 || w.kb + 1 == p.kblocks;
+            if (lane == 0) {
+                mbar_arrive(full_bar(stage));  // the stage's scales are in TMEM
+                if (last) mbar_arrive(scale_empty_bar(group));
+            }
+            if (last && ++group == kScaleRing) { group = 0; group_phase ^= 1u; }
             if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
     } else {
         const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
         uint8_t *staging = smem_gen + P::kStagingOffset + (warp - 2) * 32 * P::kStagingPitch;
-        uint32_t seq = 0, phase = 0;
+        uint32_t seq = 0, phase = 0, group = 0, group_phase = 0, chunk = 0;
         int stage = 0;
-        for (uint32_t tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++seq) {
-            uint32_t mt, nt;
-            tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+        for (Walk<kBM> w(p, blockIdx.x, gridDim.x, tiles_m); w.valid(); w.next_tile(), ++seq) {
             if constexpr (kOwnA) {
-                bool ok = true;
+                const OwnShare share(p.m);
+                const uint32_t me = (uint32_t)warp - 2u, row0 = me % share.width * 2u, set = me / share.width;
                 auto own = [&](auto type) {
                     constexpr uint32_t kType = decltype(type)::value;
-                    const uint32_t rows[2] = {(uint32_t)warp - 2u, (uint32_t)warp - 2u + kEpilogueWarps};
-                    uint4 raw[2][2], next[2][2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (rows[h] < p.m) load_row8<kType>(p, rows[h], lane * 8, raw[h]);
-                    for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+                    uint4 raw[2][2];
+                    auto fetch = [&](uint32_t kb) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
-                            if (rows[h] < p.m && kb + 1 < p.kblocks) load_row8<kType>(p, rows[h], (kb + 1) * kMxChunkValues + lane * 8, next[h]);
-                        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1]))) { ok = false; break; }
-                        uint8_t *codes = smem_gen + stage * P::kABytes, *scales = smem_gen + P::kBRing + stage * P::kStageBytes + P::kBBytes;
+                            if (row0 + h < p.m && kb < p.kblocks) load_row8<kType>(p, row0 + h, kb * kMxChunkValues + lane * 8, raw[h]);
+                    };
+                    // This warp's first chunk of the tile is the first that its set is due for.
+                    if (set < share.sets) fetch((set + share.sets - chunk % share.sets) % share.sets);
+                    for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++chunk) {
+                        const uint32_t in_group = kb % kScaleGroup;
+                        bool ok = in_group != 0 || mbar_wait(scale_empty_bar(group), group_phase ^ 1u, 1, p.error_word, p.wait_us[1]);
+                        const bool mine = chunk % share.sets == set;
+                        if (ok && mine) ok = mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1]);
+                        if (!__all_sync(0xffffffffu, ok)) return false;
+                        if (mine) {
+                            uint8_t *codes = smem_gen + stage * P::kABytes, *scales = smem_gen + P::kScaleOffset + (2 * group * kScaleGroup + in_group) * kMxScaleBytes;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t r = rows[h];
-                            if (r >= p.m) continue;
-                            uint32_t s;
-                            const uint32_t word = quantise_row8<kType>(raw[h], s);
-                            *reinterpret_cast<uint32_t *>(codes + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = word;
-                            if ((lane & 3) == 0) scales[(lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)s;
-#pragma unroll
-                            for (int q = 0; q < 2; ++q) raw[h][q] = next[h][q];
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t r = row0 + h;
+                                if (r >= p.m) continue;
+                                uint32_t s;
+                                const uint32_t word = quantise_row8<kType>(raw[h], s);
+                                *reinterpret_cast<uint32_t *>(codes + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = word;
+                                if ((lane & 3) == 0) scales[(lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)s;
+                            }
+                            fetch(kb + share.sets);
+                            fence_proxy_async_smem();  // the MMA reads the codes through the other proxy
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(full_bar(stage));
                         }
-                        fence_proxy_async_smem();  // the MMA reads the codes through the other proxy
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(full_bar(stage));
+                        if (in_group == kScaleGroup - 1 || kb + 1 == p.kblocks) {
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(scale_full_bar(group));
+                            if (++group == kScaleRing) { group = 0; group_phase ^= 1u; }
+                        }
                         if (++stage == kStages) { stage = 0; phase ^= 1u; }
                     }
+                    return true;
                 };
-                if (p.x_type == kBF16) own(std::integral_constant<uint32_t, kBF16>{});
-                else if (p.x_type == kF16) own(std::integral_constant<uint32_t, kF16>{});
-                else own(std::integral_constant<uint32_t, kF32>{});
+                const bool ok = p.x_type == kBF16 ? own(std::integral_constant<uint32_t, kBF16>{})
+                                : p.x_type == kF16 ? own(std::integral_constant<uint32_t, kF16>{}) : own(std::integral_constant<uint32_t, kF32>{});
                 if (!ok) break;
             }
-            const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u;
-            const uint32_t in_tile = quarter * 32u + lane, rows = rows_of(mt);
+            const uint32_t buf = seq & 1u, buf_phase = (seq >> 1) & 1u, in_tile = quarter * 32u + lane;
             int64_t dest = -1;
-            if (in_tile < rows) dest = p.row_dest ? (int64_t)p.row_dest[(uint64_t)mt * kBM + in_tile] : (int64_t)mt * kBM + in_tile;
+            if (in_tile < w.rows) dest = p.row_dest ? (int64_t)p.row_dest[(uint64_t)w.mt * kBM + in_tile] : (int64_t)w.mt * kBM + in_tile;
             // The whole warp leaves together: the stores below synchronise it.
             if (!__all_sync(0xffffffffu, mbar_wait(tmem_full_bar(buf), buf_phase, 4, p.error_word, p.wait_us[4]))) break;
             tc_fence_after_sync();
@@ -398,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
             for (int c = 0; c < kColsPerThread / 32; ++c) tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[c * 32]));
             tc_fence_before_sync();
             mbar_arrive(tmem_empty_bar(buf));
-            store_rows<kBf16, kColsPerThread>(acc, p, dest, nt * kBN + half * kColsPerThread, staging, P::kStagingPitch, lane);
+            store_rows<kBf16, kColsPerThread>(acc, p, dest, w.nt * kBN + half * kColsPerThread, staging, P::kStagingPitch, lane);
         }
     }
     tc_fence_before_sync();
@@ -418,17 +464,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
 // [512 - scales - 256, 512 - scales). The epilogue reads the columns they share first and then lets the next tile's MMAs
 // start, so they wait for a part of a read-out instead of all of it.
 //
-// The scale warps load a chunk's scale tiles from global memory two chunks ahead. With tcgen05.cp in their place (six tiles a
-// chunk) 8192 x 8192 x 8192 took 253 us, with no scales moved at all 215.
+// Scales come by bulk copies, four chunks at a time, into a ring of their own. 8192 x 8192 x 8192 with the scale warps loading them from
+// global memory instead: 277 us, since their loads wait behind the stores of the epilogue; with tcgen05.cp, six tiles a chunk: 253 us.
 constexpr int kPairStages = 5;
 constexpr int kPairScaleCols = 24;                                // 8 for 128 rows of A, 16 for 256 of B
 constexpr int kPairSecond = 512 - 2 * kPairScaleCols - 256;       // first column of the second accumulator; two chunks' scales behind it
 constexpr int kPairBOffset = kBM * 128;
 constexpr int kPairStageBytes = 2 * kBM * 128;                    // A codes, B codes
-constexpr int kPairBarrierOffset = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairScaleRing = 2;                            // groups of four chunks' scales: A's tiles, both row blocks of B
+constexpr int kPairGroupBytes = 3 * kScaleGroup * kMxScaleBytes;
+constexpr int kPairScaleOffset = kPairStages * kPairStageBytes;
+constexpr int kPairBarrierOffset = kPairScaleOffset + kPairScaleRing * kPairGroupBytes;
 constexpr int kPairStagingPitch = 144;
 constexpr int kPairStagingOffset = kPairBarrierOffset + 256;
 constexpr int kPairSmem = kPairStagingOffset + kEpilogueWarps * 32 * kPairStagingPitch + 1024;
+static_assert(kPairSmem <= 227 * 1024, "one CTA per SM");
 static_assert(kPairSecond >= 256 - 64, "the shared columns are the last / first 64 of the two accumulators at most");
 
 struct PairMaps {
@@ -446,19 +496,22 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * kStages + a); };
-    auto scale_bar = [&](uint32_t b) { return bar_base + 8u * (2 * kStages + 2 + b); };  // a chunk's scales are in TMEM of both CTAs
     const uint32_t shared_read_bar = bar_base + 8u * (2 * kStages + 4);  // the tile before is read, of this one the shared columns
     const uint32_t drain_bar = bar_base + 8u * (2 * kStages + 5);
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kPairBarrierOffset + 8 * (2 * kStages + 6));
+    auto scale_full_bar = [&](uint32_t g) { return bar_base + 8u * (2 * kStages + 6 + g); };
+    auto scale_empty_bar = [&](uint32_t g) { return bar_base + 8u * (2 * kStages + 6 + kPairScaleRing + g); };
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kPairBarrierOffset + 8 * (2 * kStages + 6 + 2 * kPairScaleRing));
+    static_assert(8 * (2 * kStages + 7 + 2 * kPairScaleRing) <= 256, "barriers fit");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-    const uint32_t tiles_m = p.tiles_m, num_tiles = tiles_m * p.tiles_n;
+    const uint32_t tiles_m = p.tile_count ? (uint32_t)*p.tile_count : p.tiles_m, num_tiles = tiles_m * p.tiles_n;
     if (threadIdx.x == 0) {
         prefetch_tensormap(&maps.a);
         prefetch_tensormap(&maps.b);
-        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(scale_bar(a), 2 * kScaleWarps); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1 + 2 * kScaleWarps); mbar_init(empty_bar(s), 1); }  // copies and both CTAs' scales
+        for (int a = 0; a < 2; ++a) mbar_init(tmem_full_bar(a), 1);
+        for (uint32_t g = 0; g < kPairScaleRing; ++g) { mbar_init(scale_full_bar(g), 1); mbar_init(scale_empty_bar(g), kScaleWarps); }
         mbar_init(shared_read_bar, 2 * kEpilogueWarps);
         mbar_init(drain_bar, 1);
         fence_mbar_init();
@@ -479,14 +532,17 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
             uint32_t phase = 0, issued = 0;
             bool ok = true;
             wait_for_previous_kernel();
-            for (Walk w(pair, num_pairs, tiles_m, p.tiles_n, p.kblocks); w.valid(); w.next()) {
+            for (Walk<256> w(p, pair, num_pairs, tiles_m); w.valid(); w.next()) {
                 if (!mbar_wait<true>(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
                 const uint32_t dst = smem_base + stage * kPairStageBytes, full = map_to_cta(full_bar(stage), 0);
-                if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * kPairStageBytes);
-                const uint32_t a_block = w.mt * 2u + rank, b_block = w.nt * 2u + rank;
-                if (p.a_row_major) tma_load_2d_pair(dst, &maps.a, (int)(w.kb * 128u), (int)(a_block * kBM), full);
-                else tma_load_2d_pair(dst, &maps.a, 0, (int)((a_block * p.kblocks + w.kb) * kMxChunkLines), full);
-                tma_load_2d_pair(dst + kPairBOffset, &maps.b, 0, (int)((b_block * p.kblocks + w.kb) * kMxChunkLines), full);
+                const bool second = w.rows > kBM;  // the follower's rows of A exist
+                if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * kBM * 128 + (second ? 2 : 1) * kBM * 128);
+                const uint32_t a_block = w.mt * 2u + rank, b_block = w.group * p.group_blocks + w.nt * 2u + rank;
+                if (rank == 0 || second) {
+                    if (p.a_row_major) tma_load_2d_pair(dst, &maps.a, (int)(w.kb * 128u), (int)(a_block * kBM), full);
+                    else tma_load_2d_pair(dst, &maps.a, 0, (int)((a_block * p.kblocks + w.kb) * kBM), full);
+                }
+                tma_load_2d_pair(dst + kPairBOffset, &maps.b, 0, (int)((b_block * p.kblocks + w.kb) * kBM), full);
                 ++issued;
                 if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
@@ -507,97 +563,110 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            int stage = 0;
-            uint32_t phase = 0, seq = 0, chunk = 0;
+        if (rank == 0) {  // the whole warp walks, one lane issues (see elect_one)
+            uint32_t stage = 0, phase = 0, seq = 0, chunk = 0;
             bool ok = true;
             for (uint32_t tile = pair; tile < num_tiles && ok; tile += num_pairs, ++seq) {
-                if (seq > 0 && !mbar_wait<true>(shared_read_bar, (seq - 1u) & 1u, 2, p.error_word, p.wait_us[2])) { ok = false; break; }
+                if (seq > 0 && !__all_sync(0xffffffffu, mbar_wait<true>(shared_read_bar, (seq - 1u) & 1u, 2, p.error_word, p.wait_us[2]))) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t buf = seq & 1u, d_tmem = tmem_base + buf * kPairSecond;
                 for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++chunk) {
-                    if (!mbar_wait<true>(scale_bar(chunk & 1u), (chunk >> 1) & 1u, 3, p.error_word, p.wait_us[3]) ||
-                        !mbar_wait<true>(full_bar(stage), phase, 3, p.error_word, p.wait_us[3])) { ok = false; break; }
+                    if (!__all_sync(0xffffffffu, mbar_wait<true>(full_bar(stage), phase, 3, p.error_word, p.wait_us[3]))) { ok = false; break; }
                     tc_fence_after_sync();
                     const uint32_t src = smem_base + stage * kPairStageBytes;
                     const uint64_t a_desc = make_smem_desc_sw128(src), b_desc = make_smem_desc_sw128(src + kPairBOffset);
                     const uint32_t scales_a = tmem_base + kPairSecond + 256 + (chunk & 1u) * kPairScaleCols, scales_b = scales_a + 8;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_mxf4<2>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(256, 256, (k & 1) * 2), scales_a + (k >> 1) * 4,
-                                     scales_b + (k >> 1) * 8, (kb | (uint32_t)k) != 0u);
-                    umma_commit_pair(empty_bar(stage), 3);
+                        for (int k = 0; k < 4; ++k)
+                            umma_mxf4<2>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, make_idesc_mxf4(256, 256, (k & 1) * 2), scales_a + (k >> 1) * 4,
+                                         scales_b + (k >> 1) * 8, (kb | (uint32_t)k) != 0u);
+                        umma_commit_pair(empty_bar(stage), 3);
+                        if (kb + 1 == p.kblocks) umma_commit_pair(tmem_full_bar(buf), 3);
+                    }
+                    __syncwarp();
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
-                if (ok) umma_commit_pair(tmem_full_bar(buf), 3);
             }
-            umma_commit_pair(drain_bar, 1);
+            if (elect_one()) umma_commit_pair(drain_bar, 1);
+            __syncwarp();
             mbar_wait<true>(drain_bar, 0u, 5, p.error_word, p.wait_us[5]);
+            __syncwarp();
+        }
+    } else if (warp == kSecondLoader) {
+        // ------------------------------------------------------------ scales of this CTA's rows of A and of all rows of B
+        if (lane == 0) {
+            wait_for_previous_kernel();
+            const uint32_t a_last = p.a_blocks - 1, b_last = p.group_blocks - 1;
+            uint32_t group = 0, phase = 0, groups = 0;
+            bool ok = true;
+            for (Walk<256> w(p, pair, num_pairs, tiles_m); w.valid() && ok; w.next_tile()) {
+                const uint8_t *a = p.a_scales + (uint64_t)min(w.mt * 2u + rank, a_last) * p.kblocks * kMxScaleBytes;
+                const uint8_t *b[2];
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) b[j] = p.b_scales + (uint64_t)(w.group * p.group_blocks + min(w.nt * 2u + j, b_last)) * p.kblocks * kMxScaleBytes;
+                for (uint32_t kb = 0; kb < p.kblocks; kb += kScaleGroup) {
+                    if (!mbar_wait(scale_empty_bar(group), phase ^ 1u, 1, p.error_word, p.wait_us[1])) { ok = false; break; }
+                    const uint32_t bytes = min(kScaleGroup, p.kblocks - kb) * kMxScaleBytes, dst = smem_base + kPairScaleOffset + group * kPairGroupBytes;
+                    mbar_expect_tx(scale_full_bar(group), 3 * bytes);
+                    bulk_load(dst, a + (uint64_t)kb * kMxScaleBytes, bytes, scale_full_bar(group));
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j)
+                        bulk_load(dst + (1 + j) * kScaleGroup * kMxScaleBytes, b[j] + (uint64_t)kb * kMxScaleBytes, bytes, scale_full_bar(group));
+                    ++groups;
+                    if (++group == kPairScaleRing) { group = 0; phase ^= 1u; }
+                }
+            }
+            for (uint32_t i = 0; !ok && i < groups && i < kPairScaleRing; ++i) {  // copies in flight must land before the block may retire
+                if (group == 0) { group = kPairScaleRing; phase ^= 1u; }
+                --group;
+                if (!mbar_wait(scale_full_bar(group), phase, 6, p.error_word, p.wait_us[6])) break;
+            }
         }
     } else if (warp >= 2 + kEpilogueWarps) {
-        // ------------------------------------------------------------ scales: this warp's 32-lane quarter of TMEM
+        // ------------------------------------------------------------ scales: shared memory -> this warp's 32-lane quarter of TMEM
         const uint32_t column = tmem_base + (((uint32_t)warp & 3u) * 32u << 16) + kPairSecond + 256;
-        const uint32_t a_last = (p.m + kBM - 1) / kBM - 1, b_last = p.group_blocks - 1;
-        // Lane r of every quarter holds line r of each tile: A for both halves of the chunk's depth, B for both halves of its rows.
-        auto load = [&](const Walk &w, uint4 (&r)[6]) {
-            const uint64_t a_chunk = (uint64_t)min(w.mt * 2u + rank, a_last) * p.kblocks + w.kb;
-            const uint4 *a = reinterpret_cast<const uint4 *>(p.a_scales + a_chunk * p.a_scale_step) + lane;
-            r[0] = a[0];
-            r[1] = a[32];
-#pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                const uint64_t b_chunk = (uint64_t)min(w.nt * 2u + j, b_last) * p.kblocks + w.kb;
-                const uint4 *b = reinterpret_cast<const uint4 *>(p.b_chunks + b_chunk * kMxChunkBytes + kMxCodeBytes) + lane;
-                r[2 + j] = __ldg(b);
-                r[4 + j] = __ldg(b + 32);
-            }
-        };
-        uint32_t chunk = 0;
-        int freed = 0;            // stage of the chunk whose scales are overwritten next
-        uint32_t freed_phase = 0;
-        auto store = [&](const uint4 (&r)[6]) {
+        uint32_t chunk = 0, group = 0, group_phase = 0, freed_phase = 0;
+        int stage = 0, freed = 0;  // of the chunk being stored, and of the one whose scales it overwrites
+        for (Walk<256> w(p, pair, num_pairs, tiles_m); w.valid(); w.next(), ++chunk) {
+            const uint32_t in_group = w.kb % kScaleGroup;
+            if (in_group == 0 && !__all_sync(0xffffffffu, mbar_wait(scale_full_bar(group), group_phase, 3, p.error_word, p.wait_us[3]))) break;
+            // Lane r of every quarter holds line r of each tile: A for both halves of the chunk's depth, B for both halves of its rows.
+            const uint4 *tiles = reinterpret_cast<const uint4 *>(smem_gen + kPairScaleOffset + group * kPairGroupBytes + in_group * kMxScaleBytes) + lane;
+            constexpr int kPart = kScaleGroup * kMxScaleBytes / 16;
+            const uint4 r[6] = {tiles[0], tiles[32], tiles[kPart], tiles[2 * kPart], tiles[kPart + 32], tiles[2 * kPart + 32]};
             if (chunk >= 2) {  // the MMAs of two chunks ago have read theirs
-                if (!__all_sync(0xffffffffu, mbar_wait<true>(empty_bar(freed), freed_phase, 2, p.error_word, p.wait_us[2]))) return false;
+                if (!__all_sync(0xffffffffu, mbar_wait<true>(empty_bar(freed), freed_phase, 2, p.error_word, p.wait_us[2]))) break;
                 if (++freed == kStages) { freed = 0; freed_phase ^= 1u; }
                 tc_fence_after_sync();
             }
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
-                const uint32_t w[8] = {r[2 * i].x, r[2 * i].y, r[2 * i].z, r[2 * i].w, r[2 * i + 1].x, r[2 * i + 1].y, r[2 * i + 1].z, r[2 * i + 1].w};
-                tmem_st_32x8(column + (chunk & 1u) * kPairScaleCols + i * 8, w);
+                const uint32_t words[8] = {r[2 * i].x, r[2 * i].y, r[2 * i].z, r[2 * i].w, r[2 * i + 1].x, r[2 * i + 1].y, r[2 * i + 1].z, r[2 * i + 1].w};
+                tmem_st_32x8(column + (chunk & 1u) * kPairScaleCols + i * 8, words);
             }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(scale_bar(chunk & 1u), 0));
-            ++chunk;
-            return true;
-        };
-        wait_for_previous_kernel();
-        Walk ahead(pair, num_pairs, tiles_m, p.tiles_n, p.kblocks);
-        uint4 even[6], odd[6];
-        bool has_even = ahead.valid(), has_odd = false;
-        if (has_even) { load(ahead, even); ahead.next(); }
-        has_odd = ahead.valid();
-        if (has_odd) { load(ahead, odd); ahead.next(); }
-        while (has_even) {
-            if (!store(even)) break;
-            if ((has_even = ahead.valid())) { load(ahead, even); ahead.next(); }
-            if (!has_odd || !store(odd)) break;
-            if ((has_odd = ahead.valid())) { load(ahead, odd); ahead.next(); }
+            const bool last = in_group == kScaleGroup - 1 || w.kb + 1 == p.kblocks;
+            if (lane == 0) {
+                mbar_arrive_cluster_addr(map_to_cta(full_bar(stage), 0));
+                if (last) mbar_arrive(scale_empty_bar(group));
+            }
+            if (last && ++group == kPairScaleRing) { group = 0; group_phase ^= 1u; }
+            if (++stage == kStages) stage = 0;
         }
     } else {
         const uint32_t quarter = warp & 3u, half = (uint32_t)(warp - 2) >> 2;
         uint8_t *staging = smem_gen + kPairStagingOffset + (warp - 2) * 32 * kPairStagingPitch;
         uint32_t seq = 0;
-        for (uint32_t tile = pair; tile < num_tiles; tile += num_pairs, ++seq) {
-            uint32_t mt, nt;
-            tile_coords(tile, tiles_m, p.tiles_n, mt, nt);
+        for (Walk<256> w(p, pair, num_pairs, tiles_m); w.valid(); w.next_tile(), ++seq) {
             const uint32_t buf = seq & 1u;
+            const uint32_t in_tile = rank * 128u + quarter * 32u + lane;
+            int64_t dest = -1;
+            if (in_tile < w.rows) dest = p.row_dest ? (int64_t)p.row_dest[(uint64_t)w.mt * 256u + in_tile] : (int64_t)w.mt * 256u + in_tile;
             if (!__all_sync(0xffffffffu, mbar_wait<true>(tmem_full_bar(buf), (seq >> 1) & 1u, 4, p.error_word, p.wait_us[4]))) break;
             tc_fence_after_sync();
-            const uint32_t row = mt * 256u + rank * 128u + quarter * 32u + lane;
-            const int64_t dest = row < p.m ? (int64_t)row : -1;
             // 64 columns at a time. Those shared with the other accumulator - the last of the first, the first of the second - come first.
             const uint32_t first = buf == 0 ? 64u : 0u;
             const bool shares = half == 1u - buf;
@@ -617,7 +686,7 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
                 tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[0]));
                 tmem_ld_wait_for(*reinterpret_cast<uint32_t(*)[32]>(&acc[32]));
                 if (shares && part == 0) arrive();
-                store_rows<kBf16, 64>(acc, p, dest, nt * 256u + half * 128u + in_half, staging, kPairStagingPitch, lane);
+                store_rows<kBf16, 64>(acc, p, dest, w.nt * 256u + half * 128u + in_half, staging, kPairStagingPitch, lane);
             }
         }
     }
@@ -671,7 +740,7 @@ cudaError_t launch_dependent(void (*kernel)(Args...), uint32_t grid, int threads
 }
 
 template <bool kBf16>
-cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t stream) {
+cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, uint64_t tiles, cudaStream_t stream) {
     auto kernel = gemm_mx_pair_kernel<kBf16>;
     static int max_pairs[64] = {0};
     int d = 0;
@@ -693,7 +762,7 @@ cudaError_t launch_pair(const PairMaps &maps, const MxGemmDev &dev, cudaStream_t
         if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) { cudaGetLastError(); n = sm_count() / 2; }
         max_pairs[d] = n;
     }
-    uint32_t pairs = dev.tiles_m * dev.tiles_n, most = (uint32_t)max_pairs[d];
+    uint32_t pairs = (uint32_t)(tiles < 0x7fffffffull ? tiles : 0x7fffffffull), most = (uint32_t)max_pairs[d];
     if (usable_sms() > 1 && (uint32_t)usable_sms() / 2 < most) most = (uint32_t)usable_sms() / 2;
     if (pairs > most) pairs = most;
     return launch_dependent(kernel, 2 * pairs, kThreads, kPairSmem, stream, maps, dev);
@@ -728,30 +797,33 @@ cudaError_t launch_by_width(int bn, bool bf16, const MxGemmDev &dev, uint64_t ma
 
 } // namespace
 
-bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t k) {
+bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t) {
     return ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 2;
 }
 
-bool gemm_mx_quantises(uint64_t m) { return m <= 16; }
-
-static bool use_pairs(const MxGemmArgs &args) { return args.tiles == nullptr && args.x == nullptr && gemm_mx_reads_rows(args.m, args.n, args.k); }
+// Every CTA quantises the rows again, and with more than two the loads of a chunk's rows no longer lie eight chunks ahead:
+// 8 x 8192 x 8192 took 22.8 us inside and 13.5 us after the separate kernel, 1 x 4096 x 4096 takes 9.4 us inside with one launch less.
+bool gemm_mx_quantises(uint64_t m) { return m <= 2; }
 
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     if (args.m == 0 || args.n == 0) return cudaSuccess;
     if (args.m > 0x7fffff00ull || args.n > 0x7fffff00ull || args.k > 0x7fffff00ull) return cudaErrorInvalidValue;
-    // Tensor maps address lines of 128 bytes with 31-bit coordinates.
-    const uint64_t most_chunks = 0x7fffff00ull / (kMxChunkBytes / 128);
-    if ((args.m / 128 + 2) * (args.k / 256 + 1) > most_chunks || (args.n / 128 + 2) * (args.k / 256 + 1) > most_chunks) return cudaErrorInvalidValue;
+    if (args.x && (!gemm_mx_quantises(args.m) || args.tiles)) return cudaErrorInvalidValue;
     MxGemmDev dev;
-    dev.a_chunks = static_cast<const uint8_t *>(args.a_chunks);
-    dev.b_chunks = static_cast<const uint8_t *>(args.b_chunks);
+    dev.kblocks = (uint32_t)((args.k + kMxChunkValues - 1) / kMxChunkValues);
+    dev.group_blocks = (uint32_t)((args.n + kChunkRows - 1) / kChunkRows);
+    const uint64_t a_blocks = args.tiles ? args.max_tiles * (args.tile_rows / kChunkRows) : (args.m + kBM - 1) / kBM;
+    const uint64_t a_chunks = a_blocks * dev.kblocks, b_chunks = args.groups * dev.group_blocks * dev.kblocks;
+    // Tensor maps address lines of 128 bytes with 31-bit coordinates; both kernels count chunks in 32 bits.
+    if (a_blocks > 0x00ffffffull || a_chunks > 0x7fffff00ull / 128 || b_chunks > 0x7fffff00ull / 128) return cudaErrorInvalidValue;
+    dev.a_codes = static_cast<const uint8_t *>(args.a_chunks);
+    dev.a_scales = dev.a_codes + (args.a_codes ? 0 : a_chunks * kMxCodeBytes);
+    dev.b_codes = static_cast<const uint8_t *>(args.b_chunks);
+    dev.b_scales = dev.b_codes + b_chunks * kMxCodeBytes;
     dev.c = static_cast<uint8_t *>(args.c);
     dev.c_stride = args.c_stride;
     dev.m = (uint32_t)args.m;
     dev.n = (uint32_t)args.n;
-    dev.kblocks = (uint32_t)((args.k + kMxChunkValues - 1) / kMxChunkValues);
-    dev.group_blocks = (uint32_t)((args.n + kChunkRows - 1) / kChunkRows);
-    dev.tiles_m = (uint32_t)((args.m + kBM - 1) / kBM);
     dev.tiles = args.tiles;
     dev.tile_count = args.tile_count;
     dev.row_dest = args.row_dest;
@@ -761,16 +833,13 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.k = (uint32_t)args.k;
     dev.error_word = args.error_word;
     wait_limits_us(dev.wait_us);
-    if (args.x && !gemm_mx_quantises(args.m)) return cudaErrorInvalidValue;
     dev.a_row_major = args.a_codes != nullptr;
-    dev.a_scales = dev.a_chunks + (args.a_codes ? 0u : kMxCodeBytes);
-    dev.a_scale_step = args.a_codes ? kMxScaleBytes : kMxChunkBytes;
-    if (use_pairs(args)) {
+    dev.a_blocks = (uint32_t)a_blocks;
+    if (args.tiles ? args.tile_rows == 256 : !args.x && gemm_mx_reads_rows(args.m, args.n, args.k)) {
         if (!get_encode_tiled()) return cudaErrorNotSupported;
         dev.tiles_m = (uint32_t)((args.m + 255) / 256);
         dev.tiles_n = (uint32_t)((args.n + 255) / 256);
         PairMaps maps;
-        const uint64_t a_chunks = (args.m + 127) / 128 * dev.kblocks, b_lines = (uint64_t)dev.group_blocks * dev.kblocks * kMxChunkLines;
         bool ok;
         if (args.a_codes) {
             cuuint64_t dims[2] = {(args.k + 1) / 2, args.m}, strides[1] = {args.a_codes_stride};
@@ -779,13 +848,15 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
         } else {
-            ok = line_map(maps.a, args.a_chunks, a_chunks * kMxChunkLines, 128);
+            ok = line_map(maps.a, dev.a_codes, a_chunks * kBM, kBM);
         }
-        ok = ok && line_map(maps.b, args.b_chunks, b_lines, 128);
+        ok = ok && line_map(maps.b, dev.b_codes, b_chunks * kBM, kBM);
         if (!ok) return cudaErrorInvalidValue;
-        return args.c_bf16 ? launch_pair<true>(maps, dev, stream) : launch_pair<false>(maps, dev, stream);
+        const uint64_t tiles = (args.tiles ? args.max_tiles : dev.tiles_m) * (uint64_t)dev.tiles_n;
+        return args.c_bf16 ? launch_pair<true>(maps, dev, tiles, stream) : launch_pair<false>(maps, dev, tiles, stream);
     }
     if (args.a_codes) return cudaErrorInvalidValue;
+    dev.tiles_m = (uint32_t)((args.m + kBM - 1) / kBM);
     // Narrower tiles while the wide ones are fewer than the SMs: a product with few rows is bound by the packed matrix's bytes, and every SM
     // that streams some of it counts. Sums run over the depth in the same order whatever the tile.
     const uint64_t row_tiles = args.tiles ? args.max_tiles : dev.tiles_m;

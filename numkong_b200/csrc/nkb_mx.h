@@ -5,11 +5,11 @@
 // consecutive values of a row share; s = 255 is NaN. Row-major form, as callers hold it: two codes per byte, the even value in
 // the low half, ceil(depth / 2) bytes of codes and ceil(depth / 32) scale bytes per row.
 //
-// Tile form: a chunk is 128 rows x 256 values. Its first 16 KiB are the codes, 128 bytes per row, in the 128-byte-swizzled
-// K-major image tcgen05.mma reads (as in PackedHeader); then two 512-byte scale tiles, one per 128 values of depth, each the
-// image the MMA's scales take in TMEM: the four scales of row r at byte (r % 32) * 16 + (r / 32) * 4 (lane r % 32, column r / 32). One bulk copy brings a
-// chunk to shared memory with nothing left to rearrange. Chunks are ordered [row block][depth block], so that a CTA that
-// stays on one row block reads one contiguous stream.
+// Tile form: a chunk is 128 rows x 256 values. Its codes are 16 KiB, 128 bytes per row, in the 128-byte-swizzled K-major image
+// tcgen05.mma reads (as in PackedHeader); its scales are two 512-byte tiles, one per 128 values of depth, each the image the MMA's
+// scales take in TMEM: the four scales of row r at byte (r % 32) * 16 + (r / 32) * 4 (lane r % 32, column r / 32). All chunks' codes
+// come first, then all chunks' scales, both ordered [row block][depth block], so that a CTA that stays on one row block reads two
+// contiguous streams with nothing left to rearrange.
 #pragma once
 #include "nkb_internal.h"
 
@@ -43,7 +43,7 @@ cudaError_t launch_mx_quantise(uint32_t type, const void *x, uint64_t rows, uint
 // float rows -> tile form. Tiled row i is row i of x, or, with `row_dest`, row row_dest[i] / divide of x; entries below 0 leave
 // their row as it is.
 cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t depth, uint64_t x_stride, uint64_t tiled_rows,
-                                     const int32_t *row_dest, const int32_t *tile_count, uint32_t divide, void *chunks, cudaStream_t stream);
+                                     const int32_t *row_dest, const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, void *chunks, cudaStream_t stream);
 cudaError_t launch_mx_dequantise(uint32_t type, const void *codes, uint64_t codes_stride, const void *scales, uint64_t scales_stride,
                                  uint64_t rows, uint64_t depth, void *x, uint64_t x_stride, cudaStream_t stream);
 // Row-major codes and scales -> tile form; `pad_rows`: rows behind the last one of every group are written too (zero codes, scale 1).
@@ -53,10 +53,10 @@ cudaError_t launch_mx_tile(const void *codes, uint64_t codes_stride, const void 
 // Row-major scales -> scale tiles alone, 1024 bytes per 128 rows x 256 values.
 cudaError_t launch_mx_tile_scales(const void *scales, uint64_t scales_stride, uint64_t rows, uint64_t depth, void *tiles, cudaStream_t stream);
 
-// One row tile (128 rows of A in tile form) of a grouped product.
+// One row tile (128 or 256 rows of A in tile form, see MxGemmArgs::tile_rows) of a grouped product.
 struct MxRowTile {
     int32_t group;  // packed matrix its rows multiply
-    int32_t rows;   // valid rows, 1 .. 128
+    int32_t rows;   // valid rows, 1 .. 128 (256)
 };
 struct MxGemmArgs {
     const void *a_chunks;              // A in tile form; with `a_codes` set, its scale tiles alone
@@ -74,6 +74,8 @@ struct MxGemmArgs {
     const int32_t *tile_count = nullptr;
     const int32_t *row_dest = nullptr;
     uint64_t max_tiles = 0;            // row tiles there may be at most
+    uint32_t tile_rows = 128;          // 256: CTA pairs
+    uint64_t groups = 1;
     unsigned int *error_word = nullptr;
 };
 // Whether a product of this size reads A's codes from the caller's rows when they are aligned.
@@ -96,9 +98,9 @@ constexpr uint32_t kRouteMaxExperts = 1024, kRouteMaxTop = 32, kRouteMaxGroups =
 cudaError_t launch_route(const RouteArgs &args, float *weights, int32_t *ids, cudaStream_t stream);
 cudaError_t launch_route_gradient(const RouteArgs &args, const float *weights_grad, const int32_t *ids, float *logits_grad, cudaStream_t stream);
 
-// Row tiles of at most 128 slots of one expert each. `slots` ids; those outside [0, experts) choose none.
+// Row tiles of at most `tile_rows` slots of one expert each. `slots` ids; those outside [0, experts) choose none.
 cudaError_t launch_expert_order(const int32_t *ids, uint64_t slots, uint32_t experts, MxRowTile *tiles, int32_t *tile_count, int32_t *row_dest,
-                                uint64_t max_tiles, cudaStream_t stream);
+                                uint64_t max_tiles, uint32_t tile_rows, cudaStream_t stream);
 // Zeros the rows of `out` whose slot chooses no expert.
 cudaError_t launch_zero_unrouted(const int32_t *ids, uint64_t slots, uint32_t experts, void *out, uint64_t row_bytes, uint64_t out_stride, cudaStream_t stream);
 // out[t] = sum over j of weights[t, j] * y[t * top + j], slots without an expert left out; f32 sums in order of j.

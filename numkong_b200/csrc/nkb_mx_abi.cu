@@ -123,16 +123,19 @@ uint8_t *workspace_or_scratch(Operands &ops, void *workspace, uint64_t bytes) {
 }
 
 struct ExpertsLayout {
+    uint32_t tile_rows;
     uint64_t max_tiles, tiles, count, dest, chunks, sums, total;
 };
 ExpertsLayout experts_layout(uint64_t slots, uint64_t experts, uint64_t width, uint64_t depth, bool weighted) {
     ExpertsLayout l;
-    l.max_tiles = slots / kChunkRows + (slots < experts ? slots : experts);
+    // CTA pairs on 256 rows fetch less per product but leave more of a tile empty at each expert's end: from 192 rows an expert on.
+    l.tile_rows = slots >= 192 * experts ? 256 : 128;
+    l.max_tiles = slots / l.tile_rows + (slots < experts ? slots : experts);
     l.tiles = 0;
     l.count = round_up(l.max_tiles * sizeof(MxRowTile), 256);
     l.dest = l.count + 256;
-    l.chunks = round_up(l.dest + l.max_tiles * kChunkRows * 4, 256);
-    l.sums = round_up(l.chunks + chunk_bytes(l.max_tiles * kChunkRows, depth), 256);
+    l.chunks = round_up(l.dest + l.max_tiles * l.tile_rows * 4, 256);
+    l.sums = round_up(l.chunks + chunk_bytes(l.max_tiles * l.tile_rows, depth), 256);
     l.total = l.sums + (weighted ? slots * width * 4 : 0);
     return l;
 }
@@ -180,7 +183,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
         } else if (ok) {
             ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
             ok = ad != nullptr;
-            if (ok && !inside) ok = cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 1, chunks, stream), "quantise kernel");
+            if (ok && !inside) ok = cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 0, 1, chunks, stream), "quantise kernel");
         }
         if (ok) {
             MxGemmArgs args;
@@ -408,9 +411,9 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
             args.c = weights ? static_cast<void *>(sums) : dst; args.c_stride = weights ? width * 4 : out_stride;
             args.c_bf16 = !weights && out_type == kBF16;
             args.m = slots; args.n = width; args.k = depth;
-            args.tiles = tiles; args.tile_count = count; args.row_dest = dest; args.max_tiles = l.max_tiles; args.error_word = err;
-            ok = cuda_ok(launch_expert_order(id, slots, (uint32_t)experts, tiles, count, dest, l.max_tiles, stream), "expert order kernel") &&
-                 cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, x_rows > 1 ? x_stride : 0, l.max_tiles * kChunkRows, dest, count, per_slot ? 1u : (uint32_t)top, ws + l.chunks, stream), "quantise kernel") &&
+            args.tiles = tiles; args.tile_count = count; args.row_dest = dest; args.max_tiles = l.max_tiles; args.tile_rows = l.tile_rows; args.groups = experts; args.error_word = err;
+            ok = cuda_ok(launch_expert_order(id, slots, (uint32_t)experts, tiles, count, dest, l.max_tiles, l.tile_rows, stream), "expert order kernel") &&
+                 cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, x_rows > 1 ? x_stride : 0, l.max_tiles * l.tile_rows, dest, count, l.tile_rows, per_slot ? 1u : (uint32_t)top, ws + l.chunks, stream), "quantise kernel") &&
                  cuda_ok(launch_gemm_mx(args, stream), "grouped mxfp4 GEMM kernel");
             if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, (uint32_t)experts, width, dst, out_type == kBF16, out_stride, stream), "combine kernel");
             else if (ok) ok = cuda_ok(launch_zero_unrouted(id, slots, (uint32_t)experts, dst, row_bytes, out_stride, stream), "zero kernel");

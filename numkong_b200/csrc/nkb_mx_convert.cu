@@ -68,7 +68,7 @@ template <bool kTiled>
 __device__ __forceinline__ void store_chunk_row(uint32_t codes, uint32_t row, uint32_t kb, uint64_t depth, const RowMajorSink &out, uint8_t *chunks,
                                                 uint32_t depth_blocks, int lane) {
     if constexpr (kTiled) {
-        uint8_t *chunk = chunks + ((uint64_t)(row / kChunkRows) * depth_blocks + kb) * kMxChunkBytes;
+        uint8_t *chunk = chunks + ((uint64_t)(row / kChunkRows) * depth_blocks + kb) * kMxCodeBytes;
         const uint32_t r = row % kChunkRows;
         *reinterpret_cast<uint32_t *>(chunk + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = codes;
     } else {
@@ -83,10 +83,10 @@ __device__ __forceinline__ void store_chunk_row(uint32_t codes, uint32_t row, ui
 // 8192 x 8192 bf16: 170 MB in 30 us where the copy rate allows 26; with one piece in flight 50 us.
 template <uint32_t kType, bool kTiled>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, uint32_t rows, uint64_t depth, uint64_t x_stride, RowMajorSink out,
-                                                            uint8_t *chunks, uint32_t depth_blocks, const int32_t *row_dest, const int32_t *tile_count,
-                                                            uint32_t divide) {
+                                                            uint8_t *chunks, uint8_t *scale_tiles, uint32_t depth_blocks, const int32_t *row_dest,
+                                                            const int32_t *tile_count, uint32_t tile_rows, uint32_t divide) {
     if constexpr (kTiled) allow_next_kernel();  // the product that reads the chunks may set itself up meanwhile
-    if (kTiled && row_dest) rows = (uint32_t)*tile_count * kChunkRows;
+    if (kTiled && row_dest) rows = (uint32_t)*tile_count * tile_rows;
     constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
             word |= __shfl_xor_sync(0xffffffffu, word, 2);
             const uint32_t u = (uint32_t)lane >> 3, r = piece.row % kChunkRows;
             if ((lane & 3) == 0 && u < count)
-                *reinterpret_cast<uint32_t *>(chunks + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0 + u) * kMxChunkBytes + kMxCodeBytes +
+                *reinterpret_cast<uint32_t *>(scale_tiles + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0 + u) * kMxScaleBytes +
                                               ((lane >> 2) & 1) * 512 + (r & 31u) * 16 + (r >> 5) * 4) = word;
         } else {
             const uint64_t block = (uint64_t)piece.kb0 * 8 + lane;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
 // an odd depth count, as for the other 4-bit types; what lies past the depth is zero codes under scale 1.
 __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
                                                         uint64_t width, uint64_t depth, uint64_t tiled_rows, uint32_t group_rows, uint8_t *chunks,
-                                                        uint32_t depth_blocks) {
+                                                        uint8_t *scale_tiles, uint32_t depth_blocks) {
     allow_next_kernel();
     const int lane = threadIdx.x & 31;
     const uint64_t row_bytes = (depth + 1) / 2, row_scales = (depth + kMxBlock - 1) / kMxBlock;
@@ -290,13 +290,14 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, ui
                 for (int i = 0; i < 4; ++i)
                     if (byte + i < row_bytes) w |= (uint32_t)c[i] << (8 * i);
         }
-        uint8_t *chunk = chunks + ((row / kChunkRows) * depth_blocks + kb) * kMxChunkBytes;
+        const uint64_t at = (row / kChunkRows) * depth_blocks + kb;
+        uint8_t *chunk = chunks + at * kMxCodeBytes;
         const uint32_t r = (uint32_t)(row % kChunkRows);
         *reinterpret_cast<uint32_t *>(chunk + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = w;
         if (lane < 8) {
             const uint64_t block = (uint64_t)kb * 8u + lane;
             const uint8_t s = real && block < row_scales ? scales[from * scales_stride + block] : (uint8_t)127;
-            chunk[kMxCodeBytes + (lane >> 2) * 512 + (r & 31u) * 16 + (r >> 5) * 4 + (lane & 3)] = s;
+            scale_tiles[at * kMxScaleBytes + (lane >> 2) * 512 + (r & 31u) * 16 + (r >> 5) * 4 + (lane & 3)] = s;
         }
     }
 }
@@ -346,26 +347,26 @@ cudaError_t launch_mx_quantise(uint32_t type, const void *x, uint64_t rows, uint
     const uint32_t grid = grid_for(rows * pieces(kblocks)), n = (uint32_t)rows;
     const uint8_t *src = static_cast<const uint8_t *>(x);
     switch (type) {
-    case kF32: quantise_kernel<kF32, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, kblocks, nullptr, nullptr, 1); break;
-    case kBF16: quantise_kernel<kBF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, kblocks, nullptr, nullptr, 1); break;
-    case kF16: quantise_kernel<kF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, kblocks, nullptr, nullptr, 1); break;
+    case kF32: quantise_kernel<kF32, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
+    case kBF16: quantise_kernel<kBF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
+    case kF16: quantise_kernel<kF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
 }
 
 cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t depth, uint64_t x_stride, uint64_t tiled_rows,
-                                     const int32_t *row_dest, const int32_t *tile_count, uint32_t divide, void *chunks, cudaStream_t stream) {
+                                     const int32_t *row_dest, const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, void *chunks, cudaStream_t stream) {
     const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues);
     const RowMajorSink none{nullptr, nullptr, 0, 0};
     if (tiled_rows * pieces(kblocks) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
     const uint32_t grid = grid_for(tiled_rows * pieces(kblocks)), n = (uint32_t)tiled_rows;
     const uint8_t *src = static_cast<const uint8_t *>(x);
-    uint8_t *dst = static_cast<uint8_t *>(chunks);
+    uint8_t *dst = static_cast<uint8_t *>(chunks), *tiles = dst + (tiled_rows + kChunkRows - 1) / kChunkRows * kblocks * kMxCodeBytes;
     switch (type) {
-    case kF32: quantise_kernel<kF32, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, kblocks, row_dest, tile_count, divide); break;
-    case kBF16: quantise_kernel<kBF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, kblocks, row_dest, tile_count, divide); break;
-    case kF16: quantise_kernel<kF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, kblocks, row_dest, tile_count, divide); break;
+    case kF32: quantise_kernel<kF32, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
+    case kBF16: quantise_kernel<kBF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
+    case kF16: quantise_kernel<kF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
@@ -403,7 +404,8 @@ cudaError_t launch_mx_tile(const void *codes, uint64_t codes_stride, const void 
     const uint64_t rows = pad_rows ? groups * group_rows : (groups - 1) * group_rows + width;
     tile_kernel<<<grid_for(rows * kblocks), kThreads, 0, stream>>>(static_cast<const uint8_t *>(codes), codes_stride, static_cast<const uint8_t *>(scales),
                                                                    scales_stride, width, depth, rows, (uint32_t)group_rows,
-                                                                   static_cast<uint8_t *>(chunks), kblocks);
+                                                                   static_cast<uint8_t *>(chunks),
+                                                                   static_cast<uint8_t *>(chunks) + groups * group_rows / kChunkRows * kblocks * kMxCodeBytes, kblocks);
     return cudaGetLastError();
 }
 

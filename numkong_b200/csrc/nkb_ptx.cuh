@@ -275,6 +275,14 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint
     else NKB_UMMA_MX_ASM("2");
 #undef NKB_UMMA_MX_ASM
 }
+// True in one lane of a converged warp. Code that the whole warp walks and one lane issues from keeps its addresses and descriptors
+// in uniform registers, where tcgen05.mma wants them; from inside `if (lane == 0)` every MMA first moves them there (58 cycles each).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
