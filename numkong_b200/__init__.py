@@ -50,11 +50,27 @@ def _integer_cells(dtype: str, op: str) -> bool:
     return (op == "dots" and dtype in ("i8", "u8", "i4", "u4", "u1")) or op == "hammings"
 
 
+_tensor: Any = None  # torch.Tensor once a tensor has been met
+
+
 def _is_torch(x: Any) -> bool:
-    return type(x).__module__.startswith("torch")
+    global _tensor
+    kind = type(x)
+    if kind is _tensor:
+        return True
+    if not kind.__module__.startswith("torch"):
+        return False
+    if _tensor is None and kind.__name__ == "Tensor":
+        _tensor = kind
+    return True
 
 
 _torch_names_of: dict = {}  # torch dtype -> its name, filled as types are met: spelling a dtype out costs a microsecond
+
+
+def _torch_type(dtype: Any) -> Optional[str]:
+    """This library's name of a torch dtype."""
+    return _TORCH_NAMES.get("torch." + _torch_name(dtype))
 
 
 def _torch_name(dtype: Any) -> str:
@@ -111,29 +127,32 @@ class _View:
         # Device arrays of other libraries (CuPy, Numba, ...) come in without a copy: through DLPack when the object
         # offers it for a CUDA device, else through __cuda_array_interface__. The reference's binding rejects CUDA
         # capsules (python/dlpack_interop.c:97-99); here they are the fast path.
-        if not _is_torch(x) and not isinstance(x, np.ndarray):
+        torch_like = _is_torch(x)
+        if not torch_like and not isinstance(x, np.ndarray):
             x = _adopt_device_array(x)
+            torch_like = _is_torch(x)
         self.obj = x
-        if isinstance(x, _ForeignCuda):
+        if not torch_like and isinstance(x, _ForeignCuda):
             name = dtype or x.name
             if name is None:
                 raise TypeError("pass dtype='bf16' etc. for storage words that have no element type of their own")
             self.is_cuda, self.ptr, self.rows, self.cols = True, x.ptr, x.rows, x.cols
             self.stride = x.stride if x.rows > 1 else x.cols * x.itemsize
             item = x.itemsize
-        elif _is_torch(x):
+        elif torch_like:
             if x.dim() != 2:
                 raise ValueError("expected a 2-D matrix")
-            if x.stride(1) != 1 and x.shape[1] > 1:
+            self.rows, self.cols = x.shape
+            row_step, step = x.stride()
+            if step != 1 and self.cols > 1:
                 raise ValueError("rows must be contiguous (column-major inputs are not supported)")
-            name = dtype or _TORCH_NAMES.get("torch." + _torch_name(x.dtype))
+            name = dtype or _torch_type(x.dtype)
             if name is None:
                 raise TypeError(f"unsupported torch dtype {x.dtype}")
             self.is_cuda = x.is_cuda
             self.ptr = x.data_ptr()
-            self.rows, self.cols = x.shape
             item = x.element_size()
-            self.stride = x.stride(0) * item if self.rows > 1 else self.cols * item
+            self.stride = row_step * item if self.rows > 1 else self.cols * item
         else:
             x = np.asarray(x)
             self.obj = x
@@ -652,7 +671,7 @@ def _cuda(x: Any) -> bool:
 def _enqueue(x: Any, call: Any, *arguments: Any) -> None:
     """Makes a library call that works on `x`: with the GPU of a CUDA tensor current, and for a thread that has not chosen a
     stream with set_stream on torch's current one, where the tensors come from and the results go."""
-    if not _cuda(x):
+    if not _is_torch(x) or not x.is_cuda:
         call(*arguments)
         return
     t = _torch if _torch.ready else _torch.load()
@@ -730,11 +749,12 @@ class MxMatrix:
         self._parts = c.ptr, c.stride, s.ptr, s.stride
 
     @classmethod
-    def _of(cls, codes: Any, scales: Any, depth: int) -> "MxMatrix":
-        """Of two dense arrays of the right shapes."""
+    def _new(cls, like: Any, rows: int, depth: int) -> "MxMatrix":
+        """Of uninitialised dense arrays where `like` lives."""
         self = cls.__new__(cls)
-        self.codes, self.scales, self.rows, self.depth = codes, scales, codes.shape[0], depth
-        self._parts = _ptr(codes), codes.shape[1], _ptr(scales), scales.shape[1]
+        width, blocks = (depth + 1) // 2, (depth + 31) // 32
+        self.codes, self.scales, self.rows, self.depth = _like(like, (rows, width), "u8"), _like(like, (rows, blocks), "u8"), rows, depth
+        self._parts = _ptr(self.codes), width, _ptr(self.scales), blocks
         return self
 
     @property
@@ -750,7 +770,7 @@ def mx_quantise(x: Any, *, dtype: Optional[str] = None) -> MxMatrix:
     2^(floor(log2(largest)) - 2), each value to the nearest code, ties to the even code, beyond 6 scales to 6. A block that
     holds an infinity or a NaN becomes NaN."""
     v = _float_view(x, dtype, "mx_quantise")
-    q = MxMatrix._of(_like(v.obj, (v.rows, (v.cols + 1) // 2), "u8"), _like(v.obj, (v.rows, (v.cols + 31) // 32), "u8"), v.cols)
+    q = MxMatrix._new(v.obj, v.rows, v.cols)
     _enqueue(v.obj, lib.nkb_mx_quantise, v.ptr, DTYPE_CODES[v.dtype], v.rows, v.cols, v.stride, *q._parts)
     check("mx_quantise")
     return q

@@ -26,6 +26,7 @@ struct RouteDev {
     const uint8_t *logits;
     uint64_t stride;
     uint32_t tokens, experts, groups, top_groups, top;
+    uint32_t width;                // lanes for one token's slots: 8, 16 or 32
     float scale;
     const float *bias;
     bool sigmoid, renormalise;
@@ -212,14 +213,18 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
     const uint32_t slack = (uint32_t)(((p.sigmoid ? 8.0f : (float)(kPer + 16)) + fabsf(least) + fabsf(most)) * 0x1p-23f * per_key) + 8u;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) bias[i] = (bias[i] - least) * per_key;  // -infinity stays
-    float logit[kPer];
-    uint32_t token = blockIdx.x * kWarps + warp;
-    if (token < p.tokens) load_logits<kType, kPer>(p.logits + token * p.stride, p.experts, lane, logit);
-    for (; token < p.tokens;) {
-        const uint8_t *row = p.logits + token * p.stride;
-        const uint32_t following = token + gridDim.x * kWarps;
-        float next[kPer];
-        if (following < p.tokens) load_logits<kType, kPer>(p.logits + following * p.stride, p.experts, lane, next);
+    // A warp chooses for `batch` tokens one after the other and then works out their weights together, `width` lanes each.
+    const uint32_t width = p.width, batch = 32 / width, place = lane / width, slot = lane % width;
+    const uint32_t step = gridDim.x * kWarps * batch;
+    for (uint32_t first = (blockIdx.x * kWarps + warp) * batch; first < p.tokens; first += step) {
+    int32_t chosen_all = -1;         // lane place * width + j: slot j of token first + place
+    float top_all = 0.0f;            // that token's largest logit, and the sum of its exponentials: the softmax without renormalisation
+    double total_all = 1.0;
+    float logit[kPer], next[kPer];
+    load_logits<kType, kPer>(p.logits + first * p.stride, p.experts, lane, logit);
+    for (uint32_t t = 0; t < batch && first + t < p.tokens; ++t) {
+        const uint8_t *row = p.logits + (first + t) * p.stride;
+        if (t + 1 < batch && first + t + 1 < p.tokens) load_logits<kType, kPer>(row + p.stride, p.experts, lane, next);
         float top_logit = -INFINITY;
         if (!p.sigmoid) {
 #pragma unroll
@@ -341,87 +346,99 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             chosen = choose_exactly<kType>(p, row, top_logit, keys_all + (size_t)warp * p.experts, lane);
             __syncwarp();
         }
-        const float l = chosen >= 0 ? load_logit<kType>(row, chosen) : -INFINITY;
-        const bool near_zero = p.sigmoid && __any_sync(0xffffffffu, chosen >= 0 && l < -80.0f);
-        double w = 0.0;
-        if (p.renormalise) {
-            // Scores as they are while they can be represented, ratios from differences of logarithms where they vanish.
-            const float largest = p.sigmoid && !near_zero ? 0.0f : warp_max(l);
-            if (chosen >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
-            const double sum = warp_sum(w);
-            if (chosen >= 0) w *= sum > 1e-30 ? reciprocal(sum) : 1.0 / sum;
-        } else if (p.sigmoid) {
-            if (chosen >= 0) w = near_zero ? sigmoid64(l) : fast_score(true, l, 0.0f);
-        } else {
+        const int32_t mine_of = __shfl_sync(0xffffffffu, chosen, slot);
+        if (place == t) chosen_all = mine_of;
+        if (!p.sigmoid && !p.renormalise) {
             double total = 0.0;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 if (logit[i] > -INFINITY) total += (double)exp_difference(logit[i], top_logit);
             total = warp_sum(total);
-            if (chosen >= 0) w = (double)exp_difference(l, top_logit) * reciprocal(total);
+            if (place == t) { top_all = top_logit; total_all = total; }
         }
-        if ((uint32_t)lane < p.top) {
-            weights[(uint64_t)token * p.top + lane] = (float)(w * p.scale);
-            ids[(uint64_t)token * p.top + lane] = chosen;
-        }
-        token = following;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) logit[i] = next[i];
     }
+    const uint64_t token = first + place;
+    const float l = chosen_all >= 0 ? load_logit<kType>(p.logits + token * p.stride, chosen_all) : -INFINITY;
+    const bool near_zero = p.sigmoid && __any_sync(0xffffffffu, chosen_all >= 0 && l < -80.0f);
+    double w = 0.0;
+    if (p.renormalise) {
+        // Scores as they are while they can be represented, ratios from differences of logarithms where they vanish.
+        float largest = l;
+        if (!p.sigmoid || near_zero)
+            for (uint32_t o = 1; o < width; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        if (chosen_all >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
+        double sum = w;
+        for (uint32_t o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (chosen_all >= 0) w *= sum > 1e-30 ? reciprocal(sum) : 1.0 / sum;
+    } else if (p.sigmoid) {
+        if (chosen_all >= 0) w = near_zero ? sigmoid64(l) : fast_score(true, l, 0.0f);
+    } else if (chosen_all >= 0) {
+        w = (double)exp_difference(l, top_all) * reciprocal(total_all);
+    }
+    if (slot < p.top && token < p.tokens) {
+        weights[token * p.top + slot] = (float)(w * p.scale);
+        ids[token * p.top + slot] = chosen_all;
+    }
+    }
 }
 
-// One warp per token. What reaches a logit through the token's own slots is worked out in 64 bits, one slot per lane, and put into a
-// row in shared memory; the row then goes out in whole lines. Only the softmax without renormalisation gives every logit something.
+// One warp per batch of one, two or four tokens, `width` lanes for the slots of each. What reaches a logit through the token's own slots
+// is worked out in 64 bits, one slot per lane, and put into a row in shared memory; the rows then go out in whole lines. Only the softmax
+// without renormalisation gives every logit something.
 template <uint32_t kType>
 __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const RouteDev p, const float *weights_grad, const int32_t *ids, float *logits_grad) {
     extern __shared__ float rows_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t padded = (p.experts + 3) / 4 * 4;
-    float *line = rows_all + (size_t)warp * padded;
+    const uint32_t width = p.width, batch = 32 / width, place = lane / width, slot = lane % width;
+    float *lines = rows_all + (size_t)warp * batch * padded, *line = lines + place * padded;
     const bool dense = !p.sigmoid && !p.renormalise;
-    const uint32_t step = gridDim.x * kWarps;
-    // The slots of the token after this one are on their way while this one is worked on, and so are the logits they name.
-    struct Slot { int32_t id; float grad, logit; };
-    auto load_slot = [&](uint32_t token, Slot &s) {
-        s = {-1, 0.0f, -INFINITY};
-        if (token < p.tokens && (uint32_t)lane < p.top) {
-            s.id = ids[(uint64_t)token * p.top + lane];
-            s.grad = weights_grad[(uint64_t)token * p.top + lane];
+    auto over_slots = [&](double v) {
+        for (uint32_t o = 1; o < width; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    for (uint32_t first = (blockIdx.x * kWarps + warp) * batch; first < p.tokens; first += gridDim.x * kWarps * batch) {
+        const uint64_t token = first + place;
+        const uint32_t here = min(batch, p.tokens - first);
+        int32_t id = -1;
+        float l = -INFINITY, incoming = 0.0f;
+        if (slot < p.top && token < p.tokens) {
+            id = ids[token * p.top + slot];
+            incoming = weights_grad[token * p.top + slot];
+            if (id >= 0 && id < (int32_t)p.experts) l = load_logit<kType>(p.logits + token * p.stride, id);
         }
-    };
-    auto load_named = [&](uint32_t token, Slot &s) {
-        if (s.id >= 0 && s.id < (int32_t)p.experts) s.logit = load_logit<kType>(p.logits + token * p.stride, s.id);
-    };
-    Slot slot, ahead;
-    load_slot(blockIdx.x * kWarps + warp, slot);
-    load_named(blockIdx.x * kWarps + warp, slot);
-    for (uint32_t token = blockIdx.x * kWarps + warp; token < p.tokens; token += step) {
-        const uint8_t *row = p.logits + token * p.stride;
-        load_slot(token + step, ahead);
-        const float l = slot.logit;
-        const int32_t id = l > -INFINITY ? slot.id : -1;  // a masked expert has score 0 whatever its logit: no gradient
-        const double g = id >= 0 ? (double)slot.grad * p.scale : 0.0;
+        if (!(l > -INFINITY)) id = -1;  // a masked expert has score 0 whatever its logit: no gradient
+        const double g = id >= 0 ? (double)incoming * p.scale : 0.0;
         float top_logit = -INFINITY;
         double total = 0.0;
         if (dense) {
-            for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
-            top_logit = warp_max(top_logit);
-            for (uint32_t e = lane; e < p.experts; e += 32) {
-                const float v = load_logit<kType>(row, e), part = v > -INFINITY ? exp_difference(v, top_logit) : 0.0f;
-                line[e] = part;
-                total += (double)part;
+            for (uint32_t t = 0; t < here; ++t) {
+                const uint8_t *row = p.logits + (first + t) * p.stride;
+                float largest = -INFINITY;
+                double sum = 0.0;
+                for (uint32_t e = lane; e < p.experts; e += 32) largest = fmaxf(largest, load_logit<kType>(row, e));
+                largest = warp_max(largest);
+                for (uint32_t e = lane; e < p.experts; e += 32) {
+                    const float v = load_logit<kType>(row, e), part = v > -INFINITY ? exp_difference(v, largest) : 0.0f;
+                    lines[t * padded + e] = part;
+                    sum += (double)part;
+                }
+                sum = warp_sum(sum);
+                if (place == t) { top_logit = largest; total = sum; }
             }
-            total = warp_sum(total);
         } else {
-            for (uint32_t i = lane; i < padded / 4; i += 32) reinterpret_cast<float4 *>(line)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t i = lane; i < here * padded / 4; i += 32) reinterpret_cast<float4 *>(lines)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         double d = 0.0;  // what this slot's logit gets through the slot itself
         const bool near_limit = p.sigmoid && __any_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f);
         if (p.renormalise) {
-            const float most = warp_max(l);
+            float most = l;
+            for (uint32_t o = 1; o < width; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             double part = 0.0;
             if (id >= 0) part = !near_limit ? fast_score(p.sigmoid, l, most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
-            const double sum = warp_sum(part), u = id >= 0 ? part * (sum > 1e-30 ? reciprocal(sum) : 1.0 / sum) : 0.0, mean = warp_sum(g * u);
+            const double sum = over_slots(part), u = id >= 0 ? part * (sum > 1e-30 ? reciprocal(sum) : 1.0 / sum) : 0.0, mean = over_slots(g * u);
             d = u * (g - mean);
         } else if (id >= 0) {
             d = p.sigmoid ? g * (near_limit ? sigmoid64(l) : fast_score(true, l, 0.0f)) : g * ((double)exp_difference(l, top_logit) * reciprocal(total));
@@ -429,47 +446,54 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
         if (p.sigmoid && id >= 0) d *= near_limit ? sigmoid64(-(double)l) : fast_score(true, -l, 0.0f);  // 1 - s
         __syncwarp();
         if (dense) {
-            const double spread = warp_sum(d);
+            const double spread = over_slots(d);
             const float per_part = total > 0.0 ? (float)(-spread * reciprocal(total)) : 0.0f;
-            for (uint32_t e = lane; e < p.experts; e += 32) line[e] *= per_part;
+            for (uint32_t t = 0; t < here; ++t) {
+                const float factor = __shfl_sync(0xffffffffu, per_part, t * width);
+                for (uint32_t e = lane; e < p.experts; e += 32) lines[t * padded + e] *= factor;
+            }
             __syncwarp();
         }
         // An expert named twice gets its slots' sum in their order, from the first of them.
-        const uint32_t same = __match_any_sync(0xffffffffu, id);
+        const uint32_t segment = (width == 32 ? 0xffffffffu : (1u << width) - 1u) << (place * width);
+        const uint32_t same = __match_any_sync(0xffffffffu, id) & segment;
         if (__any_sync(0xffffffffu, id >= 0 && __popc(same) > 1)) {
             double sum = 0.0;
-            for (uint32_t j = 0; j < p.top; ++j) {
-                const double other = __shfl_sync(0xffffffffu, d, j);
-                if ((same >> j) & 1u) sum += other;
+            for (uint32_t j = 0; j < width; ++j) {
+                const double other = __shfl_sync(0xffffffffu, d, place * width + j);
+                if ((same >> (place * width + j)) & 1u) sum += other;
             }
             d = sum;
         }
         if (id >= 0 && __ffs(same) - 1 == lane) line[id] += (float)d;
-        load_named(token + step, ahead);
-        slot = ahead;
         __syncwarp();
-        float *out = logits_grad + (uint64_t)token * p.experts;
-        if ((p.experts & 3u) == 0 && (reinterpret_cast<uintptr_t>(logits_grad) & 15u) == 0)
-            for (uint32_t i = lane; i < p.experts / 4; i += 32) __stcs(reinterpret_cast<float4 *>(out) + i, reinterpret_cast<const float4 *>(line)[i]);
+        float *out = logits_grad + (uint64_t)first * p.experts;
+        if ((p.experts & 3u) == 0 && (reinterpret_cast<uintptr_t>(logits_grad) & 15u) == 0)  // the rows lie one behind the other here and there
+            for (uint32_t i = lane; i < here * (p.experts / 4); i += 32) __stcs(reinterpret_cast<float4 *>(out) + i, reinterpret_cast<const float4 *>(lines)[i]);
         else
-            for (uint32_t e = lane; e < p.experts; e += 32) out[e] = line[e];
+            for (uint32_t t = 0; t < here; ++t)
+                for (uint32_t e = lane; e < p.experts; e += 32) out[(uint64_t)t * p.experts + e] = lines[t * padded + e];
         __syncwarp();
     }
 }
 
-// Two blocks' worth of tokens in turn per resident block at least, so that the last wave is short.
-uint32_t route_grid(uint64_t tokens) {
-    const uint64_t blocks = (tokens + kWarps - 1) / kWarps;
+uint32_t route_grid(const RouteDev &p) {
+    const uint64_t tokens = (uint64_t)kWarps * (32 / p.width), blocks = (p.tokens + tokens - 1) / tokens;
     return (uint32_t)(blocks < 148ull * 16 ? blocks : 148ull * 16);
 }
 
 RouteDev route_dev(const RouteArgs &a) {
-    return RouteDev{static_cast<const uint8_t *>(a.logits), a.logits_stride, (uint32_t)a.tokens, a.experts, a.groups, a.top_groups, a.top, a.scale, a.bias, a.sigmoid, a.renormalise};
+    // Several tokens share a warp's 64-bit work where there are enough of them to fill the GPU all the same, and their rows of the
+    // gradient 48 KiB.
+    uint32_t width = a.tokens < 4096 || a.top > 16 ? 32 : a.top <= 8 ? 8 : 16;
+    if (width == 8 && a.experts > 768) width = 16;
+    return RouteDev{static_cast<const uint8_t *>(a.logits), a.logits_stride, (uint32_t)a.tokens, a.experts, a.groups, a.top_groups, a.top, width, a.scale, a.bias,
+                    a.sigmoid, a.renormalise};
 }
 
 template <uint32_t kType>
 void route_by_width(const RouteDev &p, float *weights, int32_t *ids, cudaStream_t stream) {
-    const uint32_t grid = route_grid(p.tokens), smem = kWarps * p.experts * sizeof(double);
+    const uint32_t grid = route_grid(p), smem = kWarps * p.experts * sizeof(double);
     if (p.experts <= 32) route_kernel<kType, 1><<<grid, kWarps * 32, smem, stream>>>(p, weights, ids);
     else if (p.experts <= 64) route_kernel<kType, 2><<<grid, kWarps * 32, smem, stream>>>(p, weights, ids);
     else if (p.experts <= 128) route_kernel<kType, 4><<<grid, kWarps * 32, smem, stream>>>(p, weights, ids);
@@ -493,7 +517,7 @@ cudaError_t launch_route(const RouteArgs &a, float *weights, int32_t *ids, cudaS
 
 cudaError_t launch_route_gradient(const RouteArgs &a, const float *weights_grad, const int32_t *ids, float *logits_grad, cudaStream_t stream) {
     const RouteDev p = route_dev(a);
-    const uint32_t grid = route_grid(a.tokens), smem = kWarps * ((a.experts + 3) / 4 * 4) * sizeof(float);
+    const uint32_t grid = route_grid(p), smem = kWarps * (32 / p.width) * ((a.experts + 3) / 4 * 4) * sizeof(float);
     switch (a.type) {
     case kF32: route_gradient_kernel<kF32><<<grid, kWarps * 32, smem, stream>>>(p, weights_grad, ids, logits_grad); break;
     case kBF16: route_gradient_kernel<kBF16><<<grid, kWarps * 32, smem, stream>>>(p, weights_grad, ids, logits_grad); break;

@@ -56,6 +56,29 @@ def test_route_odd_sizes(experts, top):
         run(t, exact, dict(top=top, score=score, bias=True, renormalise=False), np.zeros(experts, np.float32))
 
 
+@pytest.mark.parametrize("tokens", [4095, 4096, 4097, 5003])
+@pytest.mark.parametrize("experts,top", [(64, 6), (40, 9), (200, 20), (1000, 8), (33, 1)])
+def test_many_tokens(tokens, experts, top):
+    """Enough tokens that a warp works on several at once, numbers of them that fill no batch, infinities and ties among them."""
+    rng = np.random.default_rng(tokens + experts)
+    x = (rng.standard_normal((tokens, experts)) * 2).astype(np.float32)
+    x[5, :], x[7, ::2], x[tokens - 1, 1:] = -np.inf, np.nan, -np.inf
+    x[11] = 0
+    g = rng.standard_normal((tokens, top)).astype(np.float32)
+    for score, renormalise in (("softmax", True), ("sigmoid", True), ("softmax", False)):
+        how = dict(score=score, renormalise=renormalise, scale=1.5)
+        w, ids = nk.route(torch.from_numpy(x).cuda(), top, **how)
+        some = np.r_[0:40, tokens // 2:tokens // 2 + 9, tokens - 9:tokens]
+        want_w, want_ids = ref.route(x[some], top, **how)
+        assert np.array_equal(ids.cpu().numpy()[some], want_ids)
+        assert np.allclose(w.double().cpu().numpy()[some], want_w, rtol=WEIGHT_RTOL, atol=1e-37)
+        grad = nk.route_gradient(torch.from_numpy(g).cuda(), ids, torch.from_numpy(x).cuda(), **how)
+        assert nk.synchronize() == 0
+        want = ref.route_gradient(g[some], want_ids, x[some], **how)
+        size = 1.5 * np.abs(g[some]).sum(1, keepdims=True)
+        assert (np.abs(grad.double().cpu().numpy()[some] - want) <= WEIGHT_RTOL * (np.abs(want) + size)).all()
+
+
 def test_ties_go_to_the_lower_index():
     x = np.zeros((4, 64), np.float32)
     x[1, 50:] = 1
