@@ -117,6 +117,24 @@ __device__ __forceinline__ void load_logits(const uint8_t *row, uint32_t experts
     }
 }
 
+// Batcher's odd-even merge network: `v` in descending order.
+template <int kCount>
+__device__ __forceinline__ void sort_descending(uint32_t (&v)[kCount]) {
+#pragma unroll
+    for (int p = 1; p < kCount; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j <= kCount - 1 - k; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i <= kCount - j - k - 1 && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t a = v[i + j], b = v[i + j + k];
+                        v[i + j] = max(a, b);
+                        v[i + j + k] = min(a, b);
+                    }
+}
+
 // The choice in 64 bits, for the tokens whose keys 32 bits leave undecided. `keys`: room for one key per expert. Returns lane j's choice.
 template <uint32_t kType>
 __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, float top_logit, double *keys, int lane) {
@@ -174,13 +192,49 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     return chosen;
 }
 
+// Puts one token's choices (lane j: the j-th) in order by their keys in 64 bits, ties to the lower index.
+template <uint32_t kType>
+__device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *row, int32_t chosen, int lane) {
+    const bool direct = p.bias == nullptr && p.groups == 1;
+    double total = 1.0;
+    float top_logit = 0.0f;
+    if (!direct && !p.sigmoid) {
+        top_logit = -INFINITY;
+        for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
+        top_logit = warp_max(top_logit);
+        total = 0.0;
+#pragma unroll 4
+        for (uint32_t e = lane; e < p.experts; e += 32) total += exp((double)load_logit<kType>(row, e) - top_logit);
+        total = warp_sum(total);
+    }
+    double key = -INFINITY;
+    if (chosen >= 0) {
+        const float l = load_logit<kType>(row, chosen);
+        key = direct ? (double)l : (p.sigmoid ? sigmoid64(l) : exp((double)l - top_logit) / total) + load_bias(p.bias, chosen);
+    }
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < p.top; ++i) {
+        const double other = __shfl_sync(0xffffffffu, key, i);
+        const int32_t who = __shfl_sync(0xffffffffu, chosen, i);
+        rank += who >= 0 && (other > key || (other == key && who < chosen));
+    }
+    int32_t result = -1;
+    for (uint32_t j = 0; j < p.top; ++j) {
+        const uint32_t holder = __ballot_sync(0xffffffffu, chosen >= 0 && rank == j);
+        if (holder == 0) break;
+        const int32_t who = __shfl_sync(0xffffffffu, chosen, __ffs(holder) - 1);
+        if (lane == (int)j) result = who;
+    }
+    return result;
+}
+
 // One warp per token; lane i holds the experts i * kPer .. in registers.
 //
 // A key and its expert share one 32-bit word: the key in fixed point above, 31 - e of the warp's width below, so that one integer
 // maximum over the warp finds the next choice and gives ties to the lower index. The fixed point comes from scores in 32 bits;
 // `slack` bounds, in its units, how far it is off. Where every decision (chosen against next, open group against closed) is wider
-// than that, or is a tie of equal inputs, the choice is the one 64 bits would make; the other tokens, a few in a thousand on
-// random logits, go through choose_exactly. Keys that are the logits themselves (no bias, no groups) are the upper bits of their
+// than that, or is a tie of equal inputs, the choice is the one 64 bits would make; otherwise the chosen ones
+// are put in order in 64 bits, or, where groups or the last place are in question, the whole choice is made there (choose_exactly). Keys that are the logits themselves (no bias, no groups) are the upper bits of their
 // order-preserving integers, exact for 16-bit logits.
 //
 // Bound by instructions, about 600 a token. 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token
@@ -188,9 +242,11 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
 template <uint32_t kType, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, float *weights, int32_t *ids) {
     constexpr uint32_t kIndexBits = kPer == 1 ? 5 : kPer == 2 ? 6 : kPer == 4 ? 7 : kPer == 8 ? 8 : kPer == 16 ? 9 : 10;
+    constexpr bool kSorted = kPer <= 8;  // each lane keeps its keys in order; beyond that the network costs more than it saves
     constexpr uint32_t kWidth = 32 * kPer, kUnits = (1u << (32 - kIndexBits)) - 64;  // some room above for rounding
     extern __shared__ double keys_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto expert_of = [](uint32_t word) { return kWidth - 1 - (word & (kWidth - 1)); };
     const bool direct = p.bias == nullptr && p.groups == 1;
     const uint32_t size = p.experts / p.groups, lanes = size / kPer;
     const bool whole_lanes = size % kPer == 0 && (lanes & (lanes - 1)) == 0;  // a group is a power of two of lanes
@@ -208,9 +264,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
     least = fminf(least, 0.0f);                 // so that a key of 0 is on the scale
     const bool workable = direct || (fabsf(least) < 16.0f && fabsf(most) < 16.0f);  // wider biases leave the scale too coarse
     const float per_key = (float)kUnits / (1.0f + (most - least)), zero_key = -least * per_key;
-    // A score is off by a few units of its last place (exp, division), the softmax's sum one more per addition; the sum with the bias and
-    // the step to fixed point round four times more.
-    const uint32_t slack = (uint32_t)(((p.sigmoid ? 8.0f : (float)(kPer + 16)) + fabsf(least) + fabsf(most)) * 0x1p-23f * per_key) + 8u;
+    // A score is off by a few units of its last place (exp, division), the softmax's sum one more per addition (and its scores are at most
+    // 1 / sum); the sum with the bias and the step to fixed point round four times more.
+    const float score_error = (p.sigmoid ? 8.0f : (float)(kPer + 16)) * 0x1p-23f * per_key, bias_error = (fabsf(least) + fabsf(most)) * 0x1p-23f * per_key + 8.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) bias[i] = (bias[i] - least) * per_key;  // -infinity stays
     // A warp chooses for `batch` tokens one after the other and then works out their weights together, `width` lanes each.
@@ -231,13 +287,13 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
             top_logit = warp_max(top_logit);
         }
-        uint32_t key[kPer];
+        uint32_t key[kPer], slack = 0;
         const uint32_t last = kWidth - 1 - lane * kPer;
         if (direct) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) key[i] = logit[i] > -INFINITY ? (selection_key(logit[i]) & ~(kWidth - 1)) | (last - i) : 0u;
         } else {
-            float scaled = per_key;
+            float scaled = per_key, largest_score = 1.0f;
             float part[kPer];
             if (p.sigmoid) {
 #pragma unroll
@@ -249,7 +305,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
 #pragma unroll
                 for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
                 scaled = __fdividef(per_key, total);
+                largest_score = __fdividef(1.0f, total);
             }
+            slack = (uint32_t)fmaf(score_error, largest_score, bias_error) + 1u;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const float units = fmaf(part[i], scaled, bias[i]);
@@ -257,6 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                 key[i] = logit[i] > -INFINITY && units > -INFINITY ? ((__float2uint_rz(units) + 1u) << kIndexBits) | (last - i) : 0u;
             }
         }
+        if constexpr (kSorted) sort_descending(key);
         bool sure = workable;
         if (p.groups > 1) {
             uint32_t worth = 0;  // lane g: group g's, in units; 0 where nobody is left
@@ -267,9 +326,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                 return (a >> 1) + (b >> 1) + 1u;  // half units: the sum fits 32 bits
             };
             if (whole_lanes) {
-                uint32_t first = 0, second = 0;
+                uint32_t first = key[0], second = 0;
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) {
+                for (int i = 1; i < (kSorted && kPer > 2 ? 2 : kPer); ++i) {
                     second = max(second, min(first, key[i]));
                     first = max(first, key[i]);
                 }
@@ -284,7 +343,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                     uint32_t first = 0, second = 0;
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) {
-                        const uint32_t e = lane * kPer + i, k = e >= g * size && e < (g + 1) * size ? key[i] : 0u;
+                        const uint32_t e = expert_of(key[i]), k = e >= g * size && e < (g + 1) * size ? key[i] : 0u;
                         second = max(second, min(first, k));
                         first = max(first, k);
                     }
@@ -312,31 +371,53 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const uint32_t group = (lane * kPer + i) / size;
-                    if (group >= 32u || !((open_groups >> group) & 1u)) key[i] = 0u;
+                for (int i = 0; i < kPer; ++i)
+                    if (key[i] != 0u && !((open_groups >> (expert_of(key[i]) / size)) & 1u)) key[i] = 0u;
+                if constexpr (kSorted) sort_descending(key);
+            }
+        }
+        // Lane j takes the j-th word; one more is looked at, since it has to be further off than the error, too.
+        const uint32_t unsure_at = direct ? 0u : 2 * slack;
+        uint32_t word = 0, behind = 0;
+        for (uint32_t j = 0; j <= p.top; ++j) {
+            uint32_t mine = key[0];
+            if constexpr (!kSorted) {
+#pragma unroll
+                for (int i = 1; i < kPer; ++i) mine = max(mine, key[i]);
+            }
+            behind = __reduce_max_sync(0xffffffffu, mine);
+            if (behind == 0) break;
+            if (mine == behind) {
+                if constexpr (kSorted) {
+#pragma unroll
+                    for (int i = 0; i + 1 < kPer; ++i) key[i] = key[i + 1];
+                    key[kPer - 1] = 0u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        if (key[i] == behind) key[i] = 0u;
                 }
             }
+            if (lane == (int)j) word = behind;
         }
-        int32_t chosen = -1;  // lane j: the expert of slot j
-        uint32_t before = 0xffffffffu;  // the word before; the one behind the last choice has to be further off than the error, too
-        for (uint32_t j = 0; j <= p.top && sure; ++j) {
-            uint32_t mine = key[0];
-#pragma unroll
-            for (int i = 1; i < kPer; ++i) mine = max(mine, key[i]);
-            const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
-            if (best == 0) break;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (key[i] == best) key[i] = 0u;
-            const uint32_t who = kWidth - 1 - (best & (kWidth - 1));
-            if (j > 0 && (before >> kIndexBits) - (best >> kIndexBits) <= (direct ? 0u : 2 * slack)) {
-                const uint32_t previous = kWidth - 1 - (before & (kWidth - 1));
-                sure = load_logit<kType>(row, who) == load_logit<kType>(row, previous) && load_bias(p.bias, who) == load_bias(p.bias, previous);
+        auto undecided = [&](uint32_t ahead, uint32_t then) {  // closer than the error, and not a tie of equal inputs
+            if (then == 0 || (ahead >> kIndexBits) - (then >> kIndexBits) > unsure_at) return false;
+            const uint32_t x = expert_of(ahead), y = expert_of(then);
+            return !(load_logit<kType>(row, x) == load_logit<kType>(row, y) && load_bias(p.bias, x) == load_bias(p.bias, y));
+        };
+        const uint32_t before = __shfl_up_sync(0xffffffffu, word, 1);
+        bool ordered = !__any_sync(0xffffffffu, lane > 0 && undecided(before, word));
+        if (p.top == 32) ordered = ordered && !undecided(__shfl_sync(0xffffffffu, word, 31), behind);
+        int32_t chosen = word != 0 && lane < (int)p.top ? (int32_t)expert_of(word) : -1;
+        if (sure && !ordered) {
+            // Too near to one another, but clear of the expert behind the last: the chosen ones are put in order by their keys in 64 bits.
+            const uint32_t last_word = __shfl_sync(0xffffffffu, word, p.top - 1);
+            if (behind == 0 || (last_word >> kIndexBits) - (behind >> kIndexBits) > unsure_at) {
+                chosen = order_exactly<kType>(p, row, chosen, lane);
+                ordered = true;
             }
-            before = best;
-            if (lane == (int)j && j < p.top) chosen = (int32_t)who;
         }
+        sure = sure && ordered;
         if (!sure) {
             if (p.sigmoid) {
 #pragma unroll
