@@ -102,7 +102,29 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
         const uint8_t *row = x + (uint64_t)from * x_stride;
         const uint32_t count = min((uint32_t)kAhead, depth_blocks - piece.kb0);
         uint32_t my_scale = 0;  // lane i: the scale of block i % 8 of chunk row kb0 + i / 8
-        if (aligned) {
+        const uint64_t byte0 = (uint64_t)piece.kb0 * 128 + lane * 4;
+        uint8_t *to = kTiled ? chunks + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0) * kMxCodeBytes + (piece.row % kChunkRows) * 128u +
+                                   ((((uint32_t)lane >> 2) ^ (piece.row & 7u)) << 4) + (lane & 3) * 4
+                             : out.codes + piece.row * out.codes_stride + byte0;
+        if (aligned && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth && (kTiled || (out.codes_stride & 3u) == 0 && (reinterpret_cast<uintptr_t>(out.codes) & 3u) == 0)) {
+            // Whole pieces on their boundaries: nothing to guard.
+            const uint8_t *from8 = row + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
+            uint4 raw[kAhead][kBytes / 2];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int h = 0; h < kBytes / 2; ++h) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(from8 + u * kMxChunkValues * kBytes) + h);
+            uint32_t four = 0;  // this thread's block's scales in the four chunk rows
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                float v[8];
+                uint32_t s;
+                const uint32_t largest = unpack8<kType>(raw[u], v);
+                *reinterpret_cast<uint32_t *>(to + u * (kTiled ? kMxCodeBytes : 128u)) = quantise8(v, largest, s);
+                four |= s << (8 * u);
+            }
+            my_scale = (__shfl_sync(0xffffffffu, four, (lane & 7) * 4) >> (lane & 24)) & 255u;
+        } else if (aligned) {
             uint4 raw[kAhead][kBytes / 2];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
@@ -205,7 +227,37 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
         uint8_t *to = x + piece.row * x_stride;
         const uint64_t block = (uint64_t)piece.kb0 * 8 + lane;
         const uint32_t my_scale = block * kMxBlock < depth ? scales[piece.row * scales_stride + block] : 0u;
-        if (aligned) {
+        if (aligned && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth) {
+            // Whole pieces on their boundaries: nothing to guard.
+            const uint8_t *from8 = row + (uint64_t)piece.kb0 * 128 + lane * 4;
+            uint8_t *to8 = to + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
+            uint32_t w[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) w[u] = __ldg(reinterpret_cast<const uint32_t *>(from8 + u * 128));
+            const float own_scale = scale_value(my_scale);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const float scale = __shfl_sync(0xffffffffu, own_scale, u * 8 + (lane >> 2));
+                uint32_t value[2 * kBytes];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = decode2((w[u] >> (8 * i)) & 255u);
+                    if constexpr (kType == kF32) {
+                        value[2 * i] = __float_as_uint(v.x * scale);
+                        value[2 * i + 1] = __float_as_uint(v.y * scale);
+                    } else if constexpr (kType == kBF16) {
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(v.x * scale, v.y * scale);
+                        value[i] = *reinterpret_cast<const uint32_t *>(&two);
+                    } else {
+                        const __half2 two = __floats2half2_rn(v.x * scale, v.y * scale);
+                        value[i] = *reinterpret_cast<const uint32_t *>(&two);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < kBytes / 2; ++h)
+                    reinterpret_cast<uint4 *>(to8 + u * kMxChunkValues * kBytes)[h] = make_uint4(value[4 * h], value[4 * h + 1], value[4 * h + 2], value[4 * h + 3]);
+            }
+        } else if (aligned) {
             uint32_t w[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
