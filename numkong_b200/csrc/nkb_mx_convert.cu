@@ -30,19 +30,13 @@ struct RowMajorSink {
 
 constexpr int kAhead = 4;  // chunk rows (256 values) a warp has in flight
 
-// The warp's piece of work: chunk rows kb0 .. kb0 + kAhead of one row.
+// The warp's piece of work: chunk rows kb0 .. kb0 + ahead of one row (kAhead of them, or one where there are few).
 struct Piece {
     uint32_t row, kb0;
 };
-__device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t pieces_per_row) {
+__device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t pieces_per_row, uint32_t ahead) {
     const uint32_t row = item / pieces_per_row;
-    return {row, (item - row * pieces_per_row) * kAhead};
-}
-
-template <uint32_t kType>
-__device__ __forceinline__ float load_value(const uint8_t *p) {
-    if constexpr (kType == kF32) return __ldg(reinterpret_cast<const float *>(p));
-    else return decode_bits<kType>(__ldg(reinterpret_cast<const uint16_t *>(p)));
+    return {row, (item - row * pieces_per_row) * ahead};
 }
 
 // The warp's 32 words (lane i: bytes 4 i .. 4 i + 3) to `p`, of which `bytes` exist. Off a four-byte boundary the words are
@@ -79,20 +73,23 @@ __device__ __forceinline__ void store_chunk_row(uint32_t codes, uint32_t row, ui
 
 // A warp turns 256 values of a row (a chunk row) into 128 bytes of codes and eight scales at a time, four such pieces in flight.
 //   rows on 16-byte boundaries: a thread loads eight consecutive values, four threads share a block
-//   otherwise: a thread loads value `lane` of each block, so that a load still covers whole lines; the codes change hands by shuffles
+//   otherwise: a thread loads value `lane` of each block, so that a load still covers whole lines, and the values change hands in
+//   shared memory
 // 8192 x 8192 bf16: 170 MB in 30 us where the copy rate allows 26; with one piece in flight 50 us.
 template <uint32_t kType, bool kTiled>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, uint32_t rows, uint64_t depth, uint64_t x_stride, RowMajorSink out,
                                                             uint8_t *chunks, uint8_t *scale_tiles, uint32_t depth_blocks, const int32_t *row_dest,
-                                                            const int32_t *tile_count, uint32_t tile_rows, uint32_t divide) {
+                                                            const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, uint32_t ahead) {
     if constexpr (kTiled) allow_next_kernel();  // the product that reads the chunks may set itself up meanwhile
     if (kTiled && row_dest) rows = (uint32_t)*tile_count * tile_rows;
     constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0;
-    const uint32_t pieces_per_row = (depth_blocks + kAhead - 1) / kAhead, items = rows * pieces_per_row;
+    __shared__ __align__(16) uint8_t staging_all[kThreads / 32][kMxChunkValues * kBytes];
+    uint8_t *staging = staging_all[threadIdx.x >> 5];
+    const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = rows * pieces_per_row;
     for (uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (kThreads / 32)) {
-        const Piece piece = piece_of(item, pieces_per_row);
+        const Piece piece = piece_of(item, pieces_per_row, ahead);
         uint32_t from = piece.row;
         if (kTiled && row_dest) {
             const int32_t d = row_dest[piece.row];
@@ -100,13 +97,13 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
             from = (uint32_t)d / divide;
         }
         const uint8_t *row = x + (uint64_t)from * x_stride;
-        const uint32_t count = min((uint32_t)kAhead, depth_blocks - piece.kb0);
+        const uint32_t count = min(ahead, depth_blocks - piece.kb0);
         uint32_t my_scale = 0;  // lane i: the scale of block i % 8 of chunk row kb0 + i / 8
         const uint64_t byte0 = (uint64_t)piece.kb0 * 128 + lane * 4;
         uint8_t *to = kTiled ? chunks + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0) * kMxCodeBytes + (piece.row % kChunkRows) * 128u +
                                    ((((uint32_t)lane >> 2) ^ (piece.row & 7u)) << 4) + (lane & 3) * 4
                              : out.codes + piece.row * out.codes_stride + byte0;
-        if (aligned && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth && (kTiled || (out.codes_stride & 3u) == 0 && (reinterpret_cast<uintptr_t>(out.codes) & 3u) == 0)) {
+        if (aligned && ahead == kAhead && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth && (kTiled || (out.codes_stride & 3u) == 0 && (reinterpret_cast<uintptr_t>(out.codes) & 3u) == 0)) {
             // Whole pieces on their boundaries: nothing to guard.
             const uint8_t *from8 = row + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
             uint4 raw[kAhead][kBytes / 2];
@@ -155,28 +152,37 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
                 if ((lane >> 3) == u) my_scale = mine;
             }
         } else {
-#pragma unroll 2
-            for (uint32_t u = 0; u < count; ++u) {
-                const uint64_t first = (uint64_t)(piece.kb0 + u) * kMxChunkValues + lane;
-                float v[8];
+            uint32_t all[kAhead][8];
 #pragma unroll
-                for (int b = 0; b < 8; ++b) v[b] = first + b * 32 < depth ? load_value<kType>(row + (first + b * 32) * kBytes) : 0.0f;
-                uint32_t codes = 0;
+            for (int u = 0; u < kAhead; ++u)
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
-                    const uint32_t s = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
-                    const float scaled = s == 255u ? 0.0f : v[b] * inverse_scale(s);
-                    uint32_t code;
-                    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(code) : "f"(scaled), "f"(0.0f));
-                    uint32_t word = code << (4 * (lane & 7));  // eight lanes make a word
-                    word |= __shfl_xor_sync(0xffffffffu, word, 1);
-                    word |= __shfl_xor_sync(0xffffffffu, word, 2);
-                    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                    word = __shfl_sync(0xffffffffu, word, (lane & 3) * 8);
-                    if ((lane >> 2) == b) codes = word;
-                    if (lane == (int)(u * 8 + b)) my_scale = s;
+                    const uint64_t at = (uint64_t)(piece.kb0 + u) * kMxChunkValues + b * 32 + lane;
+                    all[u][b] = 0;
+                    if (u < (int)count && at < depth) {
+                        if constexpr (kType == kF32) all[u][b] = __ldg(reinterpret_cast<const uint32_t *>(row) + at);
+                        else all[u][b] = __ldg(reinterpret_cast<const uint16_t *>(row) + at);
+                    }
                 }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (u >= (int)count) break;
+                __syncwarp();
+#pragma unroll
+                for (int b = 0; b < 8; ++b) {
+                    if constexpr (kType == kF32) reinterpret_cast<uint32_t *>(staging)[b * 32 + lane] = all[u][b];
+                    else reinterpret_cast<uint16_t *>(staging)[b * 32 + lane] = (uint16_t)all[u][b];
+                }
+                __syncwarp();
+                uint4 raw[kBytes / 2];
+#pragma unroll
+                for (int h = 0; h < kBytes / 2; ++h) raw[h] = reinterpret_cast<const uint4 *>(staging + lane * 8 * kBytes)[h];
+                float v[8];
+                uint32_t s;
+                const uint32_t largest = unpack8<kType>(raw, v), codes = quantise8(v, largest, s);
                 store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
+                const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
+                if ((lane >> 3) == u) my_scale = mine;
             }
         }
         if constexpr (kTiled) {
@@ -210,24 +216,27 @@ __device__ __forceinline__ uint32_t encode16(float v) {
 }
 
 // The way back, a warp per piece as above: the values the codes stand for (rounded to nearest where the type is narrower: f16
-// only, whose range the scale can leave). Rows off their boundaries are read byte by byte and written value by value, a warp's
-// accesses side by side.
+// only, whose range the scale can leave). Rows off their boundaries are read byte by byte and written value by value, through shared
+// memory, so that a warp's accesses lie side by side.
 template <uint32_t kType>
 __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
-                                                              uint32_t rows, uint64_t depth, uint8_t *x, uint64_t x_stride, uint32_t depth_blocks) {
+                                                              uint32_t rows, uint64_t depth, uint8_t *x, uint64_t x_stride, uint32_t depth_blocks,
+                                                              uint32_t ahead) {
     constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0 && ((reinterpret_cast<uintptr_t>(codes) | codes_stride) & 3u) == 0;
+    __shared__ __align__(16) uint8_t staging_all[kThreads / 32][kMxChunkValues * kBytes];
+    uint8_t *staging = staging_all[threadIdx.x >> 5];
     const uint64_t row_bytes = (depth + 1) / 2;
-    const uint32_t pieces_per_row = (depth_blocks + kAhead - 1) / kAhead, items = rows * pieces_per_row;
+    const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = rows * pieces_per_row;
     for (uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (kThreads / 32)) {
-        const Piece piece = piece_of(item, pieces_per_row);
-        const uint32_t count = min((uint32_t)kAhead, depth_blocks - piece.kb0);
+        const Piece piece = piece_of(item, pieces_per_row, ahead);
+        const uint32_t count = min(ahead, depth_blocks - piece.kb0);
         const uint8_t *row = codes + piece.row * codes_stride;
         uint8_t *to = x + piece.row * x_stride;
         const uint64_t block = (uint64_t)piece.kb0 * 8 + lane;
         const uint32_t my_scale = block * kMxBlock < depth ? scales[piece.row * scales_stride + block] : 0u;
-        if (aligned && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth) {
+        if (aligned && ahead == kAhead && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth) {
             // Whole pieces on their boundaries: nothing to guard.
             const uint8_t *from8 = row + (uint64_t)piece.kb0 * 128 + lane * 4;
             uint8_t *to8 = to + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
@@ -297,20 +306,41 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
                 }
             }
         } else {
-#pragma unroll 2
-            for (uint32_t u = 0; u < count; ++u) {
-                const uint64_t first = (uint64_t)(piece.kb0 + u) * kMxChunkValues + lane;
-                uint32_t byte[8];
+            uint32_t w[kAhead];
 #pragma unroll
-                for (int b = 0; b < 8; ++b) byte[b] = first + b * 32 < depth ? __ldg(row + (first + b * 32) / 2) : 0u;
+            for (int u = 0; u < kAhead; ++u) {
+                const uint64_t byte = (uint64_t)(piece.kb0 + u) * 128 + lane * 4;
+                w[u] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (u < (int)count && byte + i < row_bytes) w[u] |= (uint32_t)__ldg(row + byte + i) << (8 * i);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (u >= (int)count) break;
+                const float scale = scale_value(__shfl_sync(0xffffffffu, my_scale, u * 8 + (lane >> 2)));
+                uint32_t value[2 * kBytes];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = decode2((w[u] >> (8 * i)) & 255u);
+                    if constexpr (kType == kF32) {
+                        value[2 * i] = __float_as_uint(v.x * scale);
+                        value[2 * i + 1] = __float_as_uint(v.y * scale);
+                    } else {
+                        value[i] = encode16<kType>(v.x * scale) | (encode16<kType>(v.y * scale) << 16);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < kBytes / 2; ++h)
+                    reinterpret_cast<uint4 *>(staging + lane * 8 * kBytes)[h] = make_uint4(value[4 * h], value[4 * h + 1], value[4 * h + 2], value[4 * h + 3]);
+                __syncwarp();
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
-                    const float scale = scale_value(__shfl_sync(0xffffffffu, my_scale, u * 8 + b));
-                    const float2 two = decode2(byte[b]);
-                    const float v = (lane & 1 ? two.y : two.x) * scale;
-                    if (first + b * 32 < depth) {
-                        if constexpr (kType == kF32) reinterpret_cast<float *>(to)[first + b * 32] = v;
-                        else reinterpret_cast<uint16_t *>(to)[first + b * 32] = (uint16_t)encode16<kType>(v);
+                    const uint64_t at = (uint64_t)(piece.kb0 + u) * kMxChunkValues + b * 32 + lane;
+                    if (at < depth) {
+                        if constexpr (kType == kF32) reinterpret_cast<uint32_t *>(to)[at] = reinterpret_cast<const uint32_t *>(staging)[b * 32 + lane];
+                        else reinterpret_cast<uint16_t *>(to)[at] = reinterpret_cast<const uint16_t *>(staging)[b * 32 + lane];
                     }
                 }
             }
@@ -382,7 +412,10 @@ __global__ void __launch_bounds__(kThreads) tile_scales_kernel(const uint8_t *sc
     }
 }
 
-uint64_t pieces(uint32_t kblocks) { return (kblocks + kAhead - 1) / kAhead; }  // per row
+// Chunk rows a warp takes. So few that the GPU has warps to spare go to one warp each: 8 x 4096 bf16 1.9 us against 2.6; 5003 x 776, where it
+// has not, 8.4 us against 6.5.
+uint32_t ahead_for(uint64_t rows, uint32_t kblocks) { return rows * kblocks < 2048 ? 1 : kAhead; }
+uint64_t pieces(uint32_t kblocks, uint32_t ahead) { return (kblocks + ahead - 1) / ahead; }  // per row
 uint32_t grid_for(uint64_t warps) {
     const uint64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
     return (uint32_t)(blocks < 148ull * 8 * 4 ? (blocks ? blocks : 1) : 148ull * 8 * 4);
@@ -395,13 +428,14 @@ cudaError_t launch_mx_quantise(uint32_t type, const void *x, uint64_t rows, uint
     const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues);
     if (rows == 1) x_stride = 0;  // no stride to be aligned
     const RowMajorSink out{static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), codes_stride, scales_stride};
-    if (rows * pieces(kblocks) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
-    const uint32_t grid = grid_for(rows * pieces(kblocks)), n = (uint32_t)rows;
+    const uint32_t ahead = ahead_for(rows, kblocks);
+    if (rows * pieces(kblocks, ahead) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
+    const uint32_t grid = grid_for(rows * pieces(kblocks, ahead)), n = (uint32_t)rows;
     const uint8_t *src = static_cast<const uint8_t *>(x);
     switch (type) {
-    case kF32: quantise_kernel<kF32, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
-    case kBF16: quantise_kernel<kBF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
-    case kF16: quantise_kernel<kF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1); break;
+    case kF32: quantise_kernel<kF32, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1, ahead); break;
+    case kBF16: quantise_kernel<kBF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1, ahead); break;
+    case kF16: quantise_kernel<kF16, false><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, out, nullptr, nullptr, kblocks, nullptr, nullptr, 0, 1, ahead); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
@@ -411,14 +445,15 @@ cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t dept
                                      const int32_t *row_dest, const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, void *chunks, cudaStream_t stream) {
     const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues);
     const RowMajorSink none{nullptr, nullptr, 0, 0};
-    if (tiled_rows * pieces(kblocks) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
-    const uint32_t grid = grid_for(tiled_rows * pieces(kblocks)), n = (uint32_t)tiled_rows;
+    const uint32_t ahead = ahead_for(tiled_rows, kblocks);
+    if (tiled_rows * pieces(kblocks, ahead) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
+    const uint32_t grid = grid_for(tiled_rows * pieces(kblocks, ahead)), n = (uint32_t)tiled_rows;
     const uint8_t *src = static_cast<const uint8_t *>(x);
     uint8_t *dst = static_cast<uint8_t *>(chunks), *tiles = dst + (tiled_rows + kChunkRows - 1) / kChunkRows * kblocks * kMxCodeBytes;
     switch (type) {
-    case kF32: quantise_kernel<kF32, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
-    case kBF16: quantise_kernel<kBF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
-    case kF16: quantise_kernel<kF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide); break;
+    case kF32: quantise_kernel<kF32, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
+    case kBF16: quantise_kernel<kBF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
+    case kF16: quantise_kernel<kF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
@@ -427,15 +462,16 @@ cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t dept
 cudaError_t launch_mx_dequantise(uint32_t type, const void *codes, uint64_t codes_stride, const void *scales, uint64_t scales_stride,
                                  uint64_t rows, uint64_t depth, void *x, uint64_t x_stride, cudaStream_t stream) {
     const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues);
-    if (rows * pieces(kblocks) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
-    const uint32_t grid = grid_for(rows * pieces(kblocks)), n = (uint32_t)rows;
+    const uint32_t ahead = ahead_for(rows, kblocks);
+    if (rows * pieces(kblocks, ahead) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
+    const uint32_t grid = grid_for(rows * pieces(kblocks, ahead)), n = (uint32_t)rows;
     if (rows == 1) codes_stride = x_stride = 0;
     const uint8_t *c = static_cast<const uint8_t *>(codes), *s = static_cast<const uint8_t *>(scales);
     uint8_t *dst = static_cast<uint8_t *>(x);
     switch (type) {
-    case kF32: dequantise_kernel<kF32><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks); break;
-    case kBF16: dequantise_kernel<kBF16><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks); break;
-    case kF16: dequantise_kernel<kF16><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks); break;
+    case kF32: dequantise_kernel<kF32><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks, ahead); break;
+    case kBF16: dequantise_kernel<kBF16><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks, ahead); break;
+    case kF16: dequantise_kernel<kF16><<<grid, kThreads, 0, stream>>>(c, codes_stride, s, scales_stride, n, depth, dst, x_stride, kblocks, ahead); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();
