@@ -348,39 +348,53 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
     }
 }
 
-// Row-major codes and scales -> chunks: one warp per chunk row, four bytes of codes per thread. Both codes of the last byte of
-// an odd depth count, as for the other 4-bit types; what lies past the depth is zero codes under scale 1.
+// Bytes [0, count) from any address, four to a thread: aligned words, of which only those that hold one of the bytes are read, shifted into
+// place. `count` may be negative.
+__device__ __forceinline__ uint32_t load_words(const uint8_t *p, int64_t count, int lane) {
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 3u;
+    const uint32_t *from = reinterpret_cast<const uint32_t *>(p - off);
+    const int64_t end = count > 0 ? count + off : 0;
+    const uint32_t w = 4 * lane < end ? __ldg(from + lane) : 0u;
+    uint32_t behind = __shfl_down_sync(0xffffffffu, w, 1);
+    if (lane == 31) behind = off != 0 && 128 < end ? __ldg(from + 32) : 0u;
+    const uint32_t v = __funnelshift_r(w, behind, 8 * off);
+    const int64_t left = count - 4 * lane;
+    return left >= 4 ? v : left > 0 ? v & ((1u << (8 * (int)left)) - 1u) : 0u;
+}
+
+// Row-major codes and scales -> chunks: one warp per piece of up to four chunk rows, four bytes of codes per thread. Both codes of the
+// last byte of an odd depth count, as for the other 4-bit types; what lies past the depth is zero codes under scale 1.
 __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
-                                                        uint64_t width, uint64_t depth, uint64_t tiled_rows, uint32_t group_rows, uint8_t *chunks,
-                                                        uint8_t *scale_tiles, uint32_t depth_blocks) {
+                                                        uint32_t width, uint64_t depth, uint32_t tiled_rows, uint32_t group_rows, uint8_t *chunks,
+                                                        uint8_t *scale_tiles, uint32_t depth_blocks, uint32_t ahead) {
     allow_next_kernel();
     const int lane = threadIdx.x & 31;
     const uint64_t row_bytes = (depth + 1) / 2, row_scales = (depth + kMxBlock - 1) / kMxBlock;
-    const uint64_t items = tiled_rows * depth_blocks, step = (uint64_t)gridDim.x * (kThreads / 32);
-    for (uint64_t item = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += step) {
-        const uint64_t row = item / depth_blocks;
-        const uint32_t kb = (uint32_t)(item - row * depth_blocks);
-        const uint64_t group = row / group_rows, in_group = row - group * group_rows;
+    const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = tiled_rows * pieces_per_row;
+    for (uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (kThreads / 32)) {
+        const Piece piece = piece_of(item, pieces_per_row, ahead);
+        const uint32_t group = piece.row / group_rows, in_group = piece.row - group * group_rows, r = piece.row % kChunkRows;
+        const uint32_t count = min(ahead, depth_blocks - piece.kb0);
         const bool real = in_group < width;
-        const uint64_t from = group * width + in_group;
-        const uint64_t byte = (uint64_t)kb * 128u + lane * 4;
-        uint32_t w = 0;
-        if (real) {
-            const uint8_t *c = codes + from * codes_stride + byte;
-            if (byte + 4 <= row_bytes && (reinterpret_cast<uintptr_t>(c) & 3u) == 0) w = __ldg(reinterpret_cast<const uint32_t *>(c));
-            else
-                for (int i = 0; i < 4; ++i)
-                    if (byte + i < row_bytes) w |= (uint32_t)c[i] << (8 * i);
+        const uint64_t from = (uint64_t)group * width + in_group;
+        uint32_t w[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint64_t byte = (uint64_t)(piece.kb0 + u) * 128u;
+            w[u] = load_words(codes + from * codes_stride + byte, real && u < (int)count ? (int64_t)row_bytes - (int64_t)byte : 0, lane);
         }
-        const uint64_t at = (row / kChunkRows) * depth_blocks + kb;
-        uint8_t *chunk = chunks + at * kMxCodeBytes;
-        const uint32_t r = (uint32_t)(row % kChunkRows);
-        *reinterpret_cast<uint32_t *>(chunk + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = w;
-        if (lane < 8) {
-            const uint64_t block = (uint64_t)kb * 8u + lane;
-            const uint8_t s = real && block < row_scales ? scales[from * scales_stride + block] : (uint8_t)127;
-            scale_tiles[at * kMxScaleBytes + (lane >> 2) * 512 + (r & 31u) * 16 + (r >> 5) * 4 + (lane & 3)] = s;
-        }
+        const uint64_t block = (uint64_t)piece.kb0 * 8u + lane;  // lane i: the scale of block i % 8 of chunk row kb0 + i / 8
+        const uint32_t s = real && block < row_scales ? scales[from * scales_stride + block] : 127u;
+        const uint64_t at = (uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0;
+        uint8_t *chunk = chunks + at * kMxCodeBytes + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (u < (int)count) *reinterpret_cast<uint32_t *>(chunk + u * kMxCodeBytes) = w[u];
+        uint32_t four = s << (8 * (lane & 3));
+        four |= __shfl_xor_sync(0xffffffffu, four, 1);
+        four |= __shfl_xor_sync(0xffffffffu, four, 2);
+        if ((lane & 3) == 0 && (uint32_t)(lane >> 3) < count)
+            *reinterpret_cast<uint32_t *>(scale_tiles + (at + (lane >> 3)) * kMxScaleBytes + ((lane >> 2) & 1) * 512 + (r & 31u) * 16 + (r >> 5) * 4) = four;
     }
 }
 
@@ -490,10 +504,12 @@ cudaError_t launch_mx_tile(const void *codes, uint64_t codes_stride, const void 
     const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues);
     const uint64_t group_rows = (width + kChunkRows - 1) / kChunkRows * kChunkRows;
     const uint64_t rows = pad_rows ? groups * group_rows : (groups - 1) * group_rows + width;
-    tile_kernel<<<grid_for(rows * kblocks), kThreads, 0, stream>>>(static_cast<const uint8_t *>(codes), codes_stride, static_cast<const uint8_t *>(scales),
-                                                                   scales_stride, width, depth, rows, (uint32_t)group_rows,
-                                                                   static_cast<uint8_t *>(chunks),
-                                                                   static_cast<uint8_t *>(chunks) + groups * group_rows / kChunkRows * kblocks * kMxCodeBytes, kblocks);
+    const uint32_t ahead = ahead_for(rows, kblocks);
+    if (rows * pieces(kblocks, ahead) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
+    uint8_t *dst = static_cast<uint8_t *>(chunks);
+    tile_kernel<<<grid_for(rows * pieces(kblocks, ahead)), kThreads, 0, stream>>>(static_cast<const uint8_t *>(codes), codes_stride, static_cast<const uint8_t *>(scales),
+                                                                                  scales_stride, (uint32_t)width, depth, (uint32_t)rows, (uint32_t)group_rows, dst,
+                                                                                  dst + groups * group_rows / kChunkRows * kblocks * kMxCodeBytes, kblocks, ahead);
     return cudaGetLastError();
 }
 

@@ -216,6 +216,41 @@ def test_product_strides_and_out():
         assert (wide[0] == 7).all() and (wide[-1] == 7).all() and (wide[:, 0] == 7).all() and (wide[:, 1 + n:] == 7).all()
 
 
+@pytest.mark.parametrize("cells", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(40, 301, 300), (3, 150, 64), (2300, 2311, 260)])
+def test_product_out_at_any_offset(m, n, k, cells):
+    """Result rows at every cell offset from a 16-byte boundary, what lies around them untouched."""
+    a, b = random_mx(m, k, 8), random_mx(n, k, 9)
+    x = nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in a), k)
+    packed = nk.dots_pack(nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), k))
+    want = nk.dots_packed(x, packed, out_dtype=cells)
+    check_product(a, b, k, want, cells)
+    for first, pad in ((0, 1), (1, 0), (2, 3), (3, 6), (4, 2), (5, 5), (6, 1), (7, 9)):
+        wide = torch.full((m + 2, first + n + pad), 7.0, dtype=TORCH[cells], device="cuda")
+        got = nk.dots_packed(x, packed, out=wide[1:-1, first:first + n], out_dtype=cells)
+        assert nk.synchronize() == 0
+        assert torch.equal(got, want)
+        assert (wide[0] == 7).all() and (wide[-1] == 7).all() and (wide[:, :first] == 7).all() and (wide[:, first + n:] == 7).all()
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+@pytest.mark.parametrize("depth", [1, 2, 7, 255, 513, 1291])
+def test_codes_at_any_offset(depth, offset):
+    """Codes and scales whose rows begin at every byte of a word, packed and multiplied."""
+    rows = 50
+    a, b = random_mx(rows, depth, depth), random_mx(9, depth, depth + 1)
+    def held(part):
+        wide = np.full((rows, part.shape[1] + 5), 255, np.uint8)
+        wide[:, offset:offset + part.shape[1]] = part
+        return torch.from_numpy(wide).cuda()[:, offset:offset + part.shape[1]]
+    x = nk.MxMatrix(held(a[0]), held(a[1]), depth)
+    few = nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), depth)
+    one, other = nk.dots_packed(x, nk.dots_pack(few)), nk.dots_packed(few, nk.dots_pack(x))
+    assert nk.synchronize() == 0
+    check_product(a, b, depth, one, "f32")
+    assert torch.equal(one, other.T)
+
+
 def test_product_on_the_host():
     m, n, k = 40, 150, 333
     a, b = random_mx(m, k, 6), random_mx(n, k, 7)
