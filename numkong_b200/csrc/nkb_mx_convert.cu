@@ -81,18 +81,19 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
                                                             uint8_t *chunks, uint8_t *scale_tiles, uint32_t depth_blocks, const int32_t *row_dest,
                                                             const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, uint32_t ahead) {
     if constexpr (kTiled) allow_next_kernel();  // the product that reads the chunks may set itself up meanwhile
-    if (kTiled && row_dest) rows = (uint32_t)*tile_count * tile_rows;
     constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0;
     __shared__ __align__(16) uint8_t staging_all[kThreads / 32][kMxChunkValues * kBytes];
     uint8_t *staging = staging_all[threadIdx.x >> 5];
     const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = rows * pieces_per_row;
+    const uint32_t used = kTiled && row_dest ? (uint32_t)*tile_count * tile_rows : rows;
     for (uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (kThreads / 32)) {
         const Piece piece = piece_of(item, pieces_per_row, ahead);
         uint32_t from = piece.row;
         if (kTiled && row_dest) {
-            const int32_t d = row_dest[piece.row];
+            const int32_t d = row_dest[piece.row];  // whether the row is used comes in at the same time
+            if (piece.row >= used) break;
             if (d < 0) continue;
             from = (uint32_t)d / divide;
         }

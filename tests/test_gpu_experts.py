@@ -144,3 +144,11 @@ def test_a_layer_of_experts_from_logits_to_sums():
     assert np.array_equal(ids.cpu().numpy(), want_ids)
     y, bound = expected(h.cpu(), want_ids, second_q.codes.cpu().numpy(), second_q.scales.cpu().numpy(), k, hidden, weights.cpu().numpy())
     assert (np.abs(out.double().cpu().numpy() - y) <= bound).all()
+
+
+@pytest.mark.parametrize("tokens,experts,top", [(9001, 5, 2), (700, 1024, 3), (18000, 1, 1)])
+def test_many_slots(tokens, experts, top):
+    """More slots than a pass of the order takes, experts without a slot, one expert for all."""
+    x, ids, w, _ = make(tokens, experts, top, 8, 32, False, "bf16", tokens)
+    ids[::7, 0] = -1
+    run(x, ids, w, 8, 32, None, "f32", experts)
