@@ -310,8 +310,8 @@ NKB_API int nkb_angulars_packed_noalloc(uint32_t dtype, void const *a, void cons
  * current GPU (a call with one that does not is refused). On failure the outputs are filled with 0xFF bytes, i.e. NaN scales
  * and cells and ids of -1. `workspace` is device memory of at least the stated size on a 256-byte boundary that no
  * other call uses at the same time; with NULL the calling thread's staging memory is used, which allocates on first use and is
- * shared by everything the thread enqueues - captured graphs want a workspace of their own. (Products of one or two float rows need
- * none: they quantise inside.) The first product on each GPU
+ * shared by everything the thread enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own,
+ * for as long as it may run. (Products of one or two float rows need none: they quantise inside.) The first product on each GPU
  * allocates the device error word; make it before a capture starts.
  *
  * nkb_mx_quantise: per block with largest magnitude t the scale is 2^X, X = clamp(floor(log2 t) - 2, -127, 127); each value over

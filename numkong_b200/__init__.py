@@ -713,10 +713,19 @@ def _workspace(x: Any, nbytes: int):
     return buffer, (buffer.data_ptr() + 255) // 256 * 256
 
 
+def _array(x: Any) -> Any:
+    """A torch tensor (device arrays of other libraries come in through DLPack) or a NumPy array."""
+    if _is_torch(x) or isinstance(x, np.ndarray):
+        return x
+    x = _adopt_device_array(x)
+    if isinstance(x, _ForeignCuda):
+        raise TypeError("device arrays have to be torch tensors or speak DLPack here")
+    return x if _is_torch(x) else np.asarray(x)
+
+
 def _checked(x: Any, shape: Tuple[int, ...], names: Tuple[str, ...], what: str, like: Any = None):
     """`x` as a dense array of the given shape and one of the given types, where `like` lives."""
-    if not _is_torch(x):
-        x = np.asarray(x)
+    x = _array(x)
     name = _torch_name(x.dtype) if _is_torch(x) else x.dtype.name
     if name not in names or tuple(x.shape) != shape:
         raise ValueError(f"{what} must be {' or '.join(names)} of shape {shape}, got {name} of shape {tuple(x.shape)}")
@@ -728,7 +737,7 @@ def _checked(x: Any, shape: Tuple[int, ...], names: Tuple[str, ...], what: str, 
 
 
 def _float_view(x: Any, dtype: Optional[str], what: str) -> _View:
-    v = _View(x, dtype)
+    v = _View(_array(x), dtype)
     if v.dtype not in ("f32", "f16", "bf16"):
         raise TypeError(f"{what} takes f32, f16 or bf16, not {v.dtype!r}")
     return v
@@ -740,7 +749,7 @@ class MxMatrix:
 
     def __init__(self, codes: Any, scales: Any, depth: int):
         self.depth = int(depth)
-        c, s = _View(codes, "u8"), _View(scales, "u8")
+        c, s = _View(_array(codes), "u8"), _View(_array(scales), "u8")
         if c.cols != (self.depth + 1) // 2 or s.cols != (self.depth + 31) // 32 or c.rows != s.rows:
             raise ValueError(f"depth {self.depth} needs rows of {(self.depth + 1) // 2} code bytes and {(self.depth + 31) // 32} scale bytes")
         if _is_torch(c.obj) != _is_torch(s.obj) or (_is_torch(c.obj) and c.obj.device != s.obj.device):
@@ -866,6 +875,7 @@ def route_gradient(weights_grad: Any, ids: Any, logits: Any, *, score: str = "so
     v = _float_view(logits, dtype, "route_gradient")
     if score not in _SCORES:
         raise ValueError(f"score is 'softmax' or 'sigmoid', not {score!r}")
+    ids = _array(ids)
     top = int(ids.shape[-1])
     ids = _checked(ids, (v.rows, top), ("int32",), "ids", v.obj)
     weights_grad = _checked(weights_grad, (v.rows, top), ("float32",), "weights_grad", v.obj)
@@ -885,11 +895,12 @@ def experts_packed(x: Any, ids: Any, packed: PackedMatrix, *, weights: Any = Non
     token's choices, [tokens, width]."""
     if not isinstance(packed, PackedMatrix) or packed.dtype != "mxfp4":
         raise TypeError("experts_packed needs a matrix packed from an MxMatrix with groups")
-    if not _is_torch(ids):
-        ids = np.asarray(ids)
+    x, ids = _array(x), _array(ids)
     if len(ids.shape) != 2:
         raise ValueError("ids must be [tokens, top]")
     tokens, top = (int(n) for n in ids.shape)
+    if top == 0:
+        raise ValueError("every token has at least one choice")
     per_slot = len(x.shape) == 3
     if per_slot and tuple(x.shape[:2]) != (tokens, top) or not per_slot and x.shape[0] != tokens:
         raise ValueError(f"x must be [{tokens}, depth] or [{tokens}, {top}, depth]")

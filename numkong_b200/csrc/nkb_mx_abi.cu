@@ -5,7 +5,6 @@
 // on several streams and captured graphs need not share one; without it the calling thread's staging memory is used.
 #include <cstdio>
 #include <cstring>
-#include <vector>
 
 #include "../../include/numkong_b200.h"
 #include "nkb_host.h"
@@ -22,12 +21,12 @@ public:
     explicit Operands(cudaStream_t stream) : stream_(stream) { cudaGetDevice(&device_); }
     Operands(const Operands &) = delete;
     ~Operands() {
-        if (owned_.empty()) return;
+        if (!on_host()) return;
         cudaStreamSynchronize(stream_);
-        for (void *p : owned_) cudaFree(p);
+        for (int i = 0; i < owned_count_; ++i) cudaFree(owned_[i]);
         cudaGetLastError();
     }
-    bool on_host() const { return !owned_.empty(); }
+    bool on_host() const { return owned_count_ != 0; }
 
     // An input of `rows` rows of `row_bytes`, `stride` apart; a host matrix is uploaded with its rows packed 16-byte aligned.
     const uint8_t *in(const void *p, uint64_t rows, uint64_t row_bytes, uint64_t &stride) {
@@ -45,7 +44,7 @@ public:
         const uint64_t pitch = round_up(row_bytes, 16);
         uint8_t *d = allocate(rows * pitch);
         if (!d) return nullptr;
-        results_.push_back({p, d, rows, row_bytes, stride < row_bytes ? row_bytes : stride, pitch});
+        results_[result_count_++] = {p, d, rows, row_bytes, stride < row_bytes ? row_bytes : stride, pitch};
         stride = pitch;
         return d;
     }
@@ -61,8 +60,10 @@ public:
 
     // Copies host results back and waits for them, when the call had a host operand.
     bool finish(const char *what) {
-        for (const Result &r : results_)
+        for (int i = 0; i < result_count_; ++i) {
+            const Result &r = results_[i];
             if (!cuda_ok(cudaMemcpy2DAsync(r.host, r.stride, r.device, r.pitch, r.row_bytes, r.rows, cudaMemcpyDeviceToHost, stream_), "download of result")) return false;
+        }
         if (!on_host()) return true;
         if (!cuda_ok(cudaStreamSynchronize(stream_), what)) return false;
         const uint32_t w = read_device_error();
@@ -90,29 +91,42 @@ private:
     uint8_t *allocate(uint64_t bytes) {
         void *p = nullptr;
         if (!cuda_ok(cudaMalloc(&p, bytes ? bytes : 16), "cudaMalloc(operand)")) return nullptr;
-        owned_.push_back(p);
+        owned_[owned_count_++] = p;
         return static_cast<uint8_t *>(p);
     }
     cudaStream_t stream_;
     int device_ = 0;
     bool on_device_ = false;
-    std::vector<void *> owned_;
-    std::vector<Result> results_;
+    void *owned_[6];  // no call has more operands, nor more than two results
+    Result results_[2];
+    int owned_count_ = 0, result_count_ = 0;
 };
 
 void refuse(const char *why) { set_error("%s", why); }
 
-// What an output holds after a refused or failed call: 0xFF bytes (NaN scales and cells, ids of -1).
+constexpr uint64_t kMostRows = 0x7fffff00ull;  // indices inside the kernels are 32 bits wide
+
+// What an output holds after a refused or failed call: 0xFF bytes (NaN scales and cells, ids of -1), no more of them than the caller's
+// sizes and stride span. Sizes that no kernel takes are not believed.
 void spoil(void *out, uint64_t rows, uint64_t row_bytes, uint64_t stride) {
-    fill_error_output(out, classify(out), rows, row_bytes, stride < row_bytes ? row_bytes : stride);
+    if (!out || rows == 0 || rows > kMostRows || row_bytes > 4 * kMostRows) return;
+    if (stride < row_bytes) fill_error_output(out, classify(out), 1, (rows - 1) * stride + row_bytes, (rows - 1) * stride + row_bytes);
+    else fill_error_output(out, classify(out), rows, row_bytes, stride);
 }
 
 uint64_t chunk_bytes(uint64_t rows, uint64_t depth) { return mx_geometry(1, rows, depth).row_blocks * mx_geometry(1, rows, depth).depth_blocks * kMxChunkBytes; }
 
-constexpr uint64_t kMostRows = 0x7fffff00ull;  // indices inside the kernels are 32 bits wide
-
 uint8_t *workspace_or_scratch(Operands &ops, void *workspace, uint64_t bytes) {
-    if (!workspace) return static_cast<uint8_t *>(scratch(kSlotA, bytes));
+    if (!workspace) {
+        // Replays of two graphs may run at the same time, and a graph outlives what the thread's staging memory is next used for.
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (!cuda_ok(cudaStreamIsCapturing(current_stream(), &capture), "cudaStreamIsCapturing")) return nullptr;
+        if (capture != cudaStreamCaptureStatusNone) {
+            refuse("a call that is captured into a graph needs a workspace of its own");
+            return nullptr;
+        }
+        return static_cast<uint8_t *>(scratch(kSlotA, bytes));
+    }
     MemKind kind;
     if (!ops.look(workspace, kind)) return nullptr;
     if (kind != kMemDevice || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
@@ -145,13 +159,13 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
              const void *packed, void *c, uint32_t c_type, uint64_t m, uint64_t n, uint64_t k, uint64_t c_stride, void *workspace) {
     clear_error();
     if (m == 0 || n == 0) return;
-    const uint32_t cell = c_type == kF32 ? 4 : 2;
+    if (m > kMostRows || n > kMostRows || k > kMostRows) return refuse("mxfp4 product: a size does not fit 31 bits");
+    const uint32_t cell = dtype_bytes(c_type);
     const uint64_t row_bytes = n * cell;
-    auto fail = [&]() { if (c) spoil(c, m, row_bytes, c_stride); };
+    auto fail = [&]() { spoil(c, m, row_bytes, c_stride); };
     if ((c_type != kF32 && c_type != kBF16) || (!codes && !float_type(a_type))) { refuse("mxfp4 product: unsupported element type"); return fail(); }
     if (!packed || !c || (k && !(codes ? scales != nullptr : a != nullptr))) { refuse("mxfp4 product: null pointer"); return fail(); }
-    if (m > kMostRows || n > kMostRows || k > kMostRows) { refuse("mxfp4 product: a size does not fit 31 bits"); return fail(); }
-    if ((m > 1 && c_stride < row_bytes) || (reinterpret_cast<uintptr_t>(c) | c_stride) % cell) { refuse("mxfp4 product: rows of the result overlap or are not aligned to its cells"); return fail(); }
+    if ((m > 1 && c_stride < row_bytes) || (reinterpret_cast<uintptr_t>(c) | (m > 1 ? c_stride : 0)) % cell) { refuse("mxfp4 product: rows of the result overlap or are not aligned to its cells"); return fail(); }
     const uint64_t kblocks = (k + kMxBlock - 1) / kMxBlock;
     if (m > 1 && (codes ? codes_stride < (k + 1) / 2 || scales_stride < kblocks : a_stride < k * dtype_bytes(a_type))) { refuse("mxfp4 product: rows of A overlap"); return fail(); }
     if (!codes && (reinterpret_cast<uintptr_t>(a) | (m > 1 ? a_stride : 0)) % dtype_bytes(a_type)) { refuse("mxfp4 product: values of A are not aligned to their type"); return fail(); }
@@ -211,15 +225,15 @@ NKB_API void nkb_mx_quantise(void const *x, uint32_t x_type, nk_size_t rows, nk_
                              nk_size_t codes_stride, void *scales, nk_size_t scales_stride) {
     clear_error();
     if (rows == 0 || depth == 0) return;
+    if (rows > kMostRows || depth > kMostRows) return refuse("mx_quantise: a size does not fit 31 bits");
     const uint64_t code_bytes = (depth + 1) / 2, blocks = (depth + kMxBlock - 1) / kMxBlock;
     auto fail = [&]() {
-        if (codes) spoil(codes, rows, code_bytes, codes_stride);
-        if (scales) spoil(scales, rows, blocks, scales_stride);
+        spoil(codes, rows, code_bytes, codes_stride);
+        spoil(scales, rows, blocks, scales_stride);
     };
     if (!float_type(x_type) || !x || !codes || !scales) { refuse("mx_quantise: unsupported element type or null pointer"); return fail(); }
-    if (rows > kMostRows || depth > kMostRows) { refuse("mx_quantise: a size does not fit 31 bits"); return fail(); }
     if (rows > 1 && (x_stride < depth * dtype_bytes(x_type) || codes_stride < code_bytes || scales_stride < blocks)) { refuse("mx_quantise: rows overlap"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(x) | x_stride) % dtype_bytes(x_type)) { refuse("mx_quantise: values are not aligned to their type"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | (rows > 1 ? x_stride : 0)) % dtype_bytes(x_type)) { refuse("mx_quantise: values are not aligned to their type"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *xd = ops.in(x, rows, depth * dtype_bytes(x_type), x_stride);
@@ -233,14 +247,14 @@ NKB_API void nkb_mx_dequantise(void const *codes, nk_size_t codes_stride, void c
                                nk_size_t depth, void *x, uint32_t x_type, nk_size_t x_stride) {
     clear_error();
     if (rows == 0 || depth == 0) return;
+    if (rows > kMostRows || depth > kMostRows) return refuse("mx_dequantise: a size does not fit 31 bits");
     const uint64_t code_bytes = (depth + 1) / 2, blocks = (depth + kMxBlock - 1) / kMxBlock;
-    if (!float_type(x_type)) { refuse("mx_dequantise: unsupported element type"); return; }
     const uint64_t row_bytes = depth * dtype_bytes(x_type);
-    auto fail = [&]() { if (x) spoil(x, rows, row_bytes, x_stride); };
+    auto fail = [&]() { spoil(x, rows, row_bytes, x_stride); };
+    if (!float_type(x_type)) { refuse("mx_dequantise: unsupported element type"); return fail(); }
     if (!x || !codes || !scales) { refuse("mx_dequantise: null pointer"); return fail(); }
-    if (rows > kMostRows || depth > kMostRows) { refuse("mx_dequantise: a size does not fit 31 bits"); return fail(); }
     if (rows > 1 && (x_stride < row_bytes || codes_stride < code_bytes || scales_stride < blocks)) { refuse("mx_dequantise: rows overlap"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(x) | x_stride) % dtype_bytes(x_type)) { refuse("mx_dequantise: values are not aligned to their type"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | (rows > 1 ? x_stride : 0)) % dtype_bytes(x_type)) { refuse("mx_dequantise: values are not aligned to their type"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *cd = ops.in(codes, rows, code_bytes, codes_stride), *sd = cd ? ops.in(scales, rows, blocks, scales_stride) : nullptr;
@@ -257,13 +271,13 @@ NKB_API nk_size_t nkb_dots_packed_size_mxfp4(nk_size_t groups, nk_size_t width, 
 NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride, nk_size_t groups,
                                  nk_size_t width, nk_size_t depth, void *packed) {
     clear_error();
-    if (!packed) { refuse("mxfp4 pack: null output"); return; }
+    if (!packed) return refuse("mxfp4 pack: null output");
+    if (groups > kMostRows || width > kMostRows || depth > kMostRows || mx_geometry(groups, width, depth).row_blocks * kChunkRows > kMostRows) return refuse("mxfp4 pack: a size does not fit 31 bits");
     const MxGeometry g = mx_geometry(groups, width, depth);
     const uint64_t rows = groups * width, code_bytes = (depth + 1) / 2, blocks = (depth + kMxBlock - 1) / kMxBlock;
     const MemKind out_kind = classify(packed);
-    auto fail = [&]() { spoil(packed, 1, g.total_bytes, g.total_bytes); };
+    auto fail = [&]() { fill_error_output(packed, out_kind, 1, g.total_bytes, g.total_bytes); };
     if (rows && depth && (!codes || !scales)) { refuse("mxfp4 pack: null input"); return fail(); }
-    if (groups > kMostRows || width > kMostRows || depth > kMostRows || g.row_blocks * kChunkRows > kMostRows) { refuse("mxfp4 pack: a size does not fit 31 bits"); return fail(); }
     if (rows > 1 && (codes_stride < code_bytes || scales_stride < blocks)) { refuse("mxfp4 pack: rows overlap"); return fail(); }
     if (out_kind == kMemDevice && (reinterpret_cast<uintptr_t>(packed) & 15u)) { refuse("pack: device output must be 16-byte aligned"); return; }
     PackedHeader h;
@@ -302,7 +316,12 @@ NKB_API nk_size_t nkb_dots_workspace_mxfp4(nk_size_t height, nk_size_t depth) { 
 
 NKB_API void nkb_dots_packed_mxfp4(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride, void const *b_packed,
                                    void *c, uint32_t c_type, nk_size_t height, nk_size_t width, nk_size_t depth, nk_size_t c_stride, void *workspace) {
-    if (!codes) { clear_error(); refuse("mxfp4 product: null pointer"); if (c) spoil(c, height, width * (c_type == kF32 ? 4 : 2), c_stride); return; }
+    if (!codes) {
+        clear_error();
+        refuse("mxfp4 product: null pointer");
+        if (width <= kMostRows) spoil(c, height, width * dtype_bytes(c_type), c_stride);
+        return;
+    }
     product(nullptr, 0, 0, codes, codes_stride, scales, scales_stride, b_packed, c, c_type, height, width, depth, c_stride, workspace);
 }
 
@@ -315,15 +334,16 @@ NKB_API void nkb_route(void const *logits, uint32_t type, nk_size_t tokens, nk_s
                        uint32_t score, nk_size_t groups, nk_size_t top_groups, nk_size_t top, int renormalise, float scale, float *weights, int32_t *ids) {
     clear_error();
     if (tokens == 0) return;
+    if (tokens > kMostRows) return refuse("route: the tokens do not fit 31 bits");
     auto fail = [&]() {
-        if (weights) spoil(weights, 1, tokens * top * 4, 0);
-        if (ids) spoil(ids, 1, tokens * top * 4, 0);
+        spoil(weights, tokens, top * 4, top * 4);
+        spoil(ids, tokens, top * 4, top * 4);
     };
-    if (top == 0 || top > kRouteMaxTop || experts == 0 || experts > kRouteMaxExperts || top > experts) { refuse("route: 1 to 32 choices of 1 to 1024 experts"); if (top && top <= kRouteMaxTop) fail(); return; }
+    if (top == 0 || top > kRouteMaxTop || experts == 0 || experts > kRouteMaxExperts || top > experts) { refuse("route: 1 to 32 choices of 1 to 1024 experts"); return top <= kRouteMaxTop ? fail() : void(); }
     if (!float_type(type) || score > 1 || !logits || !weights || !ids) { refuse("route: unsupported element type or score, or null pointer"); return fail(); }
     if (groups == 0 || groups > kRouteMaxGroups || experts % groups || top_groups == 0 || top_groups > groups) { refuse("route: up to 32 groups of equal size, of which at least one and at most all are open"); return fail(); }
-    if (tokens > kMostRows || (tokens > 1 && logits_stride < experts * dtype_bytes(type))) { refuse("route: rows overlap or are too many"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(logits) | logits_stride) % dtype_bytes(type) || (reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(ids)) % 4) { refuse("route: operands are not aligned to their elements"); return fail(); }
+    if (tokens > 1 && logits_stride < experts * dtype_bytes(type)) { refuse("route: rows overlap"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(logits) | (tokens > 1 ? logits_stride : 0)) % dtype_bytes(type) || (reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(ids)) % 4) { refuse("route: operands are not aligned to their elements"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     RouteArgs a;
@@ -344,11 +364,12 @@ NKB_API void nkb_route_gradient(float const *weights_grad, int32_t const *ids, v
                                 nk_size_t logits_stride, uint32_t score, nk_size_t top, int renormalise, float scale, float *logits_grad) {
     clear_error();
     if (tokens == 0) return;
-    auto fail = [&]() { if (logits_grad && experts <= kRouteMaxExperts) spoil(logits_grad, 1, tokens * experts * 4, 0); };
+    if (tokens > kMostRows) return refuse("route_gradient: the tokens do not fit 31 bits");
+    auto fail = [&]() { if (experts <= kRouteMaxExperts) spoil(logits_grad, tokens, experts * 4, experts * 4); };
     if (top == 0 || top > kRouteMaxTop || experts == 0 || experts > kRouteMaxExperts) { refuse("route_gradient: 1 to 32 choices of 1 to 1024 experts"); return fail(); }
     if (!float_type(type) || score > 1 || !logits || !weights_grad || !ids || !logits_grad) { refuse("route_gradient: unsupported element type or score, or null pointer"); return fail(); }
-    if (tokens > kMostRows || (tokens > 1 && logits_stride < experts * dtype_bytes(type))) { refuse("route_gradient: rows overlap or are too many"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(logits) | logits_stride) % dtype_bytes(type) || (reinterpret_cast<uintptr_t>(weights_grad) | reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(logits_grad)) % 4) { refuse("route_gradient: operands are not aligned to their elements"); return fail(); }
+    if (tokens > 1 && logits_stride < experts * dtype_bytes(type)) { refuse("route_gradient: rows overlap"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(logits) | (tokens > 1 ? logits_stride : 0)) % dtype_bytes(type) || (reinterpret_cast<uintptr_t>(weights_grad) | reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(logits_grad)) % 4) { refuse("route_gradient: operands are not aligned to their elements"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     RouteArgs a;
@@ -373,17 +394,17 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
                                       void const *b_packed, nk_size_t experts, nk_size_t width, nk_size_t depth, float const *weights, void *out,
                                       uint32_t out_type, nk_size_t out_stride, void *workspace) {
     clear_error();
-    if (tokens == 0 || top == 0 || width == 0) return;
+    if (tokens == 0 || width == 0) return;
+    if (tokens > kMostRows || top == 0 || top > 1024 || tokens * top > kMostRows / 2 || width > kMostRows || depth > kMostRows) return refuse("experts: 1 to 1024 choices, and sizes that fit 31 bits");
     const uint64_t slots = tokens * top, rows = weights ? tokens : slots, x_rows = per_slot ? slots : tokens;
-    const uint32_t cell = out_type == kF32 ? 4 : 2;
+    const uint32_t cell = dtype_bytes(out_type);
     const uint64_t row_bytes = width * cell;
-    auto fail = [&]() { if (out) spoil(out, rows, row_bytes, out_stride); };
+    auto fail = [&]() { spoil(out, rows, row_bytes, out_stride); };
     if (!float_type(x_type) || (out_type != kF32 && out_type != kBF16)) { refuse("experts: unsupported element type"); return fail(); }
     if (!ids || !b_packed || !out || (depth && !x)) { refuse("experts: null pointer"); return fail(); }
     if (experts == 0 || experts > kRouteMaxExperts) { refuse("experts: 1 to 1024 experts"); return fail(); }
-    if (tokens > kMostRows || top > 1024 || slots > kMostRows / 2 || width > kMostRows || depth > kMostRows) { refuse("experts: a size does not fit 31 bits"); return fail(); }
     if ((x_rows > 1 && x_stride < depth * dtype_bytes(x_type)) || (rows > 1 && out_stride < row_bytes)) { refuse("experts: rows overlap"); return fail(); }
-    if ((reinterpret_cast<uintptr_t>(x) | (x_rows > 1 ? x_stride : 0)) % dtype_bytes(x_type) || (reinterpret_cast<uintptr_t>(out) | out_stride) % cell || (reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) % 4) { refuse("experts: operands are not aligned to their elements"); return fail(); }
+    if ((reinterpret_cast<uintptr_t>(x) | (x_rows > 1 ? x_stride : 0)) % dtype_bytes(x_type) || (reinterpret_cast<uintptr_t>(out) | (rows > 1 ? out_stride : 0)) % cell || (reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) % 4) { refuse("experts: operands are not aligned to their elements"); return fail(); }
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(experts, width, depth);

@@ -163,3 +163,55 @@ def test_sizes_are_pure():
     assert lib.nkb_dots_workspace_mxfp4(129, 257) == 2 * 2 * 17408
     assert lib.nkb_experts_workspace_mxfp4(4, 2, 8, 64, 256, 1) >= 8 * 17408 + 8 * 64 * 4
     assert lib.nkb_experts_workspace_mxfp4(4, 2, 8, 64, 256, 0) < lib.nkb_experts_workspace_mxfp4(4, 2, 8, 64, 256, 1)
+
+
+def test_refusals_stay_inside_what_sizes_and_strides_span():
+    """Rows that overlap are filled as far as the caller's stride reaches, sizes that nothing takes are not believed."""
+    held = np.zeros(4096, np.uint8)
+    x, codes, scales, ids = np.zeros((4, 64), np.float32), np.zeros((4, 32), np.uint8), np.zeros((4, 2), np.uint8), np.zeros((4, 1), np.int32)
+    p = lambda a: a.ctypes.data
+    blob, experts = packed(50, 64).buffer, packed(50, 64, 3).buffer
+
+    def spans(call, last):
+        held[:] = 0
+        call()
+        assert nk.last_error()
+        assert (held[:last] == 255).all() and (held[last:] == 0).all()
+    spans(lambda: lib.nkb_dots_packed_mxfp4(p(codes), 32, p(scales), 2, p(blob), p(held), F32, 4, 50, 64, 100, None), 3 * 100 + 200)
+    spans(lambda: lib.nkb_dots_packed_mxfp4(p(codes), 32, p(scales), 2, p(blob), p(held), I8, 4, 50, 64, 50, None), 4 * 50)
+    spans(lambda: lib.nkb_experts_packed_mxfp4(p(x), F32, 256, 0, p(ids), 4, 1, p(experts), 3, 50, 64, None, p(held), F32, 100, None), 3 * 100 + 200)
+    spans(lambda: lib.nkb_mx_dequantise(p(codes), 32, p(scales), 2, 4, 64, p(held), F32, 64), 3 * 64 + 256)
+    spans(lambda: lib.nkb_mx_quantise(p(x), F32, 4, 64, 256, p(held), 16, p(scales), 2), 3 * 16 + 32)
+    huge = 2 ** 64 - 1
+    for size in (huge, 2 ** 31):
+        spans(lambda: lib.nkb_dots_packed_mxfp4(p(codes), 32, p(scales), 2, p(blob), p(held), F32, size, 50, 64, 200, None), 0)
+        spans(lambda: lib.nkb_dots_packed_mxfp4(None, 32, p(scales), 2, p(blob), p(held), F32, 4, size, 64, 200, None), 0)
+        spans(lambda: lib.nkb_dots_pack_mxfp4(p(codes), 32, p(scales), 2, 1, size, 64, p(held)), 0)
+        spans(lambda: lib.nkb_dots_pack_mxfp4(p(codes), 32, p(scales), 2, size, 4, 64, p(held)), 0)
+        spans(lambda: lib.nkb_mx_quantise(p(x), F32, size, 64, 256, p(held), 32, p(scales), 2), 0)
+        spans(lambda: lib.nkb_mx_dequantise(p(codes), 32, p(scales), 2, size, 64, p(held), F32, 256), 0)
+        spans(lambda: lib.nkb_route(p(x), F32, size, 64, 256, None, 0, 1, 1, 2, 1, 1.0, p(held), p(ids)), 0)
+        spans(lambda: lib.nkb_route(p(x), F32, 4, 64, 256, None, 0, 1, 1, size, 1, 1.0, p(held), p(ids)), 0)
+        spans(lambda: lib.nkb_route_gradient(p(x), p(ids), p(x), F32, size, 64, 256, 0, 2, 1, 1.0, p(held)), 0)
+        spans(lambda: lib.nkb_route_gradient(p(x), p(ids), p(x), F32, 4, size, 256, 0, 2, 1, 1.0, p(held)), 0)
+        spans(lambda: lib.nkb_experts_packed_mxfp4(p(x), F32, 256, 0, p(ids), size, 1, p(experts), 3, 50, 64, None, p(held), F32, 200, None), 0)
+        spans(lambda: lib.nkb_experts_packed_mxfp4(p(x), F32, 256, 0, p(ids), 4, size, p(experts), 3, 50, 64, None, p(held), F32, 200, None), 0)
+
+
+def test_no_choice_is_refused():
+    with pytest.raises(ValueError):
+        nk.experts_packed(np.zeros((3, 64), np.float32), np.zeros((3, 0), np.int32), packed(5, 64, 4), weights=np.zeros((3, 0), np.float32))
+
+
+class DeviceArray:
+    """What a library without DLPack offers for device memory."""
+    shape = (3, 64)
+    __cuda_array_interface__ = {"shape": (3, 64), "typestr": "<f4", "data": (256, False), "version": 3}
+
+
+def test_device_arrays_without_dlpack_are_refused():
+    ids = np.zeros((3, 2), np.int32)
+    for call in (lambda: nk.mx_quantise(DeviceArray()), lambda: nk.route(DeviceArray(), 2), lambda: nk.experts_packed(DeviceArray(), ids, packed(5, 64, 4)),
+                 lambda: nk.dots_packed(DeviceArray(), packed(5, 64)), lambda: nk.route_gradient(DeviceArray(), ids, np.zeros((3, 8), np.float32))):
+        with pytest.raises(TypeError):
+            call()
