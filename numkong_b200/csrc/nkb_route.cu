@@ -37,7 +37,7 @@ __device__ __forceinline__ float load_logit(const uint8_t *row, uint32_t e) {
     float v;
     if constexpr (kType == kF32) v = reinterpret_cast<const float *>(row)[e];
     else v = decode_bits<kType>(reinterpret_cast<const uint16_t *>(row)[e]);
-    return v == v ? fminf(v, FLT_MAX) : -INFINITY;  // NaN masks
+    return v == v ? fminf(v, FLT_MAX) + 0.0f : -INFINITY;  // NaN masks; -0 becomes 0
 }
 // -infinity bars the expert.
 __device__ __forceinline__ float load_bias(const float *bias, uint32_t e) {
@@ -109,7 +109,7 @@ __device__ __forceinline__ void load_logits(const uint8_t *row, uint32_t experts
             float v;
             if constexpr (kType == kF32) v = __uint_as_float(w[i]);
             else v = decode_bits<kType>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
-            l[i] = v == v ? fminf(v, FLT_MAX) : -INFINITY;
+            l[i] = v == v ? fminf(v, FLT_MAX) + 0.0f : -INFINITY;
         }
     } else {
 #pragma unroll
@@ -442,12 +442,13 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
     }
     const uint64_t token = first + place;
     const float l = chosen_all >= 0 ? load_logit<kType>(p.logits + token * p.stride, chosen_all) : -INFINITY;
-    const bool near_zero = p.sigmoid && __any_sync(0xffffffffu, chosen_all >= 0 && l < -80.0f);
+    const uint32_t small = p.sigmoid ? __ballot_sync(0xffffffffu, chosen_all >= 0 && l < -80.0f) : 0u;
+    const bool near_zero = ((small >> (place * width)) & (0xffffffffu >> (32 - width))) != 0;  // in this token
     double w = 0.0;
     if (p.renormalise) {
         // Scores as they are while they can be represented, ratios from differences of logarithms where they vanish.
         float largest = l;
-        if (!p.sigmoid || near_zero)
+        if (!p.sigmoid || small != 0)
             for (uint32_t o = 1; o < width; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         if (chosen_all >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
         double sum = w;
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
             for (uint32_t i = lane; i < here * padded / 4; i += 32) reinterpret_cast<float4 *>(lines)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         double d = 0.0;  // what this slot's logit gets through the slot itself
-        const bool near_limit = p.sigmoid && __any_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f);
+        const bool near_limit = p.sigmoid && ((__ballot_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f) >> (place * width)) & (0xffffffffu >> (32 - width))) != 0;
         if (p.renormalise) {
             float most = l;
             for (uint32_t o = 1; o < width; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));

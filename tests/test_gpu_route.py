@@ -218,3 +218,33 @@ def test_route_strides_and_host():
     assert np.array_equal(host[0], want[0].cpu().numpy()) and np.array_equal(host[1], want[1].cpu().numpy())
     grad = nk.route_gradient(host[0], host[1], x)
     assert np.array_equal(grad, nk.route_gradient(want[0], want[1], wide[:, 3:73]).cpu().numpy())
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("experts,top", [(2, 1), (40, 3), (300, 32)])
+def test_zeros_of_either_sign_tie(experts, top, name):
+    logits = torch.zeros(3, experts, dtype=TORCH[name], device="cuda")
+    logits[0, ::2] = -0.0
+    logits[1, 1::2] = -0.0
+    _, ids = nk.route(logits, top)
+    assert (ids.cpu() == torch.arange(top)).all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_tokens_do_not_depend_on_one_another(score, renormalise):
+    """The same bits for a token alone, in a batch, and beside tokens whose scores almost vanish."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits = 3 * torch.randn(5000, 48, generator=g, device="cuda")
+    logits[1::4] -= 95
+    logits[2::4] += 95
+    how = dict(score=score, renormalise=renormalise)
+    weights, ids = nk.route(logits, 6, **how)
+    incoming = torch.randn(5000, 6, generator=g, device="cuda")
+    grad = nk.route_gradient(incoming, ids, logits, **how)
+    for first, count in ((0, 1), (4, 1), (8, 3), (1000, 700)):
+        part = logits[first:first + count]
+        some, chosen = nk.route(part, 6, **how)
+        assert torch.equal(some, weights[first:first + count]) and torch.equal(chosen, ids[first:first + count])
+        assert torch.equal(nk.route_gradient(incoming[first:first + count], chosen, part, **how), grad[first:first + count])
+    assert nk.synchronize() == 0
