@@ -55,17 +55,28 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-// The largest key of the warp and its index; the lower index where keys are equal.
+// The largest key of the warp and its index; the lower index where keys are equal. (No key is -0.)
 __device__ __forceinline__ void warp_best(double &key, uint32_t &index) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const double k = __shfl_xor_sync(0xffffffffu, key, o);
-        const uint32_t i = __shfl_xor_sync(0xffffffffu, index, o);
-        if (k > key || (k == key && i < index)) { key = k; index = i; }
-    }
+    const long long bits = __double_as_longlong(key);
+    const unsigned long long ordered = bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | (1ull << 63);
+    const uint32_t high = (uint32_t)(ordered >> 32), low = (uint32_t)ordered;
+    const uint32_t best_high = __reduce_max_sync(0xffffffffu, high), best_low = __reduce_max_sync(0xffffffffu, high == best_high ? low : 0u);
+    index = __reduce_min_sync(0xffffffffu, high == best_high && low == best_low ? index : 0xffffffffu);
+    const unsigned long long best = ((unsigned long long)best_high << 32) | best_low;
+    key = __longlong_as_double((long long)(best >> 63 ? best & ~(1ull << 63) : ~best));
 }
 __device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
 __device__ __forceinline__ double log_sigmoid(double l) { return fmin(l, 0.0) - log1p(exp(-fabs(l))); }
+
+// A selected or doubtful expert's score in 64 bits, and the ratio of two sigmoids that vanish. The paths that need them are taken
+// rarely, so that what they cost is the fetching of their instructions: one copy of each, outside the loops.
+__device__ __noinline__ double exact_score(bool sigmoid, float l, float top_logit, double total) {
+    const double e = exp(sigmoid ? -(double)l : (double)l - top_logit);
+    return (sigmoid ? 1.0 : e) / (sigmoid ? 1.0 + e : total);
+}
+__device__ __noinline__ double small_sigmoid(float l, float largest) {
+    return largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
+}
 
 // exp(a - b) for a <= b in f32, the rounding of the difference made good for.
 __device__ __forceinline__ float exp_difference(float a, float b) {
@@ -137,20 +148,23 @@ __device__ __forceinline__ void sort_descending(uint32_t (&v)[kCount]) {
 
 // The choice in 64 bits, for the tokens whose keys 32 bits leave undecided. `keys`: room for one key per expert. Returns lane j's choice.
 template <uint32_t kType>
-__device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, float top_logit, double *keys, int lane) {
+__device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, double *keys, int lane) {
     const bool direct = p.bias == nullptr && p.groups == 1;  // scores grow with their logits
     double total = 0.0;
+    float top_logit = -INFINITY;
     if (!p.sigmoid && !direct) {
+        for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
+        top_logit = warp_max(top_logit);
         for (uint32_t e = lane; e < p.experts; e += 32) {
             const float l = load_logit<kType>(row, e);
-            if (l > -INFINITY) total += exp((double)l - top_logit);
+            if (l > -INFINITY) total += exact_score(false, l, top_logit, 1.0);
         }
         total = warp_sum(total);
     }
     for (uint32_t e = lane; e < p.experts; e += 32) {
         const float l = load_logit<kType>(row, e), b = load_bias(p.bias, e);
         if (direct) keys[e] = l;
-        else keys[e] = l > -INFINITY && b > -INFINITY ? (p.sigmoid ? sigmoid64(l) : exp((double)l - top_logit) / total) + b : -INFINITY;
+        else keys[e] = l > -INFINITY && b > -INFINITY ? exact_score(p.sigmoid, l, top_logit, total) + b : -INFINITY;
     }
     __syncwarp();
     if (p.groups > 1) {
@@ -192,9 +206,9 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     return chosen;
 }
 
-// Puts one token's choices (lane j: the j-th) in order by their keys in 64 bits, ties to the lower index.
+// The `top` best of `count` candidates (one per lane) by their keys in 64 bits, in order, ties to the lower index. Returns lane j's choice.
 template <uint32_t kType>
-__device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *row, int32_t chosen, int lane) {
+__device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *row, int32_t chosen, uint32_t count, int32_t *places, int lane) {
     const bool direct = p.bias == nullptr && p.groups == 1;
     double total = 1.0;
     float top_logit = 0.0f;
@@ -203,29 +217,63 @@ __device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *
         for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
         top_logit = warp_max(top_logit);
         total = 0.0;
-#pragma unroll 4
-        for (uint32_t e = lane; e < p.experts; e += 32) total += exp((double)load_logit<kType>(row, e) - top_logit);
+#pragma unroll 1
+        for (uint32_t e = lane; e < p.experts; e += 32) total += exact_score(false, load_logit<kType>(row, e), top_logit, 1.0);
         total = warp_sum(total);
     }
     double key = -INFINITY;
     if (chosen >= 0) {
         const float l = load_logit<kType>(row, chosen);
-        key = direct ? (double)l : (p.sigmoid ? sigmoid64(l) : exp((double)l - top_logit) / total) + load_bias(p.bias, chosen);
+        key = direct ? (double)l : exact_score(p.sigmoid, l, top_logit, total) + load_bias(p.bias, chosen);
     }
     uint32_t rank = 0;
-    for (uint32_t i = 0; i < p.top; ++i) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < count; ++i) {
         const double other = __shfl_sync(0xffffffffu, key, i);
         const int32_t who = __shfl_sync(0xffffffffu, chosen, i);
         rank += who >= 0 && (other > key || (other == key && who < chosen));
     }
-    int32_t result = -1;
-    for (uint32_t j = 0; j < p.top; ++j) {
-        const uint32_t holder = __ballot_sync(0xffffffffu, chosen >= 0 && rank == j);
-        if (holder == 0) break;
-        const int32_t who = __shfl_sync(0xffffffffu, chosen, __ffs(holder) - 1);
-        if (lane == (int)j) result = who;
+    places[lane] = -1;
+    __syncwarp();
+    if (chosen >= 0) places[rank] = chosen;
+    __syncwarp();
+    return lane < (int)p.top ? places[lane] : -1;
+}
+
+// The choice where the last place is in question: everyone in an open group whose 32-bit key is not below `threshold` takes a lane, and
+// those are put in order in 64 bits. -2 in all lanes where they are more than 32.
+template <uint32_t kType, uint32_t kIndexBits>
+__device__ __noinline__ int32_t choose_near(const RouteDev &p, const uint8_t *row, uint32_t threshold, uint32_t open_groups, float least, float per_key, int32_t *places, int lane) {
+    const bool direct = p.bias == nullptr && p.groups == 1;
+    const uint32_t size = p.experts / p.groups;
+    float top_logit = 0.0f, scaled = per_key;
+    if (!direct && !p.sigmoid) {
+        float total = 0.0f;
+        top_logit = -INFINITY;
+        for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
+        top_logit = warp_max(top_logit);
+        for (uint32_t e = lane; e < p.experts; e += 32) total += expf(load_logit<kType>(row, e) - top_logit);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        scaled = __fdividef(per_key, total);
     }
-    return result;
+    uint32_t count = 0;
+    int32_t candidate = -1;
+    for (uint32_t base = 0; base < p.experts; base += 32) {
+        const uint32_t e = base + lane;
+        const float l = e < p.experts ? load_logit<kType>(row, e) : -INFINITY, b = e < p.experts ? load_bias(p.bias, e) : -INFINITY;
+        bool in = l > -INFINITY && b > -INFINITY && ((open_groups >> (e / size)) & 1u);
+        if (direct) in = in && (selection_key(l) >> kIndexBits) >= threshold;
+        else {
+            const float part = p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : expf(l - top_logit);
+            in = in && __float2uint_rz(fmaf(part, scaled, (b - least) * per_key)) + 1u >= threshold;
+        }
+        const uint32_t found = __ballot_sync(0xffffffffu, in), many = __popc(found);
+        if (count + many > 32) return -2;
+        if ((uint32_t)lane >= count && (uint32_t)lane < count + many) candidate = (int32_t)(base + __fns(found, 0, lane - count + 1));
+        count += many;
+    }
+    return order_exactly<kType>(p, row, candidate, count, places, lane);
 }
 
 // One warp per token; lane i holds the experts i * kPer .. in registers.
@@ -233,18 +281,23 @@ __device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *
 // A key and its expert share one 32-bit word: the key in fixed point above, 31 - e of the warp's width below, so that one integer
 // maximum over the warp finds the next choice and gives ties to the lower index. The fixed point comes from scores in 32 bits;
 // `slack` bounds, in its units, how far it is off. Where every decision (chosen against next, open group against closed) is wider
-// than that, or is a tie of equal inputs, the choice is the one 64 bits would make; otherwise the chosen ones
-// are put in order in 64 bits, or, where groups or the last place are in question, the whole choice is made there (choose_exactly). Keys that are the logits themselves (no bias, no groups) are the upper bits of their
+// than that, or is a tie of equal inputs, the choice is the one 64 bits would make; otherwise those that may
+// be chosen are put in order in 64 bits, or, where groups are in question, the whole choice is made there (choose_exactly). Keys that are the logits themselves (no bias, no groups) are the upper bits of their
 // order-preserving integers, exact for 16-bit logits.
 //
-// Bound by instructions, about 600 a token. 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token
-// in 64 bits, 38 us with 32-bit keys whose expert was looked up in every round.
+// 64 bits wait until a warp's batch is through: with the calls inside the loop its registers went to the stack around them.
+//
+// 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token in 64 bits, 38 us with 32-bit keys whose expert was
+// looked up in every round, 26 us now. 19 of these are about 700 instructions a token, a third of what the SMs can issue (the chain
+// of one maximum after the other; more warps with fewer registers each were no faster); the rest is the last warps' way through 64 bits.
+// Register bounds: 72 instead of 96 for eight keys a lane took 24 us to 20 without the 64-bit part, 64 was slower again.
 template <uint32_t kType, int kPer>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, float *weights, int32_t *ids) {
+__global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : kPer == 16 ? 4 : 2) route_kernel(const RouteDev p, float *weights, int32_t *ids) {
     constexpr uint32_t kIndexBits = kPer == 1 ? 5 : kPer == 2 ? 6 : kPer == 4 ? 7 : kPer == 8 ? 8 : kPer == 16 ? 9 : 10;
     constexpr bool kSorted = kPer <= 8;  // each lane keeps its keys in order; beyond that the network costs more than it saves
     constexpr uint32_t kWidth = 32 * kPer, kUnits = (1u << (32 - kIndexBits)) - 64;  // some room above for rounding
     extern __shared__ double keys_all[];
+    __shared__ int32_t places_all[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto expert_of = [](uint32_t word) { return kWidth - 1 - (word & (kWidth - 1)); };
     const bool direct = p.bias == nullptr && p.groups == 1;
@@ -278,6 +331,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
     double total_all = 1.0;
     float logit[kPer], next[kPer];
     load_logits<kType, kPer>(p.logits + first * p.stride, p.experts, lane, logit);
+    uint32_t unsure = 0;             // tokens of the batch that want 64 bits, and lane t: for the whole choice (0), the order of the chosen
+    uint32_t how = 0, among = 0;     // (all ones), or the choice from a threshold on, among these groups
     for (uint32_t t = 0; t < batch && first + t < p.tokens; ++t) {
         const uint8_t *row = p.logits + (first + t) * p.stride;
         if (t + 1 < batch && first + t + 1 < p.tokens) load_logits<kType, kPer>(row + p.stride, p.experts, lane, next);
@@ -287,7 +342,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
             top_logit = warp_max(top_logit);
         }
-        uint32_t key[kPer], slack = 0;
+        uint32_t key[kPer], slack = 0, open_groups = 1;
         const uint32_t last = kWidth - 1 - lane * kPer;
         if (direct) {
 #pragma unroll
@@ -363,7 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
             const uint32_t most_closed = __reduce_max_sync(0xffffffffu, open ? 0u : worth);
             // A worth is off by two keys' errors, halved, and its roundings.
             if (most_closed != 0 && least_open - most_closed <= 2 * slack + 4) sure = false;
-            const uint32_t open_groups = __ballot_sync(0xffffffffu, open);
+            open_groups = __ballot_sync(0xffffffffu, open);
             if (whole_lanes) {
                 if (!((open_groups >> (lane / lanes)) & 1u)) {
 #pragma unroll
@@ -409,23 +464,14 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
         bool ordered = !__any_sync(0xffffffffu, lane > 0 && undecided(before, word));
         if (p.top == 32) ordered = ordered && !undecided(__shfl_sync(0xffffffffu, word, 31), behind);
         int32_t chosen = word != 0 && lane < (int)p.top ? (int32_t)expert_of(word) : -1;
-        if (sure && !ordered) {
-            // Too near to one another, but clear of the expert behind the last: the chosen ones are put in order by their keys in 64 bits.
-            const uint32_t last_word = __shfl_sync(0xffffffffu, word, p.top - 1);
-            if (behind == 0 || (last_word >> kIndexBits) - (behind >> kIndexBits) > unsure_at) {
-                chosen = order_exactly<kType>(p, row, chosen, lane);
-                ordered = true;
+        if (!sure || !ordered) {
+            const uint32_t last = __shfl_sync(0xffffffffu, word, p.top - 1) >> kIndexBits;
+            const bool last_clear = behind == 0 || last - (behind >> kIndexBits) > unsure_at;
+            unsure |= 1u << t;
+            if (lane == (int)t) {
+                how = !sure ? 0u : last_clear ? 0xffffffffu : last > unsure_at + 2 ? last - unsure_at - 2 : 1u;
+                among = open_groups;
             }
-        }
-        sure = sure && ordered;
-        if (!sure) {
-            if (p.sigmoid) {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) top_logit = fmaxf(top_logit, logit[i]);
-                top_logit = warp_max(top_logit);
-            }
-            chosen = choose_exactly<kType>(p, row, top_logit, keys_all + (size_t)warp * p.experts, lane);
-            __syncwarp();
         }
         const int32_t mine_of = __shfl_sync(0xffffffffu, chosen, slot);
         if (place == t) chosen_all = mine_of;
@@ -440,6 +486,23 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
 #pragma unroll
         for (int i = 0; i < kPer; ++i) logit[i] = next[i];
     }
+    for (; unsure; unsure &= unsure - 1) {
+        const uint32_t t = __ffs(unsure) - 1, what = __shfl_sync(0xffffffffu, how, t), groups = __shfl_sync(0xffffffffu, among, t);
+        const uint8_t *row = p.logits + (first + t) * p.stride;
+        int32_t chosen = -2;
+        if (what == 0xffffffffu) {
+            chosen = __shfl_sync(0xffffffffu, chosen_all, t * width + (lane & (width - 1)));
+            chosen = order_exactly<kType>(p, row, lane < (int)p.top ? chosen : -1, p.top, places_all[warp], lane);
+        } else if (what != 0) {
+            chosen = choose_near<kType, kIndexBits>(p, row, what, groups, least, per_key, places_all[warp], lane);
+        }
+        if (__any_sync(0xffffffffu, chosen == -2)) {
+            chosen = choose_exactly<kType>(p, row, keys_all + (size_t)warp * p.experts, lane);
+            __syncwarp();
+        }
+        const int32_t mine_of = __shfl_sync(0xffffffffu, chosen, slot);
+        if (place == t) chosen_all = mine_of;
+    }
     const uint64_t token = first + place;
     const float l = chosen_all >= 0 ? load_logit<kType>(p.logits + token * p.stride, chosen_all) : -INFINITY;
     const uint32_t small = p.sigmoid ? __ballot_sync(0xffffffffu, chosen_all >= 0 && l < -80.0f) : 0u;
@@ -450,12 +513,12 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteDev p, fl
         float largest = l;
         if (!p.sigmoid || small != 0)
             for (uint32_t o = 1; o < width; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-        if (chosen_all >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : largest > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(largest));
+        if (chosen_all >= 0) w = !near_zero ? fast_score(p.sigmoid, l, largest) : small_sigmoid(l, largest);
         double sum = w;
         for (uint32_t o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (chosen_all >= 0) w *= sum > 1e-30 ? reciprocal(sum) : 1.0 / sum;
     } else if (p.sigmoid) {
-        if (chosen_all >= 0) w = near_zero ? sigmoid64(l) : fast_score(true, l, 0.0f);
+        if (chosen_all >= 0) w = near_zero ? small_sigmoid(l, 0.0f) : fast_score(true, l, 0.0f);
     } else if (chosen_all >= 0) {
         w = (double)exp_difference(l, top_all) * reciprocal(total_all);
     }
@@ -519,13 +582,13 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
             float most = l;
             for (uint32_t o = 1; o < width; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             double part = 0.0;
-            if (id >= 0) part = !near_limit ? fast_score(p.sigmoid, l, most) : most > -700.0f ? sigmoid64(l) : exp(log_sigmoid(l) - log_sigmoid(most));
+            if (id >= 0) part = !near_limit ? fast_score(p.sigmoid, l, most) : small_sigmoid(l, most);
             const double sum = over_slots(part), u = id >= 0 ? part * (sum > 1e-30 ? reciprocal(sum) : 1.0 / sum) : 0.0, mean = over_slots(g * u);
             d = u * (g - mean);
         } else if (id >= 0) {
-            d = p.sigmoid ? g * (near_limit ? sigmoid64(l) : fast_score(true, l, 0.0f)) : g * ((double)exp_difference(l, top_logit) * reciprocal(total));
+            d = p.sigmoid ? g * (near_limit ? small_sigmoid(l, 0.0f) : fast_score(true, l, 0.0f)) : g * ((double)exp_difference(l, top_logit) * reciprocal(total));
         }
-        if (p.sigmoid && id >= 0) d *= near_limit ? sigmoid64(-(double)l) : fast_score(true, -l, 0.0f);  // 1 - s
+        if (p.sigmoid && id >= 0) d *= near_limit ? small_sigmoid(-l, 0.0f) : fast_score(true, -l, 0.0f);  // 1 - s
         __syncwarp();
         if (dense) {
             const double spread = over_slots(d);
