@@ -1,7 +1,8 @@
-"""Synthetic twins of the two search workloads of the packed-contraction path, with device-side timing.
+"""Synthetic twins of the workloads of the packed-contraction path, with device-side timing.
 
     python -m numkong_b200.workloads nearest --queries 8192 --corpus 65536 --depth 768 --top 10 --dtype f16
     python -m numkong_b200.workloads maxsim  --queries 256 --docs 20000 --depth 128 --top 100
+    python -m numkong_b200.workloads experts --tokens 4096 --experts 32 --top 4 --depth 2048 --hidden 2048
     python -m torch.distributed.run --nnodes=1 --nproc-per-node 4 --master-addr 127.0.0.1 --master-port 29500 \
         -m numkong_b200.workloads nearest --queries 65536 --corpus 10000000 --sharded
 
@@ -13,6 +14,8 @@ number of ranks; sizes and distributions do not.
 `nearest`: L2-normalised N(0,1) queries against an L2-normalised corpus, angular top-k per query (the batched
 distance kernels + selection). `maxsim`: ColBERT-style late interaction, queries of 32 tokens against documents of
 64..300 tokens (uniform), L2-normalised N(0,1) token vectors in bf16, all-pairs MaxSim scores + top-k per query.
+`experts`: a layer of experts with 4-bit matrices: router
+product, routing, the experts' first product, SiLU, their second product and the weighted sum, N(0,1) tokens in bf16.
 Work is counted as 2 * rows * columns * depth (for MaxSim: query tokens x document tokens, unpadded), the
 definition the reference's benchmarks use (bench/bench.hpp:257, bench/bench_maxsim.cpp:60). One JSON line per run.
 """
@@ -145,6 +148,35 @@ def run_quantise(values: int, dtype: str = "e4m3", steps: int = 5, seed: int = 7
             "cast_ms": s_cast * 1e3, "cast_gbs": (values * 4 + out.numel()) / s_cast / 1e9}
 
 
+def run_experts(tokens: int, experts: int = 32, top: int = 4, depth: int = 2048, hidden: int = 2048, steps: int = 5, seed: int = 13, warmup: int = 2):
+    """A layer of experts on mxfp4 matrices, from the tokens to their sums, as one captured graph; tokens / s, and the rate of the
+    experts' two products over the whole layer's time."""
+    import torch
+    import numkong_b200 as nk
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+
+    def matrix(rows, columns, groups=1):
+        return nk.dots_pack(nk.mx_quantise(torch.randn((rows, columns), generator=gen, device="cuda") * columns ** -0.5), groups=groups)
+    x = torch.randn((tokens, depth), generator=gen, device="cuda").to(torch.bfloat16)
+    router, first, second = matrix(experts, depth), matrix(experts * hidden, depth, experts), matrix(experts * depth, hidden, experts)
+
+    def layer():
+        weights, ids = nk.route(nk.dots_packed(x, router), top)
+        h = torch.nn.functional.silu(nk.experts_packed(x, ids, first, out_dtype="bf16"))
+        return nk.experts_packed(h, ids, second, weights=weights, out_dtype="bf16")
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    s = _timed(torch, graph.replay, steps, warmup)
+    if nk.synchronize() or not bool(out.isfinite().all()):
+        raise RuntimeError("a layer of experts gave up or overflowed")
+    return {"workload": "experts", "tokens": tokens, "experts": experts, "top": top, "depth": depth, "hidden": hidden, "dtype": "mxfp4",
+            "ms": s * 1e3, "tokens_per_s": tokens / s, "tflops": 4 * tokens * top * depth * hidden / s / 1e12}
+
+
 class _SingleProcess:
     """Stands in for torch.distributed when the script runs as one plain process (one GPU, no launcher)."""
     ReduceOp = type("ReduceOp", (), {"MAX": None})
@@ -252,12 +284,15 @@ def run_maxsim_sharded(queries: int, docs: int, depth: int = 128, top: int = 100
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("workload", choices=["nearest", "maxsim", "quantise", "dense"])
+    ap.add_argument("workload", choices=["nearest", "maxsim", "quantise", "dense", "experts"])
     ap.add_argument("--op", default="dots", choices=["dots", "angulars", "euclideans"])
     ap.add_argument("--values", type=int, default=1 << 26)
     ap.add_argument("--queries", type=int, default=None)
     ap.add_argument("--corpus", type=int, default=65536)
     ap.add_argument("--docs", type=int, default=20000)
+    ap.add_argument("--tokens", type=int, default=4096)
+    ap.add_argument("--experts", type=int, default=32)
+    ap.add_argument("--hidden", type=int, default=2048)
     ap.add_argument("--depth", type=int, default=None)
     ap.add_argument("--top", type=int, default=None)
     ap.add_argument("--dtype", default="f16")
@@ -267,6 +302,8 @@ def main():
     a = ap.parse_args()
     if a.workload == "dense":
         out = run_dense(a.queries or 4096, a.corpus, a.depth or 4096, a.dtype, a.op, a.steps, warmup=a.warmup)
+    elif a.workload == "experts":
+        out = run_experts(a.tokens, a.experts, a.top or 4, a.depth or 2048, a.hidden, a.steps, warmup=a.warmup)
     elif a.workload == "quantise":
         out = run_quantise(a.values, a.dtype if a.dtype != "f16" else "e4m3", a.steps, warmup=a.warmup)
     elif a.workload == "nearest":

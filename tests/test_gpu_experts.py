@@ -152,3 +152,9 @@ def test_many_slots(tokens, experts, top):
     x, ids, w, _ = make(tokens, experts, top, 8, 32, False, "bf16", tokens)
     ids[::7, 0] = -1
     run(x, ids, w, 8, 32, None, "f32", experts)
+
+
+def test_the_workload_runs():
+    from numkong_b200.workloads import run_experts
+    out = run_experts(40, 6, 2, 192, 130, steps=2, warmup=1)
+    assert out["workload"] == "experts" and out["ms"] > 0 and out["tokens_per_s"] > 0
