@@ -38,6 +38,7 @@ struct MxGemmDev {
     uint32_t group_blocks;           // row blocks of 128 per packed matrix
     const MxRowTile *tiles;
     const int32_t *tile_count, *row_dest;
+    uint32_t tiles_fresh;            // the tiles are written by the kernel before, like A
     uint32_t a_row_major;            // A's codes are read from the caller's rows
     uint32_t a_blocks;               // row blocks A's buffers hold
     const uint8_t *x;                // float rows of A the kernel quantises itself, their stride, type and length
@@ -284,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    if (p.tiles_fresh) wait_for_previous_kernel();
     const uint32_t tiles_m = p.tile_count ? (uint32_t)*p.tile_count : p.tiles_m;
 
     // One loader for each operand: its scales four chunks at a time, its codes chunk by chunk.
@@ -530,6 +532,7 @@ gemm_mx_pair_kernel(const __grid_constant__ PairMaps maps, const MxGemmDev p) {
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    if (p.tiles_fresh) wait_for_previous_kernel();
     const uint32_t tiles_m = p.tile_count ? (uint32_t)*p.tile_count : p.tiles_m, num_tiles = tiles_m * p.tiles_n;
     if (threadIdx.x == 0) {
         prefetch_tensormap(&maps.a);
@@ -853,6 +856,7 @@ cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     dev.n = (uint32_t)args.n;
     dev.tiles = args.tiles;
     dev.tile_count = args.tile_count;
+    dev.tiles_fresh = args.tiles_fresh;
     dev.row_dest = args.row_dest;
     dev.x = static_cast<const uint8_t *>(args.x);
     dev.x_stride = args.x_stride;

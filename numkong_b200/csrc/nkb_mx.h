@@ -75,6 +75,7 @@ struct MxGemmArgs {
     const int32_t *row_dest = nullptr;
     uint64_t max_tiles = 0;            // row tiles there may be at most
     uint32_t tile_rows = 128;          // 256: CTA pairs
+    bool tiles_fresh = false;          // the kernel just before writes the tiles, too
     uint64_t groups = 1;
     unsigned int *error_word = nullptr;
 };
@@ -101,6 +102,12 @@ cudaError_t launch_route_gradient(const RouteArgs &args, const float *weights_gr
 // Row tiles of at most `tile_rows` slots of one expert each. `slots` ids; those outside [0, experts) choose none.
 cudaError_t launch_expert_order(const int32_t *ids, uint64_t slots, uint32_t experts, MxRowTile *tiles, int32_t *tile_count, int32_t *row_dest,
                                 uint64_t max_tiles, uint32_t tile_rows, cudaStream_t stream);
+// The same and the quantising of the slots' rows (x row slot / divide) in one launch, for at most kFewSlots slots; rows of `out`, where it is
+// not null, whose slot chooses no expert are zeroed.
+constexpr uint32_t kFewSlots = 256;
+cudaError_t launch_order_and_quantise(uint32_t type, const void *x, uint64_t depth, uint64_t x_stride, const int32_t *ids, uint32_t slots, uint32_t experts, uint32_t divide,
+                                      uint32_t tile_rows, uint64_t max_tiles, MxRowTile *tiles, int32_t *tile_count, int32_t *row_dest, void *out,
+                                      uint64_t row_bytes, uint64_t out_stride, void *chunks, cudaStream_t stream);
 // Zeros the rows of `out` whose slot chooses no expert.
 cudaError_t launch_zero_unrouted(const int32_t *ids, uint64_t slots, uint32_t experts, void *out, uint64_t row_bytes, uint64_t out_stride, cudaStream_t stream);
 // out[t] = sum over j of weights[t, j] * y[t * top + j], slots without an expert left out; f32 sums in order of j.

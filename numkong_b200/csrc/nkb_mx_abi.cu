@@ -433,12 +433,19 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
             args.c_bf16 = !weights && out_type == kBF16;
             args.m = slots; args.n = width; args.k = depth;
             args.tiles = tiles; args.tile_count = count; args.row_dest = dest; args.max_tiles = l.max_tiles; args.tile_rows = l.tile_rows; args.groups = experts; args.error_word = err;
-            ok = cuda_ok(launch_expert_order(id, slots, (uint32_t)experts, tiles, count, dest, l.max_tiles, l.tile_rows, stream), "expert order kernel") &&
-                 cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, x_rows > 1 ? x_stride : 0, l.max_tiles * l.tile_rows, dest, count, l.tile_rows, per_slot ? 1u : (uint32_t)top, ws + l.chunks, stream), "quantise kernel") &&
-                 cuda_ok(launch_gemm_mx(args, stream), "grouped mxfp4 GEMM kernel");
-            if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, (uint32_t)experts, width, dst, out_type == kBF16, out_stride, stream), "combine kernel");
-            else if (ok) ok = cuda_ok(launch_zero_unrouted(id, slots, (uint32_t)experts, dst, row_bytes, out_stride, stream), "zero kernel");
-            g_launches += 4;
+            const uint32_t divide = per_slot ? 1u : (uint32_t)top, n = (uint32_t)experts;
+            const uint64_t stride = x_rows > 1 ? x_stride : 0;
+            args.tiles_fresh = slots <= kFewSlots;
+            if (args.tiles_fresh)
+                ok = cuda_ok(launch_order_and_quantise(x_type, xd, depth, stride, id, (uint32_t)slots, n, divide, l.tile_rows, l.max_tiles, tiles, count, dest, weights ? nullptr : dst,
+                                                       row_bytes, out_stride, ws + l.chunks, stream), "order and quantise kernel");
+            else
+                ok = cuda_ok(launch_expert_order(id, slots, n, tiles, count, dest, l.max_tiles, l.tile_rows, stream), "expert order kernel") &&
+                     cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, stride, l.max_tiles * l.tile_rows, dest, count, l.tile_rows, divide, ws + l.chunks, stream), "quantise kernel");
+            ok = ok && cuda_ok(launch_gemm_mx(args, stream), "grouped mxfp4 GEMM kernel");
+            if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, n, width, dst, out_type == kBF16, out_stride, stream), "combine kernel");
+            else if (ok && !args.tiles_fresh) ok = cuda_ok(launch_zero_unrouted(id, slots, n, dst, row_bytes, out_stride, stream), "zero kernel");
+            g_launches += !args.tiles_fresh ? 4 : weights ? 3 : 2;
         }
     }
     if (ok && packed_kind == kMemHost && !ops.on_host()) ok = cuda_ok(cudaStreamSynchronize(stream), "experts");

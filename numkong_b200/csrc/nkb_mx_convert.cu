@@ -77,15 +77,120 @@ __device__ __forceinline__ void store_chunk_row(uint32_t codes, uint32_t row, ui
 //   shared memory
 // 8192 x 8192 bf16: 170 MB in 30 us where the copy rate allows 26; with one piece in flight 50 us.
 template <uint32_t kType, bool kTiled>
+__device__ __forceinline__ void quantise_piece(const uint8_t *row, const Piece &piece, uint64_t depth, bool aligned, const RowMajorSink &out, uint8_t *chunks,
+                                               uint8_t *scale_tiles, uint32_t depth_blocks, uint32_t ahead, uint8_t *staging, int lane) {
+    constexpr int kBytes = kType == kF32 ? 4 : 2;
+    const uint32_t count = min(ahead, depth_blocks - piece.kb0);
+    uint32_t my_scale = 0;  // lane i: the scale of block i % 8 of chunk row kb0 + i / 8
+    const uint64_t byte0 = (uint64_t)piece.kb0 * 128 + lane * 4;
+    uint8_t *to = kTiled ? chunks + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0) * kMxCodeBytes + (piece.row % kChunkRows) * 128u +
+                               ((((uint32_t)lane >> 2) ^ (piece.row & 7u)) << 4) + (lane & 3) * 4
+                         : out.codes + piece.row * out.codes_stride + byte0;
+    if (aligned && ahead == kAhead && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth && (kTiled || (out.codes_stride & 3u) == 0 && (reinterpret_cast<uintptr_t>(out.codes) & 3u) == 0)) {
+        // Whole pieces on their boundaries: nothing to guard.
+        const uint8_t *from8 = row + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
+        uint4 raw[kAhead][kBytes / 2];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int h = 0; h < kBytes / 2; ++h) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(from8 + u * kMxChunkValues * kBytes) + h);
+        uint32_t four = 0;  // this thread's block's scales in the four chunk rows
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float v[8];
+            uint32_t s;
+            const uint32_t largest = unpack8<kType>(raw[u], v);
+            *reinterpret_cast<uint32_t *>(to + u * (kTiled ? kMxCodeBytes : 128u)) = quantise8(v, largest, s);
+            four |= s << (8 * u);
+        }
+        my_scale = (__shfl_sync(0xffffffffu, four, (lane & 7) * 4) >> (lane & 24)) & 255u;
+    } else if (aligned) {
+        uint4 raw[kAhead][kBytes / 2];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint64_t first = (uint64_t)(piece.kb0 + u) * kMxChunkValues + lane * 8;
+#pragma unroll
+            for (int h = 0; h < kBytes / 2; ++h) {
+                raw[u][h] = make_uint4(0, 0, 0, 0);
+                if (first + 8 <= depth) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(row + first * kBytes) + h);
+            }
+            if (first < depth && first + 8 > depth) {  // the row ends inside
+                uint32_t w[2 * kBytes] = {};
+                for (int i = 0; i < (int)(depth - first); ++i) {
+                    if constexpr (kType == kF32) w[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + first + i);
+                    else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(row) + first + i) << (16 * (i & 1));
+                }
+#pragma unroll
+                for (int h = 0; h < kBytes / 2; ++h) raw[u][h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (u >= (int)count) break;
+            float v[8];
+            uint32_t s;
+            const uint32_t largest = unpack8<kType>(raw[u], v), codes = quantise8(v, largest, s);
+            store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
+            const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
+            if ((lane >> 3) == u) my_scale = mine;
+        }
+    } else {
+        uint32_t all[kAhead][8];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const uint64_t at = (uint64_t)(piece.kb0 + u) * kMxChunkValues + b * 32 + lane;
+                all[u][b] = 0;
+                if (u < (int)count && at < depth) {
+                    if constexpr (kType == kF32) all[u][b] = __ldg(reinterpret_cast<const uint32_t *>(row) + at);
+                    else all[u][b] = __ldg(reinterpret_cast<const uint16_t *>(row) + at);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (u >= (int)count) break;
+            __syncwarp();
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                if constexpr (kType == kF32) reinterpret_cast<uint32_t *>(staging)[b * 32 + lane] = all[u][b];
+                else reinterpret_cast<uint16_t *>(staging)[b * 32 + lane] = (uint16_t)all[u][b];
+            }
+            __syncwarp();
+            uint4 raw[kBytes / 2];
+#pragma unroll
+            for (int h = 0; h < kBytes / 2; ++h) raw[h] = reinterpret_cast<const uint4 *>(staging + lane * 8 * kBytes)[h];
+            float v[8];
+            uint32_t s;
+            const uint32_t largest = unpack8<kType>(raw, v), codes = quantise8(v, largest, s);
+            store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
+            const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
+            if ((lane >> 3) == u) my_scale = mine;
+        }
+    }
+    if constexpr (kTiled) {
+        // Four scales to a word of a scale tile, for which eight lanes of a chunk row hold two words.
+        uint32_t word = my_scale << (8 * (lane & 3));
+        word |= __shfl_xor_sync(0xffffffffu, word, 1);
+        word |= __shfl_xor_sync(0xffffffffu, word, 2);
+        const uint32_t u = (uint32_t)lane >> 3, r = piece.row % kChunkRows;
+        if ((lane & 3) == 0 && u < count)
+            *reinterpret_cast<uint32_t *>(scale_tiles + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0 + u) * kMxScaleBytes +
+                                          ((lane >> 2) & 1) * 512 + (r & 31u) * 16 + (r >> 5) * 4) = word;
+    } else {
+        const uint64_t block = (uint64_t)piece.kb0 * 8 + lane;
+        if (block * kMxBlock < depth && (uint32_t)(lane >> 3) < count) out.scales[piece.row * out.scales_stride + block] = (uint8_t)my_scale;
+    }
+}
+
+template <uint32_t kType, bool kTiled>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, uint32_t rows, uint64_t depth, uint64_t x_stride, RowMajorSink out,
                                                             uint8_t *chunks, uint8_t *scale_tiles, uint32_t depth_blocks, const int32_t *row_dest,
                                                             const int32_t *tile_count, uint32_t tile_rows, uint32_t divide, uint32_t ahead) {
     if constexpr (kTiled) allow_next_kernel();  // the product that reads the chunks may set itself up meanwhile
-    constexpr int kBytes = kType == kF32 ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0;
-    __shared__ __align__(16) uint8_t staging_all[kThreads / 32][kMxChunkValues * kBytes];
-    uint8_t *staging = staging_all[threadIdx.x >> 5];
+    __shared__ __align__(16) uint8_t staging_all[kThreads / 32][kMxChunkValues * (kType == kF32 ? 4 : 2)];
     const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = rows * pieces_per_row;
     const uint32_t used = kTiled && row_dest ? (uint32_t)*tile_count * tile_rows : rows;
     for (uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (kThreads / 32)) {
@@ -97,107 +202,90 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const uint8_t *x, ui
             if (d < 0) continue;
             from = (uint32_t)d / divide;
         }
-        const uint8_t *row = x + (uint64_t)from * x_stride;
-        const uint32_t count = min(ahead, depth_blocks - piece.kb0);
-        uint32_t my_scale = 0;  // lane i: the scale of block i % 8 of chunk row kb0 + i / 8
-        const uint64_t byte0 = (uint64_t)piece.kb0 * 128 + lane * 4;
-        uint8_t *to = kTiled ? chunks + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0) * kMxCodeBytes + (piece.row % kChunkRows) * 128u +
-                                   ((((uint32_t)lane >> 2) ^ (piece.row & 7u)) << 4) + (lane & 3) * 4
-                             : out.codes + piece.row * out.codes_stride + byte0;
-        if (aligned && ahead == kAhead && (uint64_t)(piece.kb0 + kAhead) * kMxChunkValues <= depth && (kTiled || (out.codes_stride & 3u) == 0 && (reinterpret_cast<uintptr_t>(out.codes) & 3u) == 0)) {
-            // Whole pieces on their boundaries: nothing to guard.
-            const uint8_t *from8 = row + ((uint64_t)piece.kb0 * kMxChunkValues + lane * 8) * kBytes;
-            uint4 raw[kAhead][kBytes / 2];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-                for (int h = 0; h < kBytes / 2; ++h) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(from8 + u * kMxChunkValues * kBytes) + h);
-            uint32_t four = 0;  // this thread's block's scales in the four chunk rows
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                float v[8];
-                uint32_t s;
-                const uint32_t largest = unpack8<kType>(raw[u], v);
-                *reinterpret_cast<uint32_t *>(to + u * (kTiled ? kMxCodeBytes : 128u)) = quantise8(v, largest, s);
-                four |= s << (8 * u);
-            }
-            my_scale = (__shfl_sync(0xffffffffu, four, (lane & 7) * 4) >> (lane & 24)) & 255u;
-        } else if (aligned) {
-            uint4 raw[kAhead][kBytes / 2];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const uint64_t first = (uint64_t)(piece.kb0 + u) * kMxChunkValues + lane * 8;
-#pragma unroll
-                for (int h = 0; h < kBytes / 2; ++h) {
-                    raw[u][h] = make_uint4(0, 0, 0, 0);
-                    if (first + 8 <= depth) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(row + first * kBytes) + h);
-                }
-                if (first < depth && first + 8 > depth) {  // the row ends inside
-                    uint32_t w[2 * kBytes] = {};
-                    for (int i = 0; i < (int)(depth - first); ++i) {
-                        if constexpr (kType == kF32) w[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + first + i);
-                        else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(row) + first + i) << (16 * (i & 1));
-                    }
-#pragma unroll
-                    for (int h = 0; h < kBytes / 2; ++h) raw[u][h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (u >= (int)count) break;
-                float v[8];
-                uint32_t s;
-                const uint32_t largest = unpack8<kType>(raw[u], v), codes = quantise8(v, largest, s);
-                store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
-                const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
-                if ((lane >> 3) == u) my_scale = mine;
-            }
-        } else {
-            uint32_t all[kAhead][8];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    const uint64_t at = (uint64_t)(piece.kb0 + u) * kMxChunkValues + b * 32 + lane;
-                    all[u][b] = 0;
-                    if (u < (int)count && at < depth) {
-                        if constexpr (kType == kF32) all[u][b] = __ldg(reinterpret_cast<const uint32_t *>(row) + at);
-                        else all[u][b] = __ldg(reinterpret_cast<const uint16_t *>(row) + at);
-                    }
-                }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (u >= (int)count) break;
-                __syncwarp();
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    if constexpr (kType == kF32) reinterpret_cast<uint32_t *>(staging)[b * 32 + lane] = all[u][b];
-                    else reinterpret_cast<uint16_t *>(staging)[b * 32 + lane] = (uint16_t)all[u][b];
-                }
-                __syncwarp();
-                uint4 raw[kBytes / 2];
-#pragma unroll
-                for (int h = 0; h < kBytes / 2; ++h) raw[h] = reinterpret_cast<const uint4 *>(staging + lane * 8 * kBytes)[h];
-                float v[8];
-                uint32_t s;
-                const uint32_t largest = unpack8<kType>(raw, v), codes = quantise8(v, largest, s);
-                store_chunk_row<kTiled>(codes, piece.row, piece.kb0 + u, depth, out, chunks, depth_blocks, lane);
-                const uint32_t mine = __shfl_sync(0xffffffffu, s, (lane & 7) * 4);
-                if ((lane >> 3) == u) my_scale = mine;
-            }
+        quantise_piece<kType, kTiled>(x + (uint64_t)from * x_stride, piece, depth, aligned, out, chunks, scale_tiles, depth_blocks, ahead, staging_all[threadIdx.x >> 5], lane);
+    }
+}
+
+// The slots of a few tokens: their order by expert (see nkb_experts.cu) and the quantising of their rows in one launch. Every block orders
+// all slots for itself, one thread each, in the same way: a slot's row is its expert's first and the number of equal ids before it,
+// counted warp by warp. 128 slots of 32 experts, products with 4096 x 2048: 29.3 us for the layer, 32 us with the order and the zeroing as
+// launches of their own, 31 us against 38 from Python.
+struct FewSlots {
+    const int32_t *ids;
+    uint32_t slots, experts, divide, tile_rows;
+    MxRowTile *tiles;
+    int32_t *tile_count, *row_dest;
+    uint8_t *out;  // rows of slots without an expert are zeroed here, unless it is null
+    uint64_t row_bytes, out_stride;
+};
+template <uint32_t kType>
+__global__ void __launch_bounds__(kThreads) order_and_quantise_kernel(const uint8_t *x, uint64_t depth, uint64_t x_stride, FewSlots f, uint8_t *chunks,
+                                                                      uint8_t *scale_tiles, uint32_t depth_blocks, uint32_t ahead) {
+    constexpr uint32_t kWarps = kThreads / 32, kPer = kRouteMaxExperts / kThreads;  // experts a thread scans
+    static_assert(kFewSlots <= kThreads, "a thread per slot");
+    allow_next_kernel();
+    __shared__ uint32_t count[kRouteMaxExperts], first_row[kRouteMaxExperts], warp_sums[kWarps];
+    __shared__ int32_t row_of[kThreads];
+    __shared__ __align__(16) uint8_t staging_all[kWarps][kMxChunkValues * (kType == kF32 ? 4 : 2)];
+    const uint32_t t = threadIdx.x, warp = t >> 5;
+    const int lane = t & 31;
+    const int32_t id = t < f.slots ? f.ids[t] : -1;
+    const bool routed = (uint32_t)id < f.experts;  // none below 0 either
+    for (uint32_t e = t; e < kRouteMaxExperts; e += kThreads) count[e] = 0;
+    const uint32_t same = __match_any_sync(0xffffffffu, routed ? id : -1), before = __popc(same & ((1u << lane) - 1u));
+    uint32_t place = before;
+    __syncthreads();
+    for (uint32_t w = 0; w * 32 < f.slots; ++w) {
+        if (warp == w) {
+            const uint32_t earlier = routed ? count[id] : 0u;
+            __syncwarp();
+            place += earlier;
+            if (routed && before == 0) count[id] = earlier + __popc(same);
         }
-        if constexpr (kTiled) {
-            // Four scales to a word of a scale tile, for which eight lanes of a chunk row hold two words.
-            uint32_t word = my_scale << (8 * (lane & 3));
-            word |= __shfl_xor_sync(0xffffffffu, word, 1);
-            word |= __shfl_xor_sync(0xffffffffu, word, 2);
-            const uint32_t u = (uint32_t)lane >> 3, r = piece.row % kChunkRows;
-            if ((lane & 3) == 0 && u < count)
-                *reinterpret_cast<uint32_t *>(scale_tiles + ((uint64_t)(piece.row / kChunkRows) * depth_blocks + piece.kb0 + u) * kMxScaleBytes +
-                                              ((lane >> 2) & 1) * 512 + (r & 31u) * 16 + (r >> 5) * 4) = word;
-        } else {
-            const uint64_t block = (uint64_t)piece.kb0 * 8 + lane;
-            if (block * kMxBlock < depth && (uint32_t)(lane >> 3) < count) out.scales[piece.row * out.scales_stride + block] = (uint8_t)my_scale;
+        __syncthreads();
+    }
+    uint32_t tiles_here[kPer], mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) mine += tiles_here[i] = (count[t * kPer + i] + f.tile_rows - 1) / f.tile_rows;
+    uint32_t through = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, through, o);
+        if (lane >= o) through += v;
+    }
+    if (lane == 31) warp_sums[warp] = through;
+    __syncthreads();
+    for (uint32_t w = 0; w < warp; ++w) through += warp_sums[w];
+    if (t == kThreads - 1 && blockIdx.x == 0) *f.tile_count = (int32_t)through;
+    uint32_t tile = through - mine;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+        first_row[t * kPer + i] = tile * f.tile_rows;
+        tile += tiles_here[i];
+    }
+    __syncthreads();
+    if (t < f.slots) row_of[t] = routed ? (int32_t)(first_row[id] + place) : -1;
+    if (blockIdx.x == 0 && routed) f.row_dest[first_row[id] + place] = (int32_t)t;
+    // The experts' tiles, and the rows behind their last slots, which belong to nobody.
+    for (uint32_t e = blockIdx.x * kWarps + warp; e < f.experts; e += gridDim.x * kWarps) {
+        const uint32_t slots = count[e], row = first_row[e];
+        for (uint32_t r = slots + lane; r < (slots + f.tile_rows - 1) / f.tile_rows * f.tile_rows; r += 32) f.row_dest[row + r] = -1;
+        for (uint32_t i = lane; i * f.tile_rows < slots; i += 32) f.tiles[row / f.tile_rows + i] = {(int32_t)e, (int32_t)min(slots - i * f.tile_rows, f.tile_rows)};
+    }
+    __syncthreads();
+    const bool aligned = ((reinterpret_cast<uintptr_t>(x) | x_stride) & 15u) == 0;
+    const uint32_t pieces_per_row = (depth_blocks + ahead - 1) / ahead, items = f.slots * pieces_per_row;
+    for (uint32_t item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
+        Piece piece = piece_of(item, pieces_per_row, ahead);
+        const uint32_t slot = piece.row;
+        const int32_t to = row_of[slot];
+        if (to >= 0) {
+            piece.row = (uint32_t)to;
+            quantise_piece<kType, true>(x + (uint64_t)(slot / f.divide) * x_stride, piece, depth, aligned, RowMajorSink{}, chunks, scale_tiles, depth_blocks, ahead,
+                                        staging_all[warp], lane);
+        } else if (f.out && piece.kb0 == 0) {
+            uint16_t *row = reinterpret_cast<uint16_t *>(f.out + slot * f.out_stride);  // cells are two or four bytes
+            for (uint64_t i = lane; i < f.row_bytes / 2; i += 32) row[i] = 0;
         }
     }
 }
@@ -469,6 +557,24 @@ cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t dept
     case kF32: quantise_kernel<kF32, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
     case kBF16: quantise_kernel<kBF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
     case kF16: quantise_kernel<kF16, true><<<grid, kThreads, 0, stream>>>(src, n, depth, x_stride, none, dst, tiles, kblocks, row_dest, tile_count, tile_rows, divide, ahead); break;
+    default: return cudaErrorInvalidValue;
+    }
+    return cudaGetLastError();
+}
+
+cudaError_t launch_order_and_quantise(uint32_t type, const void *x, uint64_t depth, uint64_t x_stride, const int32_t *ids, uint32_t slots, uint32_t experts, uint32_t divide,
+                                      uint32_t tile_rows, uint64_t max_tiles, MxRowTile *tiles, int32_t *tile_count, int32_t *row_dest, void *out,
+                                      uint64_t row_bytes, uint64_t out_stride, void *chunks, cudaStream_t stream) {
+    if (slots > kFewSlots || experts > kRouteMaxExperts) return cudaErrorInvalidValue;
+    const uint32_t kblocks = (uint32_t)((depth + kMxChunkValues - 1) / kMxChunkValues), ahead = ahead_for(slots, kblocks);
+    const uint32_t grid = grid_for(slots * pieces(kblocks, ahead));
+    const FewSlots f{ids, slots, experts, divide, tile_rows, tiles, tile_count, row_dest, static_cast<uint8_t *>(out), row_bytes, out_stride};
+    const uint8_t *src = static_cast<const uint8_t *>(x);
+    uint8_t *dst = static_cast<uint8_t *>(chunks), *scale_tiles = dst + max_tiles * (tile_rows / kChunkRows) * kblocks * kMxCodeBytes;
+    switch (type) {
+    case kF32: order_and_quantise_kernel<kF32><<<grid, kThreads, 0, stream>>>(src, depth, x_stride, f, dst, scale_tiles, kblocks, ahead); break;
+    case kBF16: order_and_quantise_kernel<kBF16><<<grid, kThreads, 0, stream>>>(src, depth, x_stride, f, dst, scale_tiles, kblocks, ahead); break;
+    case kF16: order_and_quantise_kernel<kF16><<<grid, kThreads, 0, stream>>>(src, depth, x_stride, f, dst, scale_tiles, kblocks, ahead); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();

@@ -158,3 +158,18 @@ def test_the_workload_runs():
     from numkong_b200.workloads import run_experts
     out = run_experts(40, 6, 2, 192, 130, steps=2, warmup=1)
     assert out["workload"] == "experts" and out["ms"] > 0 and out["tokens_per_s"] > 0
+
+
+@pytest.mark.parametrize("tokens,experts,top", [(256, 1, 1), (200, 1, 1), (128, 3, 2), (64, 1024, 4), (86, 40, 3), (257, 2, 1), (33, 7, 3), (1, 1024, 32)])
+def test_few_slots(tokens, experts, top):
+    """As many slots as are ordered and quantised in one launch, and one more: any ids, missing ones among them."""
+    x, ids, w, rng = make(tokens, experts, top, 40, 300, False, "bf16", tokens + top)
+    weights = rng.random((tokens, top)).astype(np.float32)
+    for _ in range(2):
+        run(x, ids, w, 40, 300, None, "bf16", experts)
+        run(x, ids, w, 40, 300, weights, "f32", experts)
+        ids = np.where(rng.random(ids.shape) < 0.4, rng.integers(-3, experts + 3, ids.shape), ids).astype(np.int32)
+    ids[:] = experts - 1
+    run(x, ids, w, 40, 300, None, "f32", experts)
+    ids[:] = experts
+    assert (run(x, ids, w, 40, 300, None, "f32", experts) == 0).all()
