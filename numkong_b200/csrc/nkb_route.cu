@@ -531,7 +531,8 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
 
 // One warp per batch of one, two or four tokens, `width` lanes for the slots of each. What reaches a logit through the token's own slots
 // is worked out in 64 bits, one slot per lane, and put into a row in shared memory; the rows then go out in whole lines. Only the softmax
-// without renormalisation gives every logit something.
+// without renormalisation gives every logit something. Bound by the write of the rows and the start: 16,384 x 256, 8 chosen, 6.1 us for 18 MB
+// (2.7 us at the copy rate); 16,384 x 64, 6 chosen, 4.5 us; 16 tokens 3.3 us.
 template <uint32_t kType>
 __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const RouteDev p, const float *weights_grad, const int32_t *ids, float *logits_grad) {
     extern __shared__ float rows_all[];
