@@ -826,9 +826,10 @@ cudaError_t launch_by_width(int bn, bool bf16, const MxGemmDev &dev, uint64_t ma
 } // namespace
 
 // CTA pairs, when their tiles keep two thirds of the SMs busy. 2048^3 (64 tiles): 11.0 us against 13.5; 512 x 8192 x 8192 (64): 23.3 against
-// 28.7; 1024 x 2048 x 4096 (32): 13.6 against 13.4; 256 x 8192 x 8192 (32): 20.4 against 16.9.
+// 28.7; 1024 x 2048 x 4096 (32): 13.6 against 13.4; 256 x 8192 x 8192 (32): 20.4 against 16.9. Not for rows that one CTA's tile holds, for which
+// the follower's half would be empty: 8 x 32768 x 4096 (128): 19.6 against 16.3; 128 x 32768 x 4096: 22.7 against 18.6.
 bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t) {
-    return ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 3;
+    return m > kBM && ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 3;
 }
 
 // Every CTA quantises the rows again, and with more than two the loads of a chunk's rows no longer lie eight chunks ahead:

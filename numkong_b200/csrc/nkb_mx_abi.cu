@@ -170,6 +170,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     const uint64_t kblocks = (k + kMxBlock - 1) / kMxBlock;
     if (m > 1 && (codes ? codes_stride < (k + 1) / 2 || scales_stride < kblocks : a_stride < k * dtype_bytes(a_type))) { refuse("mxfp4 product: rows of A overlap"); return fail(); }
     if (!codes && (reinterpret_cast<uintptr_t>(a) | (m > 1 ? a_stride : 0)) % dtype_bytes(a_type)) { refuse("mxfp4 product: values of A are not aligned to their type"); return fail(); }
+    if (m == 1) c_stride = round_up(row_bytes, 16);  // whatever it was: nothing lies that far
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(1, n, k);
@@ -406,6 +407,7 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
     if (experts == 0 || experts > kRouteMaxExperts) { refuse("experts: 1 to 1024 experts"); return fail(); }
     if ((x_rows > 1 && x_stride < depth * dtype_bytes(x_type)) || (rows > 1 && out_stride < row_bytes)) { refuse("experts: rows overlap"); return fail(); }
     if ((reinterpret_cast<uintptr_t>(x) | (x_rows > 1 ? x_stride : 0)) % dtype_bytes(x_type) || (reinterpret_cast<uintptr_t>(out) | (rows > 1 ? out_stride : 0)) % cell || (reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) % 4) { refuse("experts: operands are not aligned to their elements"); return fail(); }
+    if (rows == 1) out_stride = round_up(row_bytes, 16);
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const MxGeometry g = mx_geometry(experts, width, depth);

@@ -283,3 +283,22 @@ def test_empty_and_zero_depth():
     packed = nk.dots_pack(nk.mx_quantise(torch.randn(9, 64, device="cuda")))
     assert nk.dots_packed(torch.zeros(0, 64, device="cuda"), packed).shape == (0, 9)
     assert nk.mx_quantise(torch.zeros(0, 64, device="cuda")).rows == 0
+
+
+@pytest.mark.parametrize("cells", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [1, 16, 17, 128, 129])
+def test_few_rows_of_a_wide_matrix(m, cells):
+    """Wide enough for CTA pairs, with rows for one of them; and one row whose result has a stride that is not used."""
+    n, k = 13000, 260
+    a, b = random_mx(m, k, 12), random_mx(n, k, 13)
+    q = nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in a), k)
+    packed = nk.dots_pack(nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), k))
+    got = nk.dots_packed(q, packed, out_dtype=cells)
+    assert nk.synchronize() == 0
+    check_product(a, b, k, got, cells)
+    if m == 1:
+        out = torch.full((n + 8,), 7.0, dtype=TORCH[cells], device="cuda")
+        nk.lib.nkb_dots_packed_mxfp4(q.codes.data_ptr(), 3, q.scales.data_ptr(), 1, packed.buffer.data_ptr(), out.data_ptr(),
+                                     nk.DTYPE_CODES[cells], 1, n, k, 1, None)
+        assert nk.last_error() == "" and nk.synchronize() == 0
+        assert torch.equal(out[:n], got[0]) and (out[n:] == 7).all()
