@@ -551,7 +551,11 @@ cudaError_t launch_mx_quantise_tiled(uint32_t type, const void *x, uint64_t dept
     const RowMajorSink none{nullptr, nullptr, 0, 0};
     const uint32_t ahead = ahead_for(tiled_rows, kblocks);
     if (tiled_rows * pieces(kblocks, ahead) > 0xffffffffull - 148ull * 64 * 8) return cudaErrorInvalidValue;
-    const uint32_t grid = grid_for(tiled_rows * pieces(kblocks, ahead)), n = (uint32_t)tiled_rows;
+    // Rows found through row_dest are a latency each: warps that take several of them meet it less often than new blocks do. 16,384 rows of
+    // 2,048 bf16 in a layer of experts: 69.3 us with eight blocks per SM, 70.6 with 32.
+    uint32_t grid = grid_for(tiled_rows * pieces(kblocks, ahead));
+    if (row_dest && grid > 148 * 8) grid = 148 * 8;
+    const uint32_t n = (uint32_t)tiled_rows;
     const uint8_t *src = static_cast<const uint8_t *>(x);
     uint8_t *dst = static_cast<uint8_t *>(chunks), *tiles = dst + (tiled_rows + kChunkRows - 1) / kChunkRows * kblocks * kMxCodeBytes;
     switch (type) {

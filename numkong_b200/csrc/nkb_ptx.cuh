@@ -117,6 +117,11 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t cta_
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(cta_rank));
     return r;
 }
+__device__ __forceinline__ uint32_t ld_shared_cluster(uint32_t cluster_addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void mbar_arrive_cluster_addr(uint32_t bar_cluster) {
     // Default semantics (release at CTA scope): the hand-over of TMEM is ordered by tcgen05.fence::before_thread_sync, and a
     // cluster-scope release costs every arriving warp a memory fence (seen as "membar" stalls of 1.5-1.8 per issued instruction).
