@@ -308,9 +308,10 @@ NKB_API int nkb_angulars_packed_noalloc(uint32_t dtype, void const *a, void cons
  *
  * Pointers may be host or device memory, mixed freely, as everywhere; device operands have to live on the calling thread's
  * current GPU (a call with one that does not is refused). On failure the outputs are filled with 0xFF bytes, i.e. NaN scales
- * and cells and ids of -1, as far as sizes and strides span (not where a size itself is refused: 2^31 and more). `workspace` is device memory of at least the stated size on a 256-byte boundary that no
- * other call uses at the same time; with NULL the calling thread's staging memory is used, which allocates on first use and is
- * shared by everything the thread enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own,
+ * and cells and ids of -1, as far as sizes and strides span (not where a size itself is refused: 2^31 and more; nor on another GPU).
+ * `workspace` is device memory of at least the stated size on a 256-byte boundary that no other call uses at the same time; with
+ * NULL the calling thread's staging memory is used, which allocates on first use and is shared by everything the thread
+ * enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own,
  * for as long as it may run. (Products of one or two float rows need none: they quantise inside.) The first product on each GPU
  * allocates the device error word; make it before a capture starts.
  *

@@ -110,6 +110,11 @@ constexpr uint64_t kMostRows = 0x7fffff00ull;  // indices inside the kernels are
 // sizes and stride span. Sizes that no kernel takes are not believed.
 void spoil(void *out, uint64_t rows, uint64_t row_bytes, uint64_t stride) {
     if (!out || rows == 0 || rows > kMostRows || row_bytes > 4 * kMostRows) return;
+    cudaPointerAttributes attr;
+    int device = 0;
+    cudaGetDevice(&device);
+    if (cudaPointerGetAttributes(&attr, out) != cudaSuccess) cudaGetLastError();
+    else if (attr.type == cudaMemoryTypeDevice && attr.device != device) return;  // another GPU's memory is left alone
     if (stride < row_bytes) fill_error_output(out, classify(out), 1, (rows - 1) * stride + row_bytes, (rows - 1) * stride + row_bytes);
     else fill_error_output(out, classify(out), rows, row_bytes, stride);
 }
