@@ -302,3 +302,17 @@ def test_few_rows_of_a_wide_matrix(m, cells):
                                      nk.DTYPE_CODES[cells], 1, n, k, 1, None)
         assert nk.last_error() == "" and nk.synchronize() == 0
         assert torch.equal(out[:n], got[0]) and (out[n:] == 7).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("n,k", [(13000, 3000), (2304, 520)])
+def test_every_kernel_sums_alike(n, k, name):
+    """One row, few rows, rows for CTA pairs: the bits of a row are the same from each of them."""
+    x = torch.randn(2304, k, generator=torch.Generator(device="cuda").manual_seed(k), device="cuda").to(TORCH[name])
+    b = random_mx(n, k, 14)
+    packed = nk.dots_pack(nk.MxMatrix(*(torch.from_numpy(v).cuda() for v in b), k))
+    whole = nk.dots_packed(x, packed)
+    for first, count in ((0, 1), (5, 2), (7, 3), (100, 16), (100, 17), (1000, 128), (1000, 129), (2303, 1)):
+        assert torch.equal(nk.dots_packed(x[first:first + count], packed), whole[first:first + count])
+        assert torch.equal(nk.dots_packed(nk.mx_quantise(x[first:first + count]), packed), whole[first:first + count])
+    assert nk.synchronize() == 0
