@@ -220,3 +220,24 @@ def test_scales_of_any_size(m, n):
     assert (np.abs(got[small]) <= 2.0 ** -126).all()
     large = np.abs(want) >= 2.0 ** 128
     assert np.isinf(got[large]).all() and (np.sign(got[large]) == np.sign(want[large])).all()
+
+
+@pytest.mark.parametrize("m,n", [(64, 20000), (600, 20000)])
+def test_waits_that_give_up(m, n):
+    """The epilogue's waits run out: the error word says so once, and the next call is right."""
+    k = 8192
+    g = torch.Generator(device="cuda").manual_seed(m)
+    q = nk.mx_quantise(torch.randn(m, k, generator=g, device="cuda"))
+    packed = nk.dots_pack(nk.mx_quantise(torch.randn(n, k, generator=g, device="cuda")))
+    want = nk.dots_packed(q, packed)
+    assert nk.synchronize() == 0
+    nk.set_wait_limit_ns(0, 20_000_000)  # every site: 20 ms
+    nk.set_wait_limit_ns(4, 3_000)       # the epilogue's wait for an accumulator: 3 microseconds
+    try:
+        nk.dots_packed(q, packed)
+        word = nk.synchronize()
+    finally:
+        nk.set_wait_limit_ns(0, 0)
+    assert word & 0x80000000 and (word >> 16) & 0xff == 4
+    assert torch.equal(nk.dots_packed(q, packed), want)
+    assert nk.synchronize() == 0
