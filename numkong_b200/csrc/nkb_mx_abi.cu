@@ -28,7 +28,8 @@ public:
     }
     bool on_host() const { return owned_count_ != 0; }
 
-    // An input of `rows` rows of `row_bytes`, `stride` apart; a host matrix is uploaded with its rows packed 16-byte aligned.
+    // An input of `rows` rows of `row_bytes`, `stride` apart; a host matrix is uploaded with its rows packed 16-byte aligned. `stride` becomes
+    // that of the device view, so it has to be the caller's copy of what it was given: a failed call fills the given rows.
     const uint8_t *in(const void *p, uint64_t rows, uint64_t row_bytes, uint64_t &stride) {
         if (!place(p)) return nullptr;
         if (on_device_) return static_cast<const uint8_t *>(p);
@@ -184,9 +185,10 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     const uint8_t *blob = resident_blob_of_size(packed, packed_kind, kMagicMx, kMxfp4, n, k, g.total_bytes, nullptr);
     unsigned int *err = blob ? device_error_word() : nullptr;
     if (!err) { if (blob) refuse("could not allocate the device error word"); return fail(); }
-    uint8_t *c_dev = ops.out(c, m, row_bytes, c_stride);
+    uint64_t c_pitch = c_stride;
+    uint8_t *c_dev = ops.out(c, m, row_bytes, c_pitch);
     bool ok = c_dev != nullptr;
-    if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_stride, 0, row_bytes, m, stream), "clear result");
+    if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_pitch, 0, row_bytes, m, stream), "clear result");
     else if (ok) {
         const bool inside = !codes && gemm_mx_quantises(m);
         uint8_t *chunks = inside ? nullptr : workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
@@ -211,7 +213,7 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
             args.a_chunks = chunks; args.b_chunks = blob + g.payload_offset;
             if (inside) { args.x = ad; args.x_stride = m > 1 ? a_stride : 0; args.x_type = a_type; }
             if (rows_in_place) { args.a_codes = cd; args.a_codes_stride = codes_stride; }
-            args.c = c_dev; args.c_stride = c_stride; args.c_bf16 = c_type == kBF16;
+            args.c = c_dev; args.c_stride = c_pitch; args.c_bf16 = c_type == kBF16;
             args.m = m; args.n = n; args.k = k; args.error_word = err;
             ok = cuda_ok(launch_gemm_mx(args, stream), "mxfp4 GEMM kernel");
             g_launches += inside ? 1 : 2;
@@ -244,8 +246,9 @@ NKB_API void nkb_mx_quantise(void const *x, uint32_t x_type, nk_size_t rows, nk_
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *xd = ops.in(x, rows, depth * dtype_bytes(x_type), x_stride);
-    uint8_t *cd = xd ? ops.out(codes, rows, code_bytes, codes_stride) : nullptr, *sd = cd ? ops.out(scales, rows, blocks, scales_stride) : nullptr;
-    const bool ok = sd && cuda_ok(launch_mx_quantise(x_type, xd, rows, depth, x_stride, cd, codes_stride, sd, scales_stride, stream), "quantise kernel");
+    uint64_t codes_pitch = codes_stride, scales_pitch = scales_stride;
+    uint8_t *cd = xd ? ops.out(codes, rows, code_bytes, codes_pitch) : nullptr, *sd = cd ? ops.out(scales, rows, blocks, scales_pitch) : nullptr;
+    const bool ok = sd && cuda_ok(launch_mx_quantise(x_type, xd, rows, depth, x_stride, cd, codes_pitch, sd, scales_pitch, stream), "quantise kernel");
     g_launches++;
     if (!ok || !ops.finish("mx_quantise")) fail();
 }
@@ -265,8 +268,9 @@ NKB_API void nkb_mx_dequantise(void const *codes, nk_size_t codes_stride, void c
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     const uint8_t *cd = ops.in(codes, rows, code_bytes, codes_stride), *sd = cd ? ops.in(scales, rows, blocks, scales_stride) : nullptr;
-    uint8_t *xd = sd ? ops.out(x, rows, row_bytes, x_stride) : nullptr;
-    const bool ok = xd && cuda_ok(launch_mx_dequantise(x_type, cd, codes_stride, sd, scales_stride, rows, depth, xd, x_stride, stream), "dequantise kernel");
+    uint64_t x_pitch = x_stride;
+    uint8_t *xd = sd ? ops.out(x, rows, row_bytes, x_pitch) : nullptr;
+    const bool ok = xd && cuda_ok(launch_mx_dequantise(x_type, cd, codes_stride, sd, scales_stride, rows, depth, xd, x_pitch, stream), "dequantise kernel");
     g_launches++;
     if (!ok || !ops.finish("mx_dequantise")) fail();
 }
@@ -421,9 +425,10 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
     const uint8_t *blob = resident_blob_of_size(b_packed, packed_kind, kMagicMx, kMxfp4, experts * width, depth, g.total_bytes, nullptr);
     unsigned int *err = blob ? device_error_word() : nullptr;
     if (!err) { if (blob) refuse("could not allocate the device error word"); return fail(); }
-    uint8_t *dst = ops.out(out, rows, row_bytes, out_stride);
+    uint64_t out_pitch = out_stride;
+    uint8_t *dst = ops.out(out, rows, row_bytes, out_pitch);
     bool ok = dst != nullptr;
-    if (ok && depth == 0) ok = cuda_ok(cudaMemset2DAsync(dst, out_stride, 0, row_bytes, rows, stream), "clear result");
+    if (ok && depth == 0) ok = cuda_ok(cudaMemset2DAsync(dst, out_pitch, 0, row_bytes, rows, stream), "clear result");
     else if (ok) {
         const ExpertsLayout l = experts_layout(slots, experts, width, depth, weights != nullptr);
         uint8_t *ws = workspace_or_scratch(ops, workspace, l.total);
@@ -437,7 +442,7 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
             float *sums = reinterpret_cast<float *>(ws + l.sums);
             MxGemmArgs args;
             args.a_chunks = ws + l.chunks; args.b_chunks = blob + g.payload_offset;
-            args.c = weights ? static_cast<void *>(sums) : dst; args.c_stride = weights ? width * 4 : out_stride;
+            args.c = weights ? static_cast<void *>(sums) : dst; args.c_stride = weights ? width * 4 : out_pitch;
             args.c_bf16 = !weights && out_type == kBF16;
             args.m = slots; args.n = width; args.k = depth;
             args.tiles = tiles; args.tile_count = count; args.row_dest = dest; args.max_tiles = l.max_tiles; args.tile_rows = l.tile_rows; args.groups = experts; args.error_word = err;
@@ -446,13 +451,13 @@ NKB_API void nkb_experts_packed_mxfp4(void const *x, uint32_t x_type, nk_size_t 
             args.tiles_fresh = slots <= kFewSlots;
             if (args.tiles_fresh)
                 ok = cuda_ok(launch_order_and_quantise(x_type, xd, depth, stride, id, (uint32_t)slots, n, divide, l.tile_rows, l.max_tiles, tiles, count, dest, weights ? nullptr : dst,
-                                                       row_bytes, out_stride, ws + l.chunks, stream), "order and quantise kernel");
+                                                       row_bytes, out_pitch, ws + l.chunks, stream), "order and quantise kernel");
             else
                 ok = cuda_ok(launch_expert_order(id, slots, n, tiles, count, dest, l.max_tiles, l.tile_rows, stream), "expert order kernel") &&
                      cuda_ok(launch_mx_quantise_tiled(x_type, xd, depth, stride, l.max_tiles * l.tile_rows, dest, count, l.tile_rows, divide, ws + l.chunks, stream), "quantise kernel");
             ok = ok && cuda_ok(launch_gemm_mx(args, stream), "grouped mxfp4 GEMM kernel");
-            if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, n, width, dst, out_type == kBF16, out_stride, stream), "combine kernel");
-            else if (ok && !args.tiles_fresh) ok = cuda_ok(launch_zero_unrouted(id, slots, n, dst, row_bytes, out_stride, stream), "zero kernel");
+            if (ok && weights) ok = cuda_ok(launch_combine(sums, wd, id, tokens, (uint32_t)top, n, width, dst, out_type == kBF16, out_pitch, stream), "combine kernel");
+            else if (ok && !args.tiles_fresh) ok = cuda_ok(launch_zero_unrouted(id, slots, n, dst, row_bytes, out_pitch, stream), "zero kernel");
             g_launches += !args.tiles_fresh ? 4 : weights ? 3 : 2;
         }
     }
