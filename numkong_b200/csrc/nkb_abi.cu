@@ -271,7 +271,12 @@ const uint8_t *resident_blob_of_size(const void *blob, MemKind kind, uint32_t ma
     evict_for_insert();
     void *d = nullptr;
     if (!cuda_ok(cudaMalloc(&d, h.total_bytes), "cudaMalloc(packed blob copy)")) return nullptr;
-    if (!cuda_ok(cudaMemcpyAsync(d, blob, h.total_bytes, cudaMemcpyHostToDevice, t_ctx.stream), "upload of packed blob")) { cudaFree(d); return nullptr; }
+    // Waited for before the entry can be found: calls on other streams, of this thread or another, take what is here as complete.
+    if (!cuda_ok(cudaMemcpyAsync(d, blob, h.total_bytes, cudaMemcpyHostToDevice, current_stream()), "upload of packed blob") ||
+        !cuda_ok(cudaStreamSynchronize(current_stream()), "upload of packed blob")) {
+        cudaFree(d);
+        return nullptr;
+    }
     CachedBlob e; e.nonce = h.nonce; e.bytes = h.total_bytes; e.device = dev; e.dev_ptr = d; e.last_use = ++g_cache_clock;
     e.pins = 1;
     t_ctx.pins.emplace_back(e.nonce, dev);
