@@ -668,8 +668,13 @@ def _cuda(x: Any) -> bool:
     return _is_torch(x) and x.is_cuda
 
 
+def _place(x: Any, packed: PackedMatrix) -> Any:
+    """The operand that says where a product runs: `x`, or the packed matrix where that alone lives on a GPU."""
+    return packed.buffer if not _cuda(x) and packed.is_cuda else x
+
+
 def _enqueue(x: Any, call: Any, *arguments: Any) -> None:
-    """Makes a library call that works on `x`: with the GPU of a CUDA tensor current, and for a thread that has not chosen a
+    """Makes a library call that works where `x` lives: with the GPU of a CUDA tensor current, and for a thread that has not chosen a
     stream with set_stream on torch's current one, where the tensors come from and the results go."""
     if not _is_torch(x) or not x.is_cuda:
         call(*arguments)
@@ -832,16 +837,17 @@ def _packed_mx(a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], out
     if depth != packed.depth:
         raise ValueError(f"depth mismatch: a has {depth} dimensions, packed matrix has depth {packed.depth}")
     x = v.codes if isinstance(v, MxMatrix) else v.obj
+    place = _place(x, packed)
     result, stride = _mx_result(x, v.rows, packed.width, out, out_dtype)
     if isinstance(v, MxMatrix) or v.rows > 2:  # one or two float rows are quantised inside the product
-        workspace, ws = _workspace(x, (v.rows + 127) // 128 * ((depth + 255) // 256) * 17408)  # nkb_dots_workspace_mxfp4
+        workspace, ws = _workspace(place, (v.rows + 127) // 128 * ((depth + 255) // 256) * 17408)  # nkb_dots_workspace_mxfp4
     else:
         workspace = ws = None
     rest = _ptr(packed.buffer), _ptr(result), DTYPE_CODES[out_dtype], v.rows, packed.width, depth, stride, ws
     if isinstance(v, MxMatrix):
-        _enqueue(x, lib.nkb_dots_packed_mxfp4, *v._parts, *rest)
+        _enqueue(place, lib.nkb_dots_packed_mxfp4, *v._parts, *rest)
     else:
-        _enqueue(x, lib.nkb_dots_packed_quantised_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, *rest)
+        _enqueue(place, lib.nkb_dots_packed_quantised_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, *rest)
     check("dots_packed")
     return result
 
@@ -914,8 +920,9 @@ def experts_packed(x: Any, ids: Any, packed: PackedMatrix, *, weights: Any = Non
     if out is not None and weights is None:
         out = _checked(out, (tokens, top, packed.width), ("float32", "bfloat16", "uint16"), "out", v.obj).reshape(rows, packed.width)
     result, stride = _mx_result(v.obj, rows, packed.width, out, out_dtype)
-    workspace, ws = _workspace(v.obj, lib.nkb_experts_workspace_mxfp4(tokens, top, packed.groups, packed.width, v.depth, int(weights is not None)))
-    _enqueue(v.obj, lib.nkb_experts_packed_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, int(per_slot), _ptr(ids), tokens, top, _ptr(packed.buffer),
+    place = _place(v.obj, packed)
+    workspace, ws = _workspace(place, lib.nkb_experts_workspace_mxfp4(tokens, top, packed.groups, packed.width, v.depth, int(weights is not None)))
+    _enqueue(place, lib.nkb_experts_packed_mxfp4, v.ptr, DTYPE_CODES[v.dtype], v.stride, int(per_slot), _ptr(ids), tokens, top, _ptr(packed.buffer),
              packed.groups, packed.width, v.depth, None if weights is None else _ptr(weights), _ptr(result), DTYPE_CODES[out_dtype], stride, ws)
     check("experts_packed")
     return result if weights is not None else result.reshape(tokens, top, packed.width)

@@ -1,5 +1,5 @@
-"""Packed matrices in host memory with operands on a side stream of torch's: what is uploaded is there before the product reads it,
-whatever the other streams are busy with."""
+"""Packed matrices in host memory with operands on a side stream of torch's, and the other way round: what is uploaded, packed or
+prepared for a product is there before the product reads it, whatever the other streams are busy with."""
 import numpy as np
 import pytest
 import torch
@@ -90,4 +90,29 @@ def test_experts_in_host_memory_on_a_side_stream():
             got = nk.experts_packed(x, ids, pairs[i][0])
             side.synchronize()
         assert torch.equal(got, want[i]), i
+    assert nk.synchronize() == 0
+
+
+@pytest.mark.parametrize("kind", ["numpy", "torch"])
+def test_host_operands_against_a_matrix_packed_on_a_side_stream(kind):
+    """The call works where the matrix lives, and after what prepares it there."""
+    rng, busy, side = np.random.default_rng(3), Busy(), torch.cuda.Stream()
+    x, ids = rng.standard_normal((30, K)).astype(np.float32), rng.integers(0, 4, (30, 2)).astype(np.int32)
+    part = rng.random((30, 2)).astype(np.float32)
+    as_given = (lambda a: a) if kind == "numpy" else torch.from_numpy
+    for attempt in range(4):
+        w = torch.from_numpy(rng.standard_normal((4 * WIDTH, K)).astype(np.float32)).cuda()
+        torch.cuda.synchronize()
+        busy.keep(side)
+        with torch.cuda.stream(side):
+            q = nk.mx_quantise(w)
+            plain, grouped = nk.dots_pack(q), nk.dots_pack(q, groups=4)
+            got = [nk.dots_packed(as_given(x), plain), nk.dots_packed(as_given(x[:1]), plain), nk.dots_packed(nk.mx_quantise(as_given(x)), plain),
+                   nk.experts_packed(as_given(x), as_given(ids), grouped), nk.experts_packed(as_given(x), as_given(ids), grouped, weights=as_given(part))]
+        torch.cuda.synchronize()
+        xd, idsd, partd = (torch.from_numpy(a).cuda() for a in (x, ids, part))
+        want = [nk.dots_packed(xd, plain), nk.dots_packed(xd[:1], plain), nk.dots_packed(nk.mx_quantise(xd), plain),
+                nk.experts_packed(xd, idsd, grouped), nk.experts_packed(xd, idsd, grouped, weights=partd)]
+        for g, v in zip(got, want, strict=True):
+            assert np.array_equal(np.asarray(g), v.cpu().numpy()), attempt
     assert nk.synchronize() == 0
