@@ -718,6 +718,18 @@ def _workspace(x: Any, nbytes: int):
     return buffer, (buffer.data_ptr() + 255) // 256 * 256
 
 
+def _as_rows(x: Any, rows: int):
+    """[tokens, top, depth] as `rows` rows. Where the strides do not fold that is a copy, made on the stream the call will run on: there it
+    is finished when the kernels come, and the allocator hands it on only behind them."""
+    if _cuda(x):
+        t = _torch if _torch.ready else _torch.load()
+        chosen = getattr(_thread, "stream", 0)
+        if chosen and chosen != t.stream(x.get_device()):
+            with t.module.cuda.stream(t.module.cuda.ExternalStream(chosen, device=x.device)):
+                return x.reshape(rows, x.shape[2])
+    return x.reshape(rows, x.shape[2])
+
+
 def _array(x: Any) -> Any:
     """A torch tensor (device arrays of other libraries come in through DLPack) or a NumPy array."""
     if _is_torch(x) or isinstance(x, np.ndarray):
@@ -910,7 +922,7 @@ def experts_packed(x: Any, ids: Any, packed: PackedMatrix, *, weights: Any = Non
     per_slot = len(x.shape) == 3
     if per_slot and tuple(x.shape[:2]) != (tokens, top) or not per_slot and x.shape[0] != tokens:
         raise ValueError(f"x must be [{tokens}, depth] or [{tokens}, {top}, depth]")
-    v = _float_view(x.reshape(tokens * top, x.shape[2]) if per_slot else x, dtype, "experts_packed")
+    v = _float_view(_as_rows(x, tokens * top) if per_slot else x, dtype, "experts_packed")
     if v.depth != packed.depth:
         raise ValueError(f"depth mismatch: x has {v.depth} dimensions, packed matrices have depth {packed.depth}")
     ids = _checked(ids, (tokens, top), ("int32",), "ids", v.obj)
