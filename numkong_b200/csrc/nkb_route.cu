@@ -529,10 +529,19 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
     }
 }
 
-// One warp per batch of one, two or four tokens, `width` lanes for the slots of each. What reaches a logit through the token's own slots
-// is worked out in 64 bits, one slot per lane, and put into a row in shared memory; the rows then go out in whole lines. Only the softmax
-// without renormalisation gives every logit something. Bound by the write of the rows and the start: 16,384 x 256, 8 chosen, 6.1 us for 18 MB
-// (2.7 us at the copy rate); 16,384 x 64, 6 chosen, 4.5 us; 16 tokens 3.3 us.
+// One warp per batch of one, two or four tokens, `width` lanes for the slots of each. What reaches a chosen expert's logit is worked out in
+// 64 bits from the 32-bit exponentials, one slot per lane, and put into a row in shared memory; the rows then go out in whole lines. Only
+// the softmax without renormalisation gives every logit something.
+//
+// With n the scores' numerators (exponentials, or sigmoids), N their sum over the chosen, or over all experts without renormalisation, and
+// O the part of it that was not chosen, the gradient of a chosen logit is
+//   n_e / N^2 (sum over the chosen j of n_j (g_e - g_j) + g_e O), for sigmoids times 1 - s_e.
+// Where one score is nearly all of N the terms of g_e N - sum of n_j g_j cancel. So every g is taken relative to that of the largest
+// numerator first (relative to 0 if that is not among the chosen), which leaves the bracket as it is and takes its largest terms out.
+// Bound by the write of the rows and the start: 16,384 x 256 f32, sigmoid, 8 chosen, 5.8 us for 18 MB (2.7 us at the copy rate); 16,384 x 64
+// bf16, softmax renormalised, 6 chosen, 4.1 us; 16 tokens 3.2 us. Softmax without renormalisation, which reads every logit: 16,384 x 256
+// 14.0 us, 16,384 x 64 8.8 us (8.1 us with the subtraction of two 32-bit values, which lost what nearly cancels: half of a chosen logit's
+// gradient and more where it lies 20 above the others).
 template <uint32_t kType>
 __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const RouteDev p, const float *weights_grad, const int32_t *ids, float *logits_grad) {
     extern __shared__ float rows_all[];
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
         if (!(l > -INFINITY)) id = -1;  // a masked expert has score 0 whatever its logit: no gradient
         const double g = id >= 0 ? (double)incoming * p.scale : 0.0;
         float top_logit = -INFINITY;
-        double total = 0.0;
+        double all = 0.0;  // the numerators of all experts
         if (dense) {
             for (uint32_t t = 0; t < here; ++t) {
                 const uint8_t *row = p.logits + (first + t) * p.stride;
@@ -572,46 +581,76 @@ __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const Route
                     sum += (double)part;
                 }
                 sum = warp_sum(sum);
-                if (place == t) { top_logit = largest; total = sum; }
+                if (place == t) { top_logit = largest; all = sum; }
             }
+            __syncwarp();
         } else {
             for (uint32_t i = lane; i < here * padded / 4; i += 32) reinterpret_cast<float4 *>(lines)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        double d = 0.0;  // what this slot's logit gets through the slot itself
-        const bool near_limit = p.sigmoid && ((__ballot_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f) >> (place * width)) & (0xffffffffu >> (32 - width))) != 0;
-        if (p.renormalise) {
-            float most = l;
-            for (uint32_t o = 1; o < width; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            double part = 0.0;
-            if (id >= 0) part = !near_limit ? fast_score(p.sigmoid, l, most) : small_sigmoid(l, most);
-            const double sum = over_slots(part), u = id >= 0 ? part * (sum > 1e-30 ? reciprocal(sum) : 1.0 / sum) : 0.0, mean = over_slots(g * u);
-            d = u * (g - mean);
-        } else if (id >= 0) {
-            d = p.sigmoid ? g * (near_limit ? small_sigmoid(l, 0.0f) : fast_score(true, l, 0.0f)) : g * ((double)exp_difference(l, top_logit) * reciprocal(total));
-        }
-        if (p.sigmoid && id >= 0) d *= near_limit ? small_sigmoid(-l, 0.0f) : fast_score(true, -l, 0.0f);  // 1 - s
-        __syncwarp();
-        if (dense) {
-            const double spread = over_slots(d);
-            const float per_part = total > 0.0 ? (float)(-spread * reciprocal(total)) : 0.0f;
-            for (uint32_t t = 0; t < here; ++t) {
-                const float factor = __shfl_sync(0xffffffffu, per_part, t * width);
-                for (uint32_t e = lane; e < p.experts; e += 32) lines[t * padded + e] *= factor;
-            }
-            __syncwarp();
-        }
-        // An expert named twice gets its slots' sum in their order, from the first of them.
+        // An expert named twice counts once in the softmax, with its slots' sum, in their order, in the first of them.
         const uint32_t segment = (width == 32 ? 0xffffffffu : (1u << width) - 1u) << (place * width);
         const uint32_t same = __match_any_sync(0xffffffffu, id) & segment;
-        if (__any_sync(0xffffffffu, id >= 0 && __popc(same) > 1)) {
+        const bool first_of = id >= 0 && __ffs(same) - 1 == lane, twice = __any_sync(0xffffffffu, id >= 0 && __popc(same) > 1);
+        auto over_same = [&](double v) {
             double sum = 0.0;
             for (uint32_t j = 0; j < width; ++j) {
-                const double other = __shfl_sync(0xffffffffu, d, place * width + j);
+                const double other = __shfl_sync(0xffffffffu, v, place * width + j);
                 if ((same >> (place * width + j)) & 1u) sum += other;
             }
-            d = sum;
+            return sum;
+        };
+        double d = 0.0;  // what this slot's logit gets through the slot itself
+        const bool near_limit = p.sigmoid && ((__ballot_sync(0xffffffffu, id >= 0 && fabsf(l) > 80.0f) >> (place * width)) & (0xffffffffu >> (32 - width))) != 0;
+        if (p.renormalise || dense) {
+            double mine = dense && twice ? over_same(g) : g, part = 0.0;
+            const bool counts = dense ? first_of : id >= 0;
+            if (!counts) mine = 0.0;
+            // The gradient that comes in at the slot with the largest logit; of several such the largest, so that no order matters.
+            float most = counts ? l : -INFINITY;
+            double ref = mine;
+            for (uint32_t o = 1; o < width; o <<= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, most, o);
+                const double other_ref = __shfl_xor_sync(0xffffffffu, ref, o);
+                if (other > most || (other == most && other_ref > ref)) { most = other; ref = other_ref; }
+            }
+            if (counts) part = dense ? (double)exp_difference(l, top_logit) : !near_limit ? fast_score(p.sigmoid, l, most) : small_sigmoid(l, most);
+            const double chosen = over_slots(part);
+            double others = 0.0;
+            if (dense) {
+                // The difference loses 20 of its 53 bits at most, or the others are added up by themselves.
+                others = all - chosen;
+                uint32_t rare = __ballot_sync(0xffffffffu, slot == 0 && others < all * 0x1p-20);
+                if (rare != 0) {
+                    if (counts) line[id] = 0.0f;
+                    __syncwarp();
+                    for (; rare; rare &= rare - 1) {
+                        const uint32_t t = (__ffs(rare) - 1) / width;
+                        double sum = 0.0;
+                        for (uint32_t e = lane; e < p.experts; e += 32) sum += (double)lines[t * padded + e];
+                        sum = warp_sum(sum);
+                        if (place == t) others = sum;
+                    }
+                }
+                if (most < top_logit || others > 1.0) ref = 0.0;  // the slot's numerator is 1 at most
+            }
+            if (!(fabs(ref) < INFINITY)) ref = 0.0;
+            const double total = chosen + others, shifted = over_slots(part * (mine - ref)) - others * ref;
+            const double inverse = total > 0.0 ? total > 1e-30 ? reciprocal(total) : 1.0 / total : 0.0;
+            if (counts) d = part * inverse * (((mine - ref) * total - shifted) * inverse);
+            if (dense) {
+                const float per_part = (float)(-(over_slots(part * mine) * inverse) * inverse);
+                for (uint32_t t = 0; t < here; ++t) {
+                    const float factor = __shfl_sync(0xffffffffu, per_part, t * width);
+                    for (uint32_t e = lane; e < p.experts; e += 32) lines[t * padded + e] *= factor;
+                }
+            }
+        } else if (id >= 0) {
+            d = g * (near_limit ? small_sigmoid(l, 0.0f) : fast_score(true, l, 0.0f));
         }
-        if (id >= 0 && __ffs(same) - 1 == lane) line[id] += (float)d;
+        if (p.sigmoid && id >= 0) d *= near_limit ? small_sigmoid(-l, 0.0f) : fast_score(true, -l, 0.0f);  // 1 - s
+        if (!dense && twice) d = over_same(d);
+        __syncwarp();
+        if (first_of) line[id] = (float)d;
         __syncwarp();
         float *out = logits_grad + (uint64_t)first * p.experts;
         if ((p.experts & 3u) == 0 && (reinterpret_cast<uintptr_t>(logits_grad) & 15u) == 0)  // the rows lie one behind the other here and there
