@@ -872,8 +872,9 @@ def route(logits: Any, top: int, *, bias: Any = None, score: str = "softmax", gr
     """The `top` experts of every token and their weights, from its logits (nkb_route): (weights f32, ids int32), both
     [tokens, top]. Scores are the softmax or the sigmoid of the logits; `bias` (f32 per expert) is added for the selection
     only; with `groups` a group is worth the sum of its two best keys and only the `top_groups` best are open (default: all).
-    Best first, ties to the lower index. Weights are the scores, over their sum with `renormalise`, times `scale`. Logits of
-    -inf or NaN are never chosen; slots that find no expert hold id -1 and weight 0."""
+    Best first, ties in 64 bits to the lower index; without groups, and with no bias or one that is the same for all experts, the
+    logits' own order. Weights are the scores, over their sum with `renormalise`, times `scale`. Logits of -inf or NaN are never
+    chosen; slots that find no expert hold id -1 and weight 0."""
     v = _float_view(logits, dtype, "route")
     if score not in _SCORES:
         raise ValueError(f"score is 'softmax' or 'sigmoid', not {score!r}")

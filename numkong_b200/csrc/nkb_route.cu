@@ -7,7 +7,9 @@
 //
 // A logit of -infinity or NaN masks its expert: it has score 0 and is never chosen. A bias of -infinity or NaN only keeps its
 // expert from being chosen. +infinity counts as the largest finite value. Slots that find no expert get id -1 and weight 0.
-// Which of two near keys is the larger decides who is chosen, so keys are compared in 64 bits.
+// Which of two near keys is the larger decides who is chosen, so keys are compared in 64 bits. Scores grow with their logits: without
+// groups and with no bias, or one that is the same for all experts it does not bar, the logits themselves are compared, which keep
+// their order where 64 bits no longer tell the scores apart (sigmoids of 40 and 50).
 //
 // Gradient, with p the chosen scores, g the incoming gradient times the scale and S their sum:
 //   renormalised   d s_{i_j} = (g_j - sum_i g_i p_i / S) / S,   otherwise d s_{i_j} = g_j
@@ -148,11 +150,10 @@ __device__ __forceinline__ void sort_descending(uint32_t (&v)[kCount]) {
 
 // The choice in 64 bits, for the tokens whose keys 32 bits leave undecided. `keys`: room for one key per expert. Returns lane j's choice.
 template <uint32_t kType>
-__device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, double *keys, int lane) {
-    const bool direct = p.bias == nullptr && p.groups == 1;  // scores grow with their logits
+__device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t *row, bool by_logit, double *keys, int lane) {
     double total = 0.0;
     float top_logit = -INFINITY;
-    if (!p.sigmoid && !direct) {
+    if (!p.sigmoid && !by_logit) {
         for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
         top_logit = warp_max(top_logit);
         for (uint32_t e = lane; e < p.experts; e += 32) {
@@ -163,8 +164,7 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
     }
     for (uint32_t e = lane; e < p.experts; e += 32) {
         const float l = load_logit<kType>(row, e), b = load_bias(p.bias, e);
-        if (direct) keys[e] = l;
-        else keys[e] = l > -INFINITY && b > -INFINITY ? exact_score(p.sigmoid, l, top_logit, total) + b : -INFINITY;
+        keys[e] = !(l > -INFINITY && b > -INFINITY) ? -INFINITY : by_logit ? (double)l : exact_score(p.sigmoid, l, top_logit, total) + b;
     }
     __syncwarp();
     if (p.groups > 1) {
@@ -208,11 +208,10 @@ __device__ __noinline__ int32_t choose_exactly(const RouteDev &p, const uint8_t 
 
 // The `top` best of `count` candidates (one per lane) by their keys in 64 bits, in order, ties to the lower index. Returns lane j's choice.
 template <uint32_t kType>
-__device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *row, int32_t chosen, uint32_t count, int32_t *places, int lane) {
-    const bool direct = p.bias == nullptr && p.groups == 1;
+__device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *row, bool by_logit, int32_t chosen, uint32_t count, int32_t *places, int lane) {
     double total = 1.0;
     float top_logit = 0.0f;
-    if (!direct && !p.sigmoid) {
+    if (!by_logit && !p.sigmoid) {
         top_logit = -INFINITY;
         for (uint32_t e = lane; e < p.experts; e += 32) top_logit = fmaxf(top_logit, load_logit<kType>(row, e));
         top_logit = warp_max(top_logit);
@@ -224,7 +223,7 @@ __device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *
     double key = -INFINITY;
     if (chosen >= 0) {
         const float l = load_logit<kType>(row, chosen);
-        key = direct ? (double)l : exact_score(p.sigmoid, l, top_logit, total) + load_bias(p.bias, chosen);
+        key = by_logit ? (double)l : exact_score(p.sigmoid, l, top_logit, total) + load_bias(p.bias, chosen);
     }
     uint32_t rank = 0;
 #pragma unroll 1
@@ -243,7 +242,8 @@ __device__ __noinline__ int32_t order_exactly(const RouteDev &p, const uint8_t *
 // The choice where the last place is in question: everyone in an open group whose 32-bit key is not below `threshold` takes a lane, and
 // those are put in order in 64 bits. -2 in all lanes where they are more than 32.
 template <uint32_t kType, uint32_t kIndexBits>
-__device__ __noinline__ int32_t choose_near(const RouteDev &p, const uint8_t *row, uint32_t threshold, uint32_t open_groups, float least, float per_key, int32_t *places, int lane) {
+__device__ __noinline__ int32_t choose_near(const RouteDev &p, const uint8_t *row, bool by_logit, uint32_t threshold, uint32_t open_groups, float least, float per_key, int32_t *places,
+                                                int lane) {
     const bool direct = p.bias == nullptr && p.groups == 1;
     const uint32_t size = p.experts / p.groups;
     float top_logit = 0.0f, scaled = per_key;
@@ -273,7 +273,7 @@ __device__ __noinline__ int32_t choose_near(const RouteDev &p, const uint8_t *ro
         if ((uint32_t)lane >= count && (uint32_t)lane < count + many) candidate = (int32_t)(base + __fns(found, 0, lane - count + 1));
         count += many;
     }
-    return order_exactly<kType>(p, row, candidate, count, places, lane);
+    return order_exactly<kType>(p, row, by_logit, candidate, count, places, lane);
 }
 
 // One warp per token; lane i holds the experts i * kPer .. in registers.
@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
     }
     least = -warp_max(-least);
     most = warp_max(most);
+    const bool by_logit = p.groups == 1 && (p.bias == nullptr || __all_sync(0xffffffffu, !(least < most)));
     if (!(least <= most)) least = most = 0.0f;  // every expert is barred
     least = fminf(least, 0.0f);                 // so that a key of 0 is on the scale
     const bool workable = direct || (fabsf(least) < 16.0f && fabsf(most) < 16.0f);  // wider biases leave the scale too coarse
@@ -492,12 +493,12 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
         int32_t chosen = -2;
         if (what == 0xffffffffu) {
             chosen = __shfl_sync(0xffffffffu, chosen_all, t * width + (lane & (width - 1)));
-            chosen = order_exactly<kType>(p, row, lane < (int)p.top ? chosen : -1, p.top, places_all[warp], lane);
+            chosen = order_exactly<kType>(p, row, by_logit, lane < (int)p.top ? chosen : -1, p.top, places_all[warp], lane);
         } else if (what != 0) {
-            chosen = choose_near<kType, kIndexBits>(p, row, what, groups, least, per_key, places_all[warp], lane);
+            chosen = choose_near<kType, kIndexBits>(p, row, by_logit, what, groups, least, per_key, places_all[warp], lane);
         }
         if (__any_sync(0xffffffffu, chosen == -2)) {
-            chosen = choose_exactly<kType>(p, row, keys_all + (size_t)warp * p.experts, lane);
+            chosen = choose_exactly<kType>(p, row, by_logit, keys_all + (size_t)warp * p.experts, lane);
             __syncwarp();
         }
         const int32_t mine_of = __shfl_sync(0xffffffffu, chosen, slot);
@@ -540,8 +541,8 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
 // numerator first (relative to 0 if that is not among the chosen), which leaves the bracket as it is and takes its largest terms out.
 // Bound by the write of the rows and the start: 16,384 x 256 f32, sigmoid, 8 chosen, 5.8 us for 18 MB (2.7 us at the copy rate); 16,384 x 64
 // bf16, softmax renormalised, 6 chosen, 4.1 us; 16 tokens 3.2 us. Softmax without renormalisation, which reads every logit: 16,384 x 256
-// 14.0 us, 16,384 x 64 8.8 us (8.1 us with the subtraction of two 32-bit values, which lost what nearly cancels: half of a chosen logit's
-// gradient and more where it lies 20 above the others).
+// 14.0 us, 16,384 x 64 8.8 us (8.1 us with the subtraction of two 32-bit values, which lost what nearly cancels: a fifth of a chosen logit's
+// gradient where it lies 18 above the others, all of it from 22 on).
 template <uint32_t kType>
 __global__ void __launch_bounds__(kWarps * 32) route_gradient_kernel(const RouteDev p, const float *weights_grad, const int32_t *ids, float *logits_grad) {
     extern __shared__ float rows_all[];
