@@ -161,8 +161,8 @@ ExpertsLayout experts_layout(uint64_t slots, uint64_t experts, uint64_t width, u
     return l;
 }
 
-// A . B^T with A already in `chunks` or, when `codes` is null, quantised from `a` on its way there.
-void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *codes, uint64_t codes_stride, const void *scales, uint64_t scales_stride,
+// A . B^T with A given as codes and scales or, unless `coded`, as floats that are quantised on their way.
+void product(bool coded, const void *a, uint32_t a_type, uint64_t a_stride, const void *codes, uint64_t codes_stride, const void *scales, uint64_t scales_stride,
              const void *packed, void *c, uint32_t c_type, uint64_t m, uint64_t n, uint64_t k, uint64_t c_stride, void *workspace) {
     clear_error();
     if (m == 0 || n == 0) return;
@@ -170,12 +170,12 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     const uint32_t cell = dtype_bytes(c_type);
     const uint64_t row_bytes = n * cell;
     auto fail = [&]() { spoil(c, m, row_bytes, c_stride); };
-    if ((c_type != kF32 && c_type != kBF16) || (!codes && !float_type(a_type))) { refuse("mxfp4 product: unsupported element type"); return fail(); }
-    if (!packed || !c || (k && !(codes ? scales != nullptr : a != nullptr))) { refuse("mxfp4 product: null pointer"); return fail(); }
+    if ((c_type != kF32 && c_type != kBF16) || (!coded && !float_type(a_type))) { refuse("mxfp4 product: unsupported element type"); return fail(); }
+    if (!packed || !c || (k && !(coded ? codes && scales : a != nullptr))) { refuse("mxfp4 product: null pointer"); return fail(); }
     if ((m > 1 && c_stride < row_bytes) || (reinterpret_cast<uintptr_t>(c) | (m > 1 ? c_stride : 0)) % cell) { refuse("mxfp4 product: rows of the result overlap or are not aligned to its cells"); return fail(); }
     const uint64_t kblocks = (k + kMxBlock - 1) / kMxBlock;
-    if (m > 1 && (codes ? codes_stride < (k + 1) / 2 || scales_stride < kblocks : a_stride < k * dtype_bytes(a_type))) { refuse("mxfp4 product: rows of A overlap"); return fail(); }
-    if (!codes && (reinterpret_cast<uintptr_t>(a) | (m > 1 ? a_stride : 0)) % dtype_bytes(a_type)) { refuse("mxfp4 product: values of A are not aligned to their type"); return fail(); }
+    if (m > 1 && (coded ? codes_stride < (k + 1) / 2 || scales_stride < kblocks : a_stride < k * dtype_bytes(a_type))) { refuse("mxfp4 product: rows of A overlap"); return fail(); }
+    if (!coded && (reinterpret_cast<uintptr_t>(a) | (m > 1 ? a_stride : 0)) % dtype_bytes(a_type)) { refuse("mxfp4 product: values of A are not aligned to their type"); return fail(); }
     if (m == 1) c_stride = round_up(row_bytes, 16);  // whatever it was: nothing lies that far
     cudaStream_t stream = current_stream();
     Operands ops(stream);
@@ -190,13 +190,13 @@ void product(const void *a, uint32_t a_type, uint64_t a_stride, const void *code
     bool ok = c_dev != nullptr;
     if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_pitch, 0, row_bytes, m, stream), "clear result");
     else if (ok) {
-        const bool inside = !codes && gemm_mx_quantises(m);
+        const bool inside = !coded && gemm_mx_quantises(m);
         uint8_t *chunks = inside ? nullptr : workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
         ok = inside || chunks;
         bool rows_in_place = false;
         const uint8_t *ad = nullptr;
         const uint8_t *cd = nullptr;
-        if (ok && codes) {
+        if (ok && coded) {
             cd = ops.in(codes, m, (k + 1) / 2, codes_stride);
             const uint8_t *sd = cd ? ops.in(scales, m, kblocks, scales_stride) : nullptr;
             if (m == 1) codes_stride = round_up((k + 1) / 2, 16);
@@ -327,18 +327,12 @@ NKB_API nk_size_t nkb_dots_workspace_mxfp4(nk_size_t height, nk_size_t depth) { 
 
 NKB_API void nkb_dots_packed_mxfp4(void const *codes, nk_size_t codes_stride, void const *scales, nk_size_t scales_stride, void const *b_packed,
                                    void *c, uint32_t c_type, nk_size_t height, nk_size_t width, nk_size_t depth, nk_size_t c_stride, void *workspace) {
-    if (!codes) {
-        clear_error();
-        refuse("mxfp4 product: null pointer");
-        if (width <= kMostRows) spoil(c, height, width * dtype_bytes(c_type), c_stride);
-        return;
-    }
-    product(nullptr, 0, 0, codes, codes_stride, scales, scales_stride, b_packed, c, c_type, height, width, depth, c_stride, workspace);
+    product(true, nullptr, 0, 0, codes, codes_stride, scales, scales_stride, b_packed, c, c_type, height, width, depth, c_stride, workspace);
 }
 
 NKB_API void nkb_dots_packed_quantised_mxfp4(void const *a, uint32_t a_type, nk_size_t a_stride, void const *b_packed, void *c, uint32_t c_type,
                                              nk_size_t height, nk_size_t width, nk_size_t depth, nk_size_t c_stride, void *workspace) {
-    product(a, a_type, a_stride, nullptr, 0, nullptr, 0, b_packed, c, c_type, height, width, depth, c_stride, workspace);
+    product(false, a, a_type, a_stride, nullptr, 0, nullptr, 0, b_packed, c, c_type, height, width, depth, c_stride, workspace);
 }
 
 NKB_API void nkb_route(void const *logits, uint32_t type, nk_size_t tokens, nk_size_t experts, nk_size_t logits_stride, float const *bias,
