@@ -312,7 +312,9 @@ NKB_API int nkb_angulars_packed_noalloc(uint32_t dtype, void const *a, void cons
  * `workspace` is device memory of at least the stated size on a 256-byte boundary that no other call uses at the same time; with
  * NULL the calling thread's staging memory is used, which allocates on first use and is shared by everything the thread
  * enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own,
- * for as long as it may run. (Products of one or two float rows need none: they quantise inside.) The first product on each GPU
+ * for as long as it may run. (Products of one or two float rows need none: they quantise inside, unless
+ * C lies over A.) C may lie over a float A, and an experts' result may take the place of their float rows, cell for cell; no output may
+ * overlap another operand. The first product on each GPU
  * allocates the device error word; make it before a capture starts.
  *
  * nkb_mx_quantise: per block with largest magnitude t the scale is 2^X, X = clamp(floor(log2 t) - 2, -127, 127); each value over

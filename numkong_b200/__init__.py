@@ -851,7 +851,8 @@ def _packed_mx(a: Any, packed: PackedMatrix, out: Any, dtype: Optional[str], out
     x = v.codes if isinstance(v, MxMatrix) else v.obj
     place = _place(x, packed)
     result, stride = _mx_result(x, v.rows, packed.width, out, out_dtype)
-    if isinstance(v, MxMatrix) or v.rows > 2:  # one or two float rows are quantised inside the product
+    # One or two float rows are quantised inside the product, unless the result takes their place.
+    if isinstance(v, MxMatrix) or v.rows > 2 or out is not None:
         workspace, ws = _workspace(place, (v.rows + 127) // 128 * ((depth + 255) // 256) * 17408)  # nkb_dots_workspace_mxfp4
     else:
         workspace = ws = None

@@ -190,11 +190,17 @@ void product(bool coded, const void *a, uint32_t a_type, uint64_t a_stride, cons
     bool ok = c_dev != nullptr;
     if (ok && k == 0) ok = cuda_ok(cudaMemset2DAsync(c_dev, c_pitch, 0, row_bytes, m, stream), "clear result");
     else if (ok) {
-        const bool inside = !coded && gemm_mx_quantises(m);
-        uint8_t *chunks = inside ? nullptr : workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
-        ok = inside || chunks;
-        bool rows_in_place = false;
         const uint8_t *ad = nullptr;
+        if (!coded) {
+            ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
+            ok = ad != nullptr;
+        }
+        // A that the product quantises itself is read until its last CTA is through, so C may not lie over it.
+        const uint64_t a_span = (m - 1) * a_stride + k * dtype_bytes(a_type), c_span = (m - 1) * c_pitch + row_bytes;
+        const bool inside = !coded && gemm_mx_quantises(m) && !(c_dev < ad + a_span && ad < c_dev + c_span);
+        uint8_t *chunks = !ok || inside ? nullptr : workspace_or_scratch(ops, workspace, chunk_bytes(m, k));
+        ok = ok && (inside || chunks);
+        bool rows_in_place = false;
         const uint8_t *cd = nullptr;
         if (ok && coded) {
             cd = ops.in(codes, m, (k + 1) / 2, codes_stride);
@@ -203,10 +209,8 @@ void product(bool coded, const void *a, uint32_t a_type, uint64_t a_stride, cons
             rows_in_place = sd && gemm_mx_reads_rows(m, n, k) && ((reinterpret_cast<uintptr_t>(cd) | codes_stride) & 15u) == 0;
             if (rows_in_place) ok = cuda_ok(launch_mx_tile_scales(sd, scales_stride, m, k, chunks, stream), "scale tile kernel");
             else ok = sd && cuda_ok(launch_mx_tile(cd, codes_stride, sd, scales_stride, 1, m, k, false, chunks, stream), "tile kernel");
-        } else if (ok) {
-            ad = ops.in(a, m, k * dtype_bytes(a_type), a_stride);
-            ok = ad != nullptr;
-            if (ok && !inside) ok = cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 0, 1, chunks, stream), "quantise kernel");
+        } else if (ok && !inside) {
+            ok = cuda_ok(launch_mx_quantise_tiled(a_type, ad, k, m > 1 ? a_stride : 0, m, nullptr, nullptr, 0, 1, chunks, stream), "quantise kernel");
         }
         if (ok) {
             MxGemmArgs args;
