@@ -107,15 +107,18 @@ void refuse(const char *why) { set_error("%s", why); }
 
 constexpr uint64_t kMostRows = 0x7fffff00ull;  // indices inside the kernels are 32 bits wide
 
-// What an output holds after a refused or failed call: 0xFF bytes (NaN scales and cells, ids of -1), no more of them than the caller's
-// sizes and stride span. Sizes that no kernel takes are not believed.
-void spoil(void *out, uint64_t rows, uint64_t row_bytes, uint64_t stride) {
-    if (!out || rows == 0 || rows > kMostRows || row_bytes > 4 * kMostRows) return;
+bool on_another_gpu(const void *p) {
     cudaPointerAttributes attr;
     int device = 0;
     cudaGetDevice(&device);
-    if (cudaPointerGetAttributes(&attr, out) != cudaSuccess) cudaGetLastError();
-    else if (attr.type == cudaMemoryTypeDevice && attr.device != device) return;  // another GPU's memory is left alone
+    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) { cudaGetLastError(); return false; }
+    return attr.type == cudaMemoryTypeDevice && attr.device != device;
+}
+
+// What an output holds after a refused or failed call: 0xFF bytes (NaN scales and cells, ids of -1), no more of them than the caller's
+// sizes and stride span. Sizes that no kernel takes are not believed, another GPU's memory is left alone.
+void spoil(void *out, uint64_t rows, uint64_t row_bytes, uint64_t stride) {
+    if (!out || rows == 0 || rows > kMostRows || row_bytes > 4 * kMostRows || on_another_gpu(out)) return;
     if (stride < row_bytes) fill_error_output(out, classify(out), 1, (rows - 1) * stride + row_bytes, (rows - 1) * stride + row_bytes);
     else fill_error_output(out, classify(out), rows, row_bytes, stride);
 }
@@ -291,7 +294,7 @@ NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void
     const MxGeometry g = mx_geometry(groups, width, depth);
     const uint64_t rows = groups * width, code_bytes = (depth + 1) / 2, blocks = (depth + kMxBlock - 1) / kMxBlock;
     const MemKind out_kind = classify(packed);
-    auto fail = [&]() { fill_error_output(packed, out_kind, 1, g.total_bytes, g.total_bytes); };
+    auto fail = [&]() { if (!on_another_gpu(packed)) fill_error_output(packed, out_kind, 1, g.total_bytes, g.total_bytes); };
     if (rows && depth && (!codes || !scales)) { refuse("mxfp4 pack: null input"); return fail(); }
     if (rows > 1 && (codes_stride < code_bytes || scales_stride < blocks)) { refuse("mxfp4 pack: rows overlap"); return fail(); }
     if (out_kind == kMemDevice && (reinterpret_cast<uintptr_t>(packed) & 15u)) { refuse("pack: device output must be 16-byte aligned"); return; }
@@ -304,7 +307,7 @@ NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void
     cudaStream_t stream = current_stream();
     Operands ops(stream);
     MemKind looked;
-    if (!ops.look(packed, looked)) return;
+    if (!ops.look(packed, looked)) return fail();
     uint8_t *blob = static_cast<uint8_t *>(packed);
     if (out_kind == kMemHost) {
         void *d = nullptr;
