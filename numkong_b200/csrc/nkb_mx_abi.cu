@@ -297,7 +297,7 @@ NKB_API void nkb_dots_pack_mxfp4(void const *codes, nk_size_t codes_stride, void
     auto fail = [&]() { if (!on_another_gpu(packed)) fill_error_output(packed, out_kind, 1, g.total_bytes, g.total_bytes); };
     if (rows && depth && (!codes || !scales)) { refuse("mxfp4 pack: null input"); return fail(); }
     if (rows > 1 && (codes_stride < code_bytes || scales_stride < blocks)) { refuse("mxfp4 pack: rows overlap"); return fail(); }
-    if (out_kind == kMemDevice && (reinterpret_cast<uintptr_t>(packed) & 15u)) { refuse("pack: device output must be 16-byte aligned"); return; }
+    if (out_kind == kMemDevice && (reinterpret_cast<uintptr_t>(packed) & 15u)) { refuse("pack: device output must be 16-byte aligned"); return fail(); }
     PackedHeader h;
     std::memset(&h, 0, sizeof h);
     h.magic = kMagicMx; h.dtype = kMxfp4; h.element_bytes = 1; h.norm_bytes = 0;

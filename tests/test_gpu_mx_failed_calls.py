@@ -87,3 +87,14 @@ def test_a_refused_workspace(pad):
         for held in outputs:
             assert held.spoilt(), name
     assert nk.synchronize() == 0
+
+
+def test_a_pack_to_a_misaligned_address():
+    size = lib.nkb_dots_packed_size_mxfp4(1, WIDTH, DEPTH)
+    room = torch.zeros(size + 64, dtype=torch.uint8, device="cuda")
+    q = operands()[1]
+    lib.nkb_dots_pack_mxfp4(p(q.codes), 35, p(q.scales), 3, 1, ROWS, DEPTH, room.data_ptr() + 8)
+    assert "aligned" in nk.last_error()
+    torch.cuda.synchronize()
+    assert (room[8:8 + size] == 255).all() and (room[:8] == 0).all() and (room[8 + size:] == 0).all()
+    assert nk.synchronize() == 0
