@@ -762,16 +762,22 @@ def _float_view(x: Any, dtype: Optional[str], what: str) -> _View:
 
 class MxMatrix:
     """A matrix of microscaled 4-bit floats in row-major form: `codes` (rows x ceil(depth / 2) bytes, two e2m1 codes each, the
-    even value in the low half) and `scales` (rows x ceil(depth / 32) bytes, 2^(s - 127) for 32 values of a row, 255 = NaN)."""
+    even value in the low half) and `scales` (rows x ceil(depth / 32) bytes, 2^(s - 127) for 32 values of a row, 255 = NaN). Its parts
+    can be written to but not exchanged: the calls read from where they were when it was made."""
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    rows = property(lambda self: self._rows)
+    depth = property(lambda self: self._depth)
 
     def __init__(self, codes: Any, scales: Any, depth: int):
-        self.depth = int(depth)
+        self._depth = depth = int(depth)
         c, s = _View(_array(codes), "u8"), _View(_array(scales), "u8")
-        if c.cols != (self.depth + 1) // 2 or s.cols != (self.depth + 31) // 32 or c.rows != s.rows:
-            raise ValueError(f"depth {self.depth} needs rows of {(self.depth + 1) // 2} code bytes and {(self.depth + 31) // 32} scale bytes")
+        if c.cols != (depth + 1) // 2 or s.cols != (depth + 31) // 32 or c.rows != s.rows:
+            raise ValueError(f"depth {depth} needs rows of {(depth + 1) // 2} code bytes and {(depth + 31) // 32} scale bytes")
         if _is_torch(c.obj) != _is_torch(s.obj) or (_is_torch(c.obj) and c.obj.device != s.obj.device):
             raise ValueError("codes and scales must live in the same place")
-        self.codes, self.scales, self.rows = c.obj, s.obj, c.rows
+        self._codes, self._scales, self._rows = c.obj, s.obj, c.rows
         self._parts = c.ptr, c.stride, s.ptr, s.stride
 
     @classmethod
@@ -779,9 +785,12 @@ class MxMatrix:
         """Of uninitialised dense arrays where `like` lives."""
         self = cls.__new__(cls)
         width, blocks = (depth + 1) // 2, (depth + 31) // 32
-        self.codes, self.scales, self.rows, self.depth = _like(like, (rows, width), "u8"), _like(like, (rows, blocks), "u8"), rows, depth
-        self._parts = _ptr(self.codes), width, _ptr(self.scales), blocks
+        self._codes, self._scales, self._rows, self._depth = _like(like, (rows, width), "u8"), _like(like, (rows, blocks), "u8"), rows, depth
+        self._parts = _ptr(self._codes), width, _ptr(self._scales), blocks
         return self
+
+    def __reduce__(self):  # copies and pickles are made anew, with addresses of their own
+        return MxMatrix, (self._codes, self._scales, self._depth)
 
     @property
     def is_cuda(self) -> bool:
