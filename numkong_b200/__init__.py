@@ -158,7 +158,7 @@ class _View:
             self.obj = x
             if x.ndim != 2:
                 raise ValueError("expected a 2-D matrix")
-            if x.shape[1] > 1 and x.strides[1] != x.itemsize:
+            if x.size and x.shape[1] > 1 and x.strides[1] != x.itemsize:  # NumPy gives an array without values strides of 0
                 raise ValueError("rows must be contiguous (column-major inputs are not supported)")
             name = dtype or _NUMPY_NAMES.get(x.dtype.name)
             if name is None:
