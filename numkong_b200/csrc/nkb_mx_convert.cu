@@ -112,9 +112,9 @@ __device__ __forceinline__ void quantise_piece(const uint8_t *row, const Piece &
 #pragma unroll
             for (int h = 0; h < kBytes / 2; ++h) {
                 raw[u][h] = make_uint4(0, 0, 0, 0);
-                if (first + 8 <= depth) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(row + first * kBytes) + h);
+                if (u < (int)ahead && first + 8 <= depth) raw[u][h] = __ldg(reinterpret_cast<const uint4 *>(row + first * kBytes) + h);
             }
-            if (first < depth && first + 8 > depth) {  // the row ends inside
+            if (u < (int)ahead && first < depth && first + 8 > depth) {  // the row ends inside
                 uint32_t w[2 * kBytes] = {};
                 for (int i = 0; i < (int)(depth - first); ++i) {
                     if constexpr (kType == kF32) w[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + first + i);
@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
             for (int u = 0; u < kAhead; ++u) {
                 const uint64_t byte = (uint64_t)(piece.kb0 + u) * 128 + lane * 4;
                 w[u] = 0;
+                if (u >= (int)ahead) continue;
                 if (byte + 4 <= row_bytes) w[u] = __ldg(reinterpret_cast<const uint32_t *>(row + byte));
                 else
                     for (int i = 0; i < 4; ++i)
@@ -368,6 +369,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const uint8_t *cod
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
+                if (u >= (int)ahead) break;  // the next warps' chunk rows
                 const float scale = scale_value(__shfl_sync(0xffffffffu, my_scale, u * 8 + (lane >> 2)));
                 const uint64_t first = (uint64_t)(piece.kb0 + u) * kMxChunkValues + lane * 8;
                 uint32_t out[2 * kBytes];
