@@ -6,8 +6,10 @@
 // tcgen05.mma.kind::mxf4 takes 64 values of depth a step and applies the scales inside: the scales come from TMEM. Four warps,
 // one for each 32-lane quarter, bring a chunk's scale tiles there through registers (tcgen05.st) beside the MMAs. tcgen05.cp would
 // bring them from shared memory in one instruction, but runs in the queue of the MMAs and costs them about 46 cycles a tile.
-// e2m1 products are multiples of 1/4 of at most 36, so a block's sum is exact and the accumulator only loses bits when the
-// block scales of a row spread over more than 2^10.
+// e2m1 products are multiples of 1/4 of at most 36, so the sum of a block of 32 is a multiple of 1/4 of at most 1152 and exact. Over the
+// depth the f32 accumulator holds 2^24 of the smallest block's quarters: sums stay exact while 4608 times the blocks times the ratio of
+// the largest to the smallest product of scales stays below that, at worst a ratio of 2^3 at a depth of 8192; beyond, each step adds the
+// roundings of an f32 sum.
 //
 // One persistent CTA per SM: warp 0 brings B to shared memory with untiled bulk copies and warp 14 brings A, warp 1 issues the MMAs,
 // warps 2..9 read the accumulators out and store the cells, warps 10..13 store scales.
@@ -236,14 +238,9 @@ __device__ __forceinline__ uint32_t quantise_row8(const uint4 (&raw)[2], uint32_
     return quantise8(v, largest, scale);
 }
 
-// How kOwnA shares the chunks out: `width` warps, two rows each, work on one chunk, so that `sets` chunks are in hand at a time.
-struct OwnShare {
-    uint32_t width, sets;
-    __host__ __device__ explicit OwnShare(uint32_t m) : width((m + 1) / 2), sets(kEpilogueWarps / ((m + 1) / 2)) {}
-};
-
-// With kOwnA the epilogue warps quantise A's few rows chunk by chunk into the rings while the packed matrix streams in: one launch
-// and no workspace, at the price of every CTA doing it again.
+// With kOwnA the epilogue warps quantise A's one or two rows into the rings while the packed matrix streams in, every eighth chunk each:
+// one launch and no workspace, at the price of every CTA doing it again.
+constexpr uint32_t kOwnRows = 2;
 template <int kBN, int kARows, bool kOwnA, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p) {
     using P = Plan<kBN, kARows>;
@@ -269,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        // A stage is full when B's loader, A's loader or quantisers and the scale warps have arrived.
-        const uint32_t fillers = (kOwnA ? 1 + OwnShare(p.m).width : 2) + kScaleWarps;
+        // A stage is full when B's loader, A's loader or quantiser and the scale warps have arrived.
+        constexpr uint32_t fillers = 2 + kScaleWarps;
         for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), fillers); mbar_init(empty_bar(s), 1); }
         for (uint32_t g = 0; g < kScaleRing; ++g) { mbar_init(scale_full_bar(g), kOwnA ? 1 + kEpilogueWarps : 2); mbar_init(scale_empty_bar(g), kScaleWarps); }
         for (int a = 0; a < 2; ++a) { mbar_init(tmem_full_bar(a), 1); mbar_init(tmem_empty_bar(a), kEpilogueWarps * 32); }
@@ -410,36 +407,34 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_mx_kernel(const MxGemmDev p)
         int stage = 0;
         for (Walk<kBM> w(p, blockIdx.x, gridDim.x, tiles_m); w.valid(); w.next_tile(), ++seq) {
             if constexpr (kOwnA) {
-                const OwnShare share(p.m);
-                const uint32_t me = (uint32_t)warp - 2u, row0 = me % share.width * 2u, set = me / share.width;
+                constexpr uint32_t kSets = kEpilogueWarps;
+                const uint32_t set = (uint32_t)warp - 2u;
                 auto own = [&](auto type) {
                     constexpr uint32_t kType = decltype(type)::value;
-                    uint4 raw[2][2];
+                    uint4 raw[kOwnRows][2];
                     auto fetch = [&](uint32_t kb) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            if (row0 + h < p.m && kb < p.kblocks) load_row8<kType>(p, row0 + h, kb * kMxChunkValues + lane * 8, raw[h]);
+                        for (uint32_t r = 0; r < kOwnRows; ++r)
+                            if (r < p.m && kb < p.kblocks) load_row8<kType>(p, r, kb * kMxChunkValues + lane * 8, raw[r]);
                     };
-                    // This warp's first chunk of the tile is the first that its set is due for.
-                    if (set < share.sets) fetch((set + share.sets - chunk % share.sets) % share.sets);
+                    fetch((set + kSets - chunk % kSets) % kSets);  // the first chunk of the tile that is this warp's
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++chunk) {
                         const uint32_t in_group = kb % kScaleGroup;
                         bool ok = in_group != 0 || mbar_wait(scale_empty_bar(group), group_phase ^ 1u, 1, p.error_word, p.wait_us[1]);
-                        const bool mine = chunk % share.sets == set;
+                        const bool mine = chunk % kSets == set;
                         if (ok && mine) ok = mbar_wait(empty_bar(stage), phase ^ 1u, 1, p.error_word, p.wait_us[1]);
                         if (!__all_sync(0xffffffffu, ok)) return false;
                         if (mine) {
                             uint8_t *codes = smem_gen + stage * P::kABytes, *scales = smem_gen + P::kScaleOffset + (2 * group * kScaleGroup + in_group) * kMxScaleBytes;
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t r = row0 + h;
+                            for (uint32_t r = 0; r < kOwnRows; ++r) {
                                 if (r >= p.m) continue;
                                 uint32_t s;
-                                const uint32_t word = quantise_row8<kType>(raw[h], s);
+                                const uint32_t word = quantise_row8<kType>(raw[r], s);
                                 *reinterpret_cast<uint32_t *>(codes + r * 128u + ((((uint32_t)lane >> 2) ^ (r & 7u)) << 4) + (lane & 3) * 4) = word;
                                 if ((lane & 3) == 0) scales[(lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)s;
                             }
-                            fetch(kb + share.sets);
+                            fetch(kb + kSets);
                             fence_proxy_async_smem();  // the MMA reads the codes through the other proxy
                             __syncwarp();
                             if (lane == 0) mbar_arrive(full_bar(stage));
@@ -832,9 +827,9 @@ bool gemm_mx_reads_rows(uint64_t m, uint64_t n, uint64_t) {
     return m > kBM && ((m + 255) / 256) * ((n + 255) / 256) >= (uint64_t)sm_count() / 3;
 }
 
-// Every CTA quantises the rows again, and with more than two the loads of a chunk's rows no longer lie eight chunks ahead:
-// 8 x 8192 x 8192 took 22.8 us inside and 13.5 us after the separate kernel, 1 x 4096 x 4096 takes 9.4 us inside with one launch less.
-bool gemm_mx_quantises(uint64_t m) { return m <= 2; }
+// Every CTA quantises the rows again, and with more than two a chunk took several warps, so that its loads no longer lay eight chunks ahead:
+// 8 x 8192 x 8192 took 22.8 us inside and takes 13.2 us with a kernel before it; 1 x 4096 x 4096 takes 8.8 us inside, one launch.
+bool gemm_mx_quantises(uint64_t m) { return m <= kOwnRows; }
 
 cudaError_t launch_gemm_mx(const MxGemmArgs &args, cudaStream_t stream) {
     if (args.m == 0 || args.n == 0) return cudaSuccess;
