@@ -463,7 +463,17 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 4 ? 8 : kPer == 8 ? 7 : k
         };
         const uint32_t before = __shfl_up_sync(0xffffffffu, word, 1);
         bool ordered = !__any_sync(0xffffffffu, lane > 0 && undecided(before, word));
-        if (p.top == 32) ordered = ordered && !undecided(__shfl_sync(0xffffffffu, word, 31), behind);
+        // A tie of the last one chosen may hide others behind it that are near and not a tie. (Keys that are 16-bit logits are exact.)
+        if (kType == kF32 || !direct) {
+            const bool edge = p.top == 32 ? behind != 0 : lane == (int)p.top && word != 0 && (before >> kIndexBits) - (word >> kIndexBits) <= unsure_at;
+            if (__any_sync(0xffffffffu, edge) && ordered) {
+                const uint32_t last_word = __shfl_sync(0xffffffffu, word, p.top - 1);
+                bool near = p.top == 32 && undecided(last_word, behind);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) near = near || undecided(last_word, key[i]);
+                ordered = !__any_sync(0xffffffffu, near);
+            }
+        }
         int32_t chosen = word != 0 && lane < (int)p.top ? (int32_t)expert_of(word) : -1;
         if (!sure || !ordered) {
             const uint32_t last = __shfl_sync(0xffffffffu, word, p.top - 1) >> kIndexBits;
