@@ -311,16 +311,16 @@ NKB_API int nkb_angulars_packed_noalloc(uint32_t dtype, void const *a, void cons
  * and cells and ids of -1, as far as sizes and strides span (not where a size itself is refused: 2^31 and more; nor on another GPU).
  * `workspace` is device memory of at least the stated size on a 256-byte boundary that no other call uses at the same time; with
  * NULL the calling thread's staging memory is used, which allocates on first use and is shared by everything the thread
- * enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own,
- * for as long as it may run. (Products of one or two float rows need none: they quantise inside, unless
- * C lies over A.) C may lie over a float A, and an experts' result may take the place of their float rows, cell for cell; no output may
- * overlap another operand. The first product on each GPU
+ * enqueues. While the stream is being captured NULL is refused: a graph needs a workspace of its own, for as long as it may run.
+ * (Products of one or two float rows need none: they quantise inside, unless C lies over A.) C may lie over a float A, and an experts'
+ * result may take the place of their float rows, cell for cell; no output may overlap another operand. The first product on each GPU
  * allocates the device error word; make it before a capture starts.
  *
  * nkb_mx_quantise: per block with largest magnitude t the scale is 2^X, X = clamp(floor(log2 t) - 2, -127, 127); each value over
  *   it is rounded to the nearest code, ties to the even code, beyond 6 to 6. A block that holds an infinity or a NaN gets scale 255
  *   and zero codes. The unused half of the last byte of an odd depth is a zero code.
- * nkb_mx_dequantise: the values the codes stand for (f16: rounded to nearest, beyond its range infinite).
+ * nkb_mx_dequantise: the values the codes stand for, exact in f32 and bf16 but for scale bytes of 253 and 254, whose larger values are
+ *   beyond their range and become infinite (quantising gives none above 252); f16: rounded to nearest, beyond its range infinite.
  * nkb_dots_pack_mxfp4: `groups` matrices of width x depth, one after the other in rows, into one blob of
  *   nkb_dots_packed_size_mxfp4 bytes; groups = 1 is a plain packed matrix, more are the matrices of nkb_experts_packed_mxfp4.
  * nkb_dots_packed_mxfp4: C = A . B^T in f32 sums, stored as f32 or rounded to bf16. A is row-major codes and scales; the
@@ -350,6 +350,7 @@ NKB_API void nkb_dots_packed_quantised_mxfp4(void const *a, uint32_t a_type, nk_
  * Keys are compared in 64 bits; without groups and with no bias, or one that is the same for all experts it does not bar, that is the
  * order of the logits, which decide also where their scores have become equal in 64 bits. A logit of -infinity or NaN gives
  * score 0 and is never chosen, a bias of -infinity or NaN only bars its expert, +infinity counts as the largest finite value. Slots left without an expert hold id -1 and weight 0.
+ * Weights are within 8 half steps of f32 of their value, gradients within 16 of the sum of their terms' magnitudes.
  * weights and ids are dense [tokens, top]. `logits` rows are `logits_stride` bytes apart.
  * nkb_route_gradient: d(sum of weights * weights_grad) / d logits for given ids, dense f32 [tokens, experts]; ids outside
  * [0, experts) and experts whose logit is masked get and give nothing, an id named twice counts twice. */

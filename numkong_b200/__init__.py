@@ -646,6 +646,8 @@ def merge_topk(values: Any, ids: Any, top: Optional[int] = None):
 
 
 # ---- microscaled 4-bit floats, routing and the experts' products -----------------------------------------------------
+# These calls run on torch's current stream where an operand is a CUDA tensor and the thread has not chosen another with set_stream. All
+# other entry points run on the thread's own stream: on a side stream of torch's, choose it with set_stream to chain them.
 _thread = threading.local()  # .stream: what this thread gave set_stream
 
 
@@ -812,7 +814,7 @@ def mx_quantise(x: Any, *, dtype: Optional[str] = None) -> MxMatrix:
 
 
 def mx_dequantise(q: MxMatrix, to_dtype: str = "f32"):
-    """The values an MxMatrix stands for, as f32, bf16 (both exact) or f16 (nkb_mx_dequantise)."""
+    """The values an MxMatrix stands for, as f32, bf16 (both exact as far as they reach) or f16 (nkb_mx_dequantise)."""
     if not isinstance(q, MxMatrix):
         raise TypeError("mx_dequantise takes an MxMatrix")
     if to_dtype not in ("f32", "f16", "bf16"):

@@ -14,6 +14,9 @@
 // Gradient, with p the chosen scores, g the incoming gradient times the scale and S their sum:
 //   renormalised   d s_{i_j} = (g_j - sum_i g_i p_i / S) / S,   otherwise d s_{i_j} = g_j
 //   softmax        d l_e = s_e (d s_e - sum_i d s_i s_i),       sigmoid d l_e = s_e (1 - s_e) d s_e
+//
+// Exponentials of scores that are given out are taken in 32 bits (off by three half steps at most, the rounding of their argument made good
+// for) and summed in 64: a weight is within 8 half steps of f32 of its value, a gradient within 16 of the sum of its terms' magnitudes.
 #include <cfloat>
 #include "nkb_decode.cuh"
 #include "nkb_mx.h"
@@ -285,10 +288,11 @@ __device__ __noinline__ int32_t choose_near(const RouteDev &p, const uint8_t *ro
 // be chosen are put in order in 64 bits, or, where groups are in question, the whole choice is made there (choose_exactly). Keys that are the logits themselves (no bias, no groups) are the upper bits of their
 // order-preserving integers, exact for 16-bit logits.
 //
-// 64 bits wait until a warp's batch is through: with the calls inside the loop its registers went to the stack around them.
+// 64 bits wait until a warp's batch is through: with the calls inside the loop its registers went to the stack around them. (At these
+// register bounds up to 44 bytes a thread still do, for up to eight keys a lane.)
 //
 // 16,384 tokens x 256 experts, sigmoid, 4 of 8 groups, 8 chosen: 73 us with every token in 64 bits, 38 us with 32-bit keys whose expert was
-// looked up in every round, 26 us now. 19 of these are about 700 instructions a token, a third of what the SMs can issue (the chain
+// looked up in every round, 26 to 27 us now. 19 of these are about 700 instructions a token, a third of what the SMs can issue (the chain
 // of one maximum after the other; more warps with fewer registers each were no faster); the rest is the last warps' way through 64 bits.
 // Register bounds: 72 instead of 96 for eight keys a lane took 24 us to 20 without the 64-bit part, 64 was slower again.
 template <uint32_t kType, int kPer>
