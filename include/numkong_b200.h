@@ -349,7 +349,8 @@ NKB_API void nkb_dots_packed_quantised_mxfp4(void const *a, uint32_t a_type, nk_
  *   weights[token, j] = scale * s, or scale * s / (sum over the chosen) with `renormalise`
  * Keys are compared in 64 bits; without groups and with no bias, or one that is the same for all experts it does not bar, that is the
  * order of the logits, which decide also where their scores have become equal in 64 bits. A logit of -infinity or NaN gives
- * score 0 and is never chosen, a bias of -infinity or NaN only bars its expert, +infinity counts as the largest finite value. Slots left without an expert hold id -1 and weight 0.
+ * score 0 and is never chosen, a bias of -infinity or NaN only bars its expert, +infinity counts as the largest finite value. Slots
+ * left without an expert hold id -1 and weight 0.
  * Weights are within 8 half steps of f32 of their value, gradients within 16 of the sum of their terms' magnitudes.
  * weights and ids are dense [tokens, top]. `logits` rows are `logits_stride` bytes apart.
  * nkb_route_gradient: d(sum of weights * weights_grad) / d logits for given ids, dense f32 [tokens, experts]; ids outside
